@@ -235,6 +235,49 @@ hipError_t launch_canonical_pack(const void* src, void* dst, int64_t elements, i
 hipError_t launch_bool_validate(const void* src, int64_t elements, const CanonicalGeometry& g,
                                 uint32_t* status, hipStream_t s);
 
+// Microscaled tensors (mx.h): codes of 8 or 4 bits, one power of two for 32 values of a row.
+enum MxFormatId : int { MX_E4M3 = 0, MX_E5M2 = 1, MX_E2M1 = 2 };
+// Encodes x [R, C] (row stride ldx); keep_nonzero (8-bit formats): a nonzero value's code is never
+// zero.
+hipError_t launch_mx_encode(const float* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t R,
+                            int64_t C, int format, int keep_nonzero, hipStream_t s);
+// y [R, C] (row stride ldy) = the values that codes and scales stand for.
+hipError_t launch_mx_decode(const uint8_t* codes, const uint8_t* scales, float* y, int64_t ldy,
+                            int64_t R, int64_t C, int format, hipStream_t s);
+// dz = act_grad(act, dy, y) with the activation output y from its codes, and optionally the
+// column sums of dz; dy and dz may be the same memory. `partial` holds at least
+// mx_act_grad_partial_doubles(R, C) doubles when colsum is set.
+hipError_t launch_mx_act_grad(const float* dy, int64_t ldy, const uint8_t* codes,
+                              const uint8_t* scales, float* dz, int64_t ldz, float* colsum, int64_t R,
+                              int64_t C, int format, int act, double* partial, hipStream_t s);
+int64_t mx_act_grad_partial_doubles(int64_t R, int64_t C);
+// C[M,N] = op(A)[M,K] . B[K,N]: A binary32 (transA: stored [K, M]), B microscaled [K, N].
+struct MxGemmParams {
+  const float* A;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  float* C;
+  int64_t M, N, K;
+  int64_t lda, ldc;
+  int transA, format;
+};
+hipError_t launch_mx_gemm(const MxGemmParams& p, void* scratch, hipStream_t s);
+int64_t mx_gemm_scratch_bytes(int64_t M, int64_t N, int64_t K);
+// Y[M,N] = act(X . W^T + bias): X [M, K] binary32, encoded in x_format on the way, W microscaled
+// [N, K].
+struct MxLinearParams {
+  const float* X;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const float* bias;
+  float* Y;
+  int64_t M, N, K;
+  int64_t ldx, ldy;
+  int x_format, w_format, act;
+};
+hipError_t launch_mx_linear(const MxLinearParams& p, void* scratch, hipStream_t s);
+int64_t mx_linear_scratch_bytes(int64_t M, int64_t N, int64_t K);
+
 // Y[C,R] = X[R,C]^T
 hipError_t launch_transpose(const float* x, float* y, int64_t R, int64_t C, hipStream_t s);
 

@@ -184,6 +184,11 @@ enum Opcode : uint32_t {
   OP_COPY = 14,
   OP_TRANSPOSE = 15,
   OP_CE_HEAD = 16,
+  OP_MX_ENCODE = 17,
+  OP_MX_DECODE = 18,
+  OP_MX_ACT_GRAD = 19,
+  OP_MX_GEMM = 20,
+  OP_MX_LINEAR = 21,
 };
 
 #pragma pack(push, 1)
@@ -258,6 +263,7 @@ struct Program {
   uint64_t arena_bytes = 0;               // per lease
   uint64_t scratch_off = 0, scratch_side_off = 0;
   std::vector<uint64_t> internal_offset;  // per slot (internal only), within a lease's arena
+  std::vector<uint8_t> slot_alignment;    // per slot: what a bound address is a multiple of
   // Two-stream schedule (plan_streams): step j runs on the context stream (0) or its side
   // stream (1), first waiting for the events recorded after the steps in wait_for[j];
   // record_after[j] marks steps other-stream steps depend on. side_steps == 0: one stream.
@@ -424,6 +430,113 @@ int32_t validate_gemm_update(Validator& v, size_t idx, const Step& st) {
       !v.writable(e.vn, "second moment candidate"))
     return v.err;
   return SHK_HIP_STATUS_OK;
+}
+
+// The codes and scales of a microscaled [R, C] tensor in slots `codes` and `scales`.
+bool holds_mx(Validator& v, int32_t codes, int32_t scales, int64_t R, int64_t C, int64_t format,
+              bool written) {
+  // (mx kernels count groups of 128 values in 32 bits and columns in an int)
+  if (C > INT32_MAX - 256 || prod(R, (C + 127) / 128) > INT32_MAX) {
+    v.err = fail(SHK_HIP_STATUS_UNSUPPORTED_SHAPE, "step %zu: microscaled tensor too large", v.step);
+    return false;
+  }
+  if (!v.slot_ok(codes, false, "codes") || !v.slot_ok(scales, false, "scales")) return false;
+  if (codes == scales) {
+    v.err = fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED, "step %zu: codes and scales share slot %d",
+                 v.step, codes);
+    return false;
+  }
+  const int64_t groups = prod(R, (C + 127) / 128);
+  return v.holds(codes, prod(groups, format == shk::MX_E2M1 ? 64 : 128), DT_U8, "codes") &&
+         v.holds(scales, prod(groups, 4), DT_U8, "scales") &&
+         (!written || (v.writable(codes, "codes") && v.writable(scales, "scales")));
+}
+
+int32_t validate_mx_step(Validator& v, size_t idx, const Step& st, uint64_t* scratch_doubles) {
+  const StepRecord& r = st.rec;
+  const int32_t* s = r.slot;
+  const int64_t* a = r.iarg;
+  auto need = [&](int64_t bytes) {
+    *scratch_doubles = std::max<uint64_t>(*scratch_doubles, (uint64_t)(bytes + 7) / 8);
+  };
+  auto bad_shape = [&](const char* what) {
+    return fail(SHK_HIP_STATUS_UNSUPPORTED_SHAPE, "step %zu: invalid %s", idx, what);
+  };
+  auto format_ok = [](int64_t f) { return f >= 0 && f <= 2; };
+  auto flag_ok = [](int64_t f) { return f == 0 || f == 1; };
+  // a row stride of a tensor that has elements
+  auto ld_ok = [](int64_t R, int64_t C, int64_t ld) { return R <= 0 || C <= 0 || ld >= C; };
+  switch (r.opcode) {
+    case OP_MX_ENCODE: {
+      const int64_t R = a[0], C = a[1], ldx = a[2], format = a[3], keep = a[4];
+      if (R < 0 || C < 0 || !ld_ok(R, C, ldx) || !format_ok(format) || !flag_ok(keep) ||
+          (keep && format == shk::MX_E2M1))
+        return bad_shape("microscaled encoding");
+      if (!v.slot_ok(s[0], false, "X") || !v.holds(s[0], span(R, C, ldx), DT_F32, "X") ||
+          !holds_mx(v, s[1], s[2], R, C, format, true))
+        return v.err;
+      return SHK_HIP_STATUS_OK;
+    }
+    case OP_MX_DECODE: {
+      const int64_t R = a[0], C = a[1], ldy = a[2], format = a[3];
+      if (R < 0 || C < 0 || !ld_ok(R, C, ldy) || !format_ok(format))
+        return bad_shape("microscaled decoding");
+      if (!holds_mx(v, s[0], s[1], R, C, format, false) || !v.slot_ok(s[2], false, "Y") ||
+          !v.holds(s[2], span(R, C, ldy), DT_F32, "Y") || !v.writable(s[2], "Y"))
+        return v.err;
+      return SHK_HIP_STATUS_OK;
+    }
+    case OP_MX_ACT_GRAD: {
+      const int64_t R = a[0], C = a[1], ldy = a[2], ldz = a[3], format = a[4], act = a[5];
+      if (R < 0 || C < 0 || !ld_ok(R, C, ldy) || !ld_ok(R, C, ldz) || !format_ok(format) || act < 0 ||
+          act > 3)
+        return bad_shape("microscaled activation gradient");
+      if (!v.slot_ok(s[0], false, "dY") || !v.holds(s[0], span(R, C, ldy), DT_F32, "dY") ||
+          !holds_mx(v, s[1], s[2], R, C, format, false) || !v.slot_ok(s[3], false, "dZ") ||
+          !v.holds(s[3], span(R, C, ldz), DT_F32, "dZ") || !v.writable(s[3], "dZ") ||
+          !v.slot_ok(s[4], true, "column sum") || !v.holds(s[4], C, DT_F32, "column sum") ||
+          !v.writable(s[4], "column sum"))
+        return v.err;
+      // dZ may replace dY element by element
+      if ((s[0] == s[3] && ldy != ldz) || (s[4] >= 0 && (s[4] == s[0] || s[4] == s[3])))
+        return fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED,
+                    "step %zu: an activation gradient's output aliases another operand", idx);
+      if (s[4] >= 0) need(8 * shk::mx_act_grad_partial_doubles(R, C));
+      return SHK_HIP_STATUS_OK;
+    }
+    case OP_MX_GEMM: {
+      const int64_t M = a[0], N = a[1], K = a[2], lda = a[3], ldc = a[4], tA = a[5], format = a[6];
+      if (M < 0 || N < 0 || K < 0 || M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX ||
+          !flag_ok(tA) || !format_ok(format) || !ld_ok(M, N, ldc) ||
+          (M > 0 && N > 0 && !(tA ? ld_ok(K, M, lda) : ld_ok(M, K, lda))))
+        return bad_shape("microscaled product");
+      if (!v.slot_ok(s[0], false, "A") ||
+          !v.holds(s[0], tA ? span(K, M, lda) : span(M, K, lda), DT_F32, "A") ||
+          !holds_mx(v, s[1], s[2], K, N, format, false) || !v.slot_ok(s[3], false, "C") ||
+          !v.holds(s[3], span(M, N, ldc), DT_F32, "C") || !v.writable(s[3], "C"))
+        return v.err;
+      if (s[0] == s[3])
+        return fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED, "step %zu: C aliases A", idx);
+      need(shk::mx_gemm_scratch_bytes(M, N, K));
+      return SHK_HIP_STATUS_OK;
+    }
+    default: {  // OP_MX_LINEAR
+      const int64_t M = a[0], N = a[1], K = a[2], ldx = a[3], ldy = a[4], act = a[7];
+      if (M < 0 || N < 0 || K < 0 || M > INT32_MAX / 2 || N > INT32_MAX / 2 || !ld_ok(M, N, ldy) ||
+          (N > 0 && !ld_ok(M, K, ldx)) || !format_ok(a[5]) || !format_ok(a[6]) || act < 0 || act > 3)
+        return bad_shape("microscaled linear layer");
+      if (prod(M, (K + 127) / 128) > INT32_MAX) return bad_shape("microscaled linear layer");
+      if (!v.slot_ok(s[0], false, "X") || !v.holds(s[0], span(M, K, ldx), DT_F32, "X") ||
+          !holds_mx(v, s[1], s[2], N, K, a[6], false) || !v.slot_ok(s[3], true, "bias") ||
+          !v.holds(s[3], N, DT_F32, "bias") || !v.slot_ok(s[4], false, "Y") ||
+          !v.holds(s[4], span(M, N, ldy), DT_F32, "Y") || !v.writable(s[4], "Y"))
+        return v.err;
+      if (s[4] == s[0] || s[4] == s[3])
+        return fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED, "step %zu: Y aliases another operand", idx);
+      need(shk::mx_linear_scratch_bytes(M, N, K));
+      return SHK_HIP_STATUS_OK;
+    }
+  }
 }
 
 int32_t validate_step(const std::vector<SlotRecord>& slots, size_t idx, const Step& st,
@@ -712,6 +825,8 @@ int32_t validate_step(const std::vector<SlotRecord>& slots, size_t idx, const St
           !v.writable(s[1], "Y"))
         return v.err;
       return SHK_HIP_STATUS_OK;
+    case OP_MX_ENCODE: case OP_MX_DECODE: case OP_MX_ACT_GRAD: case OP_MX_GEMM: case OP_MX_LINEAR:
+      return validate_mx_step(v, idx, st, scratch_doubles);
     default:
       return fail(SHK_HIP_STATUS_UNSUPPORTED_OPERATION, "step %zu: unknown opcode %u", idx, r.opcode);
   }
@@ -850,6 +965,40 @@ hipError_t enqueue_step(const Step& st, const Bound& b, hipStream_t stream, doub
       return shk::launch_copy(b.get<const float>(s[0]), b.get<float>(s[1]), a[0], stream);
     case OP_TRANSPOSE:
       return shk::launch_transpose(b.get<const float>(s[0]), b.get<float>(s[1]), a[0], a[1], stream);
+    case OP_MX_ENCODE:
+      return shk::launch_mx_encode(b.get<const float>(s[0]), a[2], b.get<uint8_t>(s[1]),
+                                   b.get<uint8_t>(s[2]), a[0], a[1], (int)a[3], (int)a[4], stream);
+    case OP_MX_DECODE:
+      return shk::launch_mx_decode(b.get<const uint8_t>(s[0]), b.get<const uint8_t>(s[1]),
+                                   b.get<float>(s[2]), a[2], a[0], a[1], (int)a[3], stream);
+    case OP_MX_ACT_GRAD:
+      return shk::launch_mx_act_grad(b.get<const float>(s[0]), a[2], b.get<const uint8_t>(s[1]),
+                                     b.get<const uint8_t>(s[2]), b.get<float>(s[3]), a[3],
+                                     b.get<float>(s[4]), a[0], a[1], (int)a[4], (int)a[5], scratch,
+                                     stream);
+    case OP_MX_GEMM: {
+      shk::MxGemmParams p{};
+      p.A = b.get<const float>(s[0]);
+      p.codes = b.get<const uint8_t>(s[1]);
+      p.scales = b.get<const uint8_t>(s[2]);
+      p.C = b.get<float>(s[3]);
+      p.M = a[0]; p.N = a[1]; p.K = a[2];
+      p.lda = a[3]; p.ldc = a[4];
+      p.transA = (int)a[5]; p.format = (int)a[6];
+      return shk::launch_mx_gemm(p, scratch, stream);
+    }
+    case OP_MX_LINEAR: {
+      shk::MxLinearParams p{};
+      p.X = b.get<const float>(s[0]);
+      p.codes = b.get<const uint8_t>(s[1]);
+      p.scales = b.get<const uint8_t>(s[2]);
+      p.bias = b.get<const float>(s[3]);
+      p.Y = b.get<float>(s[4]);
+      p.M = a[0]; p.N = a[1]; p.K = a[2];
+      p.ldx = a[3]; p.ldy = a[4];
+      p.x_format = (int)a[5]; p.w_format = (int)a[6]; p.act = (int)a[7];
+      return shk::launch_mx_linear(p, scratch, stream);
+    }
     default:
       return hipErrorInvalidValue;
   }
@@ -913,6 +1062,11 @@ Access step_access(const Step& st) {
     }
     case OP_STEP_COMMIT: R(sl[0]); W(sl[0]); x.status_read = true; break;
     case OP_FILL: W(sl[0]); break;
+    case OP_MX_ENCODE: R(sl[0]); W(sl[1]); W(sl[2]); break;
+    case OP_MX_DECODE: R(sl[0]); R(sl[1]); W(sl[2]); break;
+    case OP_MX_ACT_GRAD: R(sl[0]); R(sl[1]); R(sl[2]); W(sl[3]); W(sl[4]); break;
+    case OP_MX_GEMM: R(sl[0]); R(sl[1]); R(sl[2]); W(sl[3]); break;
+    case OP_MX_LINEAR: R(sl[0]); R(sl[1]); R(sl[2]); R(sl[3]); W(sl[4]); break;
     default:  // unknown: conflicts with everything
       x.status_read = true;
       W(-2);
@@ -925,7 +1079,9 @@ bool step_launches(const StepRecord& r) {
   const int64_t* a = r.iarg;
   switch (r.opcode) {
     case OP_GEMM: case OP_POINTWISE: case OP_SOFTMAX_BWD: case OP_LSE_BWD: case OP_TRANSPOSE:
+    case OP_MX_ENCODE: case OP_MX_DECODE: case OP_MX_GEMM: case OP_MX_LINEAR:
       return a[0] > 0 && a[1] > 0;
+    case OP_MX_ACT_GRAD: return a[1] > 0 && (a[0] > 0 || r.slot[4] >= 0);
     case OP_COLSUM: return a[1] > 0;
     case OP_ROW_REDUCE: case OP_SOFTMAX: case OP_CE_HEAD: case OP_FILL: case OP_COPY:
       return a[0] > 0;
@@ -1832,6 +1988,7 @@ int32_t decode_image(const void* image, uint64_t image_bytes, Program* pr) {
     if (out_seen[i] != 1) {
       return fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED, "output index %zu bound %d times", i, out_seen[i]);
     }
+  pr->slot_alignment.assign(h.n_slots, 1);
   pr->n_inputs = (uint32_t)in_seen.size();
   pr->n_outputs = (uint32_t)out_seen.size();
 
@@ -1852,6 +2009,14 @@ int32_t decode_image(const void* image, uint64_t image_bytes, Program* pr) {
     p += padded;
     const int32_t v = validate_step(pr->slots, i, st, &scratch_doubles);
     if (v != SHK_HIP_STATUS_OK) return v;
+    // codes of microscaled tensors are read 16 bytes at a time, scales in words of four
+    auto aligned = [&](int32_t codes, int32_t scales) {
+      pr->slot_alignment[codes] = std::max<uint8_t>(pr->slot_alignment[codes], 16);
+      pr->slot_alignment[scales] = std::max<uint8_t>(pr->slot_alignment[scales], 4);
+    };
+    if (st.rec.opcode == OP_MX_DECODE) aligned(st.rec.slot[0], st.rec.slot[1]);
+    else if (st.rec.opcode >= OP_MX_ENCODE && st.rec.opcode <= OP_MX_LINEAR)
+      aligned(st.rec.slot[1], st.rec.slot[2]);
   }
   if (p != end) return fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED, "image has trailing bytes");
 
@@ -2173,6 +2338,9 @@ int32_t bind_external(Program* pr, uint32_t input_count, void* const* inputs,
     if (buf->bytes < s.bytes)
       return fail(SHK_HIP_STATUS_INCOMPATIBLE_RESOURCE, "slot %zu needs %llu bytes, bound buffer has %llu", i,
                   (unsigned long long)s.bytes, (unsigned long long)buf->bytes);
+    if (reinterpret_cast<uintptr_t>(buf->ptr) % pr->slot_alignment[i] != 0)
+      return fail(SHK_HIP_STATUS_INCOMPATIBLE_RESOURCE, "slot %zu needs %u-byte alignment", i,
+                  (unsigned)pr->slot_alignment[i]);
     b->ptr[i] = buf->ptr;
     const uintptr_t lo = reinterpret_cast<uintptr_t>(buf->ptr), hi = lo + std::max<uint64_t>(s.bytes, 1);
     if (s.kind != SLOT_INPUT) written.push_back({lo, hi});

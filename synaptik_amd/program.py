@@ -43,9 +43,17 @@ OP_FILL = 13
 OP_COPY = 14
 OP_TRANSPOSE = 15
 OP_CE_HEAD = 16
+OP_MX_ENCODE = 17
+OP_MX_DECODE = 18
+OP_MX_ACT_GRAD = 19
+OP_MX_GEMM = 20
+OP_MX_LINEAR = 21
 
 ACT = {None: 0, "none": 0, "relu": 1, "tanh": 2, "sigmoid": 3}
 REDUCE_KIND = {"sum": 0, "mean": 1, "max": 2, "lse": 3}
+
+# microscaled formats: 8-bit codes with 3 or 2 mantissa bits, 4-bit codes with one
+MX_FORMAT = {"e4m3": 0, "e5m2": 1, "e2m1": 2}
 
 # pointwise register-machine opcodes (elementwise.hip)
 PW = {
@@ -59,6 +67,27 @@ BROADCAST = {"full": 0, "row": 1, "col": 2, "scalar": 3}
 _STEP = struct.Struct("<II8i16q8f")
 _SLOT = struct.Struct("<QIIII")
 assert _STEP.size == 200 and _SLOT.size == 24
+
+
+def mx_groups(cols: int) -> int:
+    """Groups of 128 values that hold a microscaled row of `cols` values."""
+    return -(-int(cols) // 128)
+
+
+def mx_code_bytes(rows: int, cols: int, format: str) -> int:
+    """Bytes of a microscaled tensor's codes: whole groups of 128 values a row."""
+    return int(rows) * mx_groups(cols) * (64 if _mx_format(format) == 2 else 128)
+
+
+def mx_scale_bytes(rows: int, cols: int) -> int:
+    """Bytes of a microscaled tensor's scales: one for each block of 32 values, four a group."""
+    return int(rows) * mx_groups(cols) * 4
+
+
+def _mx_format(format: str) -> int:
+    if format not in MX_FORMAT:
+        raise ValueError(f"unknown microscaled format {format!r}")
+    return MX_FORMAT[format]
 
 
 @dataclass
@@ -259,6 +288,58 @@ class ProgramBuilder:
     def transpose(self, X, Y, R, C) -> Step:
         """Y[C,R] = X[R,C]^T."""
         return self._add(OP_TRANSPOSE, [X, Y], [R, C])
+
+    # ---- microscaled tensors ----
+    # A microscaled [R, C] tensor is a pair of u8 slots (codes, scales): per row, groups of 128
+    # values as codes of 8 bits (e4m3, e5m2) or 4 bits (e2m1, the even column in a byte's low
+    # half), and a power of two 2^(s - 127) for each block of 32 values. Codes behind the last
+    # column are zero.
+    def mx_tensor(self, rows: int, cols: int, format: str, kind: str = "internal"):
+        """The (codes, scales) slots of a microscaled tensor: "internal", "input", "inout" or
+        "output"."""
+        make = {"internal": self.internal, "input": self.input, "output": self.output,
+                "inout": lambda n, dt: self.input(n, dt, inout=True)}[kind]
+        return (make(mx_code_bytes(rows, cols, format), "u8"),
+                make(mx_scale_bytes(rows, cols), "u8"))
+
+    def mx_encode(self, X, out, R, C, *, format="e4m3", ldx=None, keep_nonzero=False) -> Step:
+        """Encodes X [R, C] into out = (codes, scales). A block's scale is the smallest power of
+        two (2^-110 at least) under which its largest finite magnitude lies within the format;
+        codes are rounded to nearest, ties to even; a finite value stays finite. With keep_nonzero
+        (8-bit formats) a nonzero value's code is never zero, so that a ReLU output keeps its mask.
+        NaN stays NaN; an infinity becomes NaN in e4m3; in e2m1 either makes its whole block NaN."""
+        return self._add(OP_MX_ENCODE, [X, *out],
+                         [R, C, ldx if ldx is not None else C, _mx_format(format), int(keep_nonzero)])
+
+    def mx_decode(self, X, Y, R, C, *, format="e4m3", ldy=None) -> Step:
+        """Y [R, C] = the values that X = (codes, scales) stands for."""
+        return self._add(OP_MX_DECODE, [*X, Y],
+                         [R, C, ldy if ldy is not None else C, _mx_format(format)])
+
+    def mx_act_grad(self, dY, Y, dZ, R, C, *, act, format="e4m3", ldy=None, ldz=None,
+                    colsum=None) -> Step:
+        """dZ = act_grad(act, dY, Y) from the activation output's codes Y = (codes, scales);
+        `colsum` optionally receives the column sums of dZ (a bias gradient). dZ may be dY."""
+        return self._add(OP_MX_ACT_GRAD, [dY, *Y, dZ, colsum],
+                         [R, C, ldy if ldy is not None else C, ldz if ldz is not None else C,
+                          _mx_format(format), ACT[act]])
+
+    def mx_gemm(self, A, B, C, M, N, K, *, format="e4m3", trans_a=False, lda=None, ldc=None) -> Step:
+        """C [M, N] = op(A) . B for a binary32 A [M, K] (trans_a: stored [K, M]) and a microscaled
+        B = (codes, scales) [K, N]: a weight gradient dW = dZ^T . X from X's checkpoint, or an
+        input gradient dX = dZ . W through microscaled weights. A is not rounded."""
+        return self._add(OP_MX_GEMM, [A, *B, C],
+                         [M, N, K, lda if lda is not None else (M if trans_a else K),
+                          ldc if ldc is not None else N, int(trans_a), _mx_format(format)])
+
+    def mx_linear(self, X, W, Y, M, N, K, *, x_format="e4m3", w_format="e2m1", bias=None, act=None,
+                  ldx=None, ldy=None) -> Step:
+        """Y [M, N] = act(X . W^T + bias) for microscaled weights W = (codes, scales) [N, K] and
+        binary32 activations X [M, K], which are encoded in x_format on the way (as mx_encode
+        without keep_nonzero does)."""
+        return self._add(OP_MX_LINEAR, [X, *W, bias, Y],
+                         [M, N, K, ldx if ldx is not None else K, ldy if ldy is not None else N,
+                          _mx_format(x_format), _mx_format(w_format), ACT[act]])
 
     # ---- encoding ----
     def image(self) -> bytes:
