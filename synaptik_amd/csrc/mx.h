@@ -65,6 +65,15 @@ __device__ __forceinline__ float mx_reciprocal(uint32_t s) {
   return __uint_as_float((254u - s) << 23);
 }
 
+// The maximum over the eight lanes that hold a block's 32 values: two quad permutations, then the
+// mirror image within eight lanes.
+__device__ __forceinline__ uint32_t mx_block_largest(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, false));
+  return v;
+}
+
 // Four values, already divided by their scale, as codes: a word of four bytes, or 16 bits of four
 // halves for e2m1. Rounding is to nearest, ties to even, and nothing overflows (mx_scale_of). x
 // holds the values before scaling: with KEEP a nonzero one never becomes a zero code; an infinity

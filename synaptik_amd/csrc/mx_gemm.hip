@@ -10,32 +10,36 @@
 // instead of the binary32 ones', 5.3 times as fast (2.5 / 3 against 0.157 PFLOP/s).
 #include <algorithm>
 
-#include "mx.h"
+#include "mx_tiles.h"
 
 namespace shk {
 namespace {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 int64_t pad256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // ---- operands as matrix-instruction fragments ----
 // v_mfma_f32_32x32x16_bf16 takes from lane l the eight values k = 8 (l / 32) .. + 7 of row l mod 32.
 // Both operands are laid out as the 1 KB fragments it takes, 16 bytes a lane: fragment (kt, block,
-// plane) covers k = 16 kt .. + 15 of rows 32 block .. + 31, planes (of A: leading, middle, last
-// bits) of a block adjacent and the blocks of one kt adjacent. Values behind K are zero; rows
-// behind the operand's last are not written (they reach only results that are not stored).
-constexpr int FRAG = 1024;
+// plane) covers k = 16 kt .. + 15 of rows 32 block .. + 31, planes of a block adjacent and the
+// blocks of one kt adjacent. Values behind K are zero; rows behind the operand's last are not
+// written (they reach only results that are not stored).
+constexpr int FRAG = 1024, PLANES = 3;
+
+// (a >> 16) | (b & 0xffff0000): the bfloat16 values that two floats hold exactly.
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+// Where the eight values k = 8 octet .. + 7 of row r lie in plane 0 of an operand of `blocks`
+// blocks and `planes` planes.
+__device__ __forceinline__ char* frag_at(char* base, int64_t octet, int64_t r, int64_t blocks, int planes) {
+  return base + ((octet >> 1) * blocks + (r >> 5)) * planes * FRAG + (((octet & 1) << 5) + (r & 31)) * 16;
+}
 
 // The three parts of eight values. An infinity is its leading part alone; a NaN stays one though
 // its low bits are cut off.
 struct Planes {
   uintx4 hi, mid, lo;
 };
-__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
-  return __builtin_amdgcn_perm(b, a, 0x07060302u);  // (a >> 16) | (b & 0xffff0000)
-}
 __device__ __forceinline__ Planes split8(const float (&v)[8]) {
   uint32_t h[8], m[8], l[8];
 #pragma unroll
@@ -59,10 +63,7 @@ __device__ __forceinline__ Planes split8(const float (&v)[8]) {
   }
   return p;
 }
-// Rows of a block: MT blocks of A, kt the fragment's ordinal along K.
-__device__ __forceinline__ void put_planes(char* pa, int64_t kt, int64_t MT, int64_t m, int octet,
-                                           const Planes& p) {
-  char* at = pa + ((kt * MT + (m >> 5)) * 3) * FRAG + (((octet & 1) << 5) + (m & 31)) * 16;
+__device__ __forceinline__ void put_planes(char* at, const Planes& p) {
   *reinterpret_cast<uintx4*>(at) = p.hi;
   *reinterpret_cast<uintx4*>(at + FRAG) = p.mid;
   *reinterpret_cast<uintx4*>(at + 2 * FRAG) = p.lo;
@@ -78,7 +79,7 @@ __device__ __forceinline__ void pack_a_t(const float* __restrict__ a, int64_t ld
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = k + i < K ? a[(k + i) * lda + m] : 0.0f;
-  put_planes(pa, octet >> 1, MT, m, (int)(octet & 1), split8(v));
+  put_planes(frag_at(pa, octet, m, MT, PLANES), split8(v));
 }
 
 // A stored [M, K]: a wave takes sixteen rows and four octets, 128 contiguous bytes a row.
@@ -98,7 +99,7 @@ __device__ __forceinline__ void pack_a_n(const float* __restrict__ a, int64_t ld
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = k + i < K ? src[i] : 0.0f;
   }
-  put_planes(pa, octet >> 1, MT, m, (int)(octet & 1), split8(v));
+  put_planes(frag_at(pa, octet, m, MT, PLANES), split8(v));
 }
 
 // B's codes [K, N] as bfloat16 fragments: a lane takes four columns 4 q .. 4 q + 3 of a block and
@@ -127,7 +128,7 @@ __device__ __forceinline__ void pack_b(const uint8_t* __restrict__ codes,
 #pragma unroll
     for (int j = 0; j < 4; ++j) b[i][j] = k + i < K ? __float_as_uint(v[j] * f) : 0u;
   }
-  char* at = pb + ((octet >> 1) * NT + (n >> 5)) * FRAG + (((octet & 1) << 5) + ((n & 31) >> 2)) * 16;
+  char* at = frag_at(pb, octet, n / 32 * 32 + (n & 31) / 4, NT, 1);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     uintx4 q;
@@ -160,12 +161,6 @@ __global__ void __launch_bounds__(256) mx_pack(PackParams p) {
 }
 
 // ---- the product ----
-// BM x BN results a workgroup, WM x WN waves of (BM / WM) x (BN / WN), one fragment (16 k) a stage
-// and operand block, NS stages in LDS. The stages are filled by global_load_lds_dwordx4, which
-// copies 16 bytes a lane without passing through registers; fragments lie in memory as in LDS, so
-// every copy and every fragment read is linear. A stage is copied NS - 1 stages before it is read;
-// at its barrier each wave has waited for its own copies into it, and has finished with the
-// stage whose place the next copies take.
 struct WideParams {
   const char* pa;
   const char* pb;
@@ -175,24 +170,25 @@ struct WideParams {
   int tiles_m, tiles_n, chunk;  // chunk: fragments along K of a slice
 };
 
+// BM x BN results a workgroup, WM x WN waves of (BM / WM) x (BN / WN), 16 k a stage, NS stages in
+// LDS. The stages are filled by global_load_lds_dwordx4, which copies 16 bytes a lane without
+// passing through registers; fragments lie in memory as in LDS, so every copy and every fragment
+// read is linear. A stage is copied NS - 1 stages before it is read; before a stage is read, each
+// wave has waited for its own copies into it, and has finished with the stage whose place the next
+// copies take. A stage's fragments are read while the one before is multiplied.
 template <int BM, int BN, int WM, int WN, int NS>
 __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
   constexpr int WAVES = WM * WN, TM = BM / 32 / WM, TN = BN / 32 / WN;
-  constexpr int CA = BM / 32 * 3, CB = BN / 32, COPIES = (CA + CB) / WAVES;
+  constexpr int CA = BM / 32 * PLANES, CB = BN / 32, COPIES = (CA + CB) / WAVES;
   static_assert((CA + CB) % WAVES == 0, "whole copies a wave");
   constexpr int STAGE = (CA + CB) * FRAG;
+  static_assert(NS >= 2 && NS * STAGE <= 160 * 1024, "LDS");
   __shared__ __align__(16) char lds[NS * STAGE];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Tiles in groups of four rows of tiles, and each of the eight XCDs (workgroups go to them in
-  // turn) a contiguous run of that order: a row of A's fragments is three times a column of B's.
-  const int tiles = p.tiles_m * p.tiles_n;
-  const int per = tiles / 8, extra = tiles % 8, xcd = blockIdx.x % 8;
-  const int t = xcd * per + min(xcd, extra) + blockIdx.x / 8;
-  const int group = t / (4 * p.tiles_n), first = 4 * group, rows = min(4, p.tiles_m - first);
-  const int in_group = t - group * 4 * p.tiles_n;
-  const int tm = first + in_group % rows, tn = in_group / rows;
-  const int kt0 = blockIdx.y * p.chunk, n_kt = min(p.chunk, p.KT - kt0);
+  int tm, tn;
+  mx_tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+  const int kt0 = blockIdx.y * p.chunk, stages = min(p.chunk, p.KT - kt0);
 
   // this wave's copies: fragment c of a stage, the operand's blocks clamped to its last
   const char* src[COPIES];
@@ -201,9 +197,9 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
   for (int i = 0; i < COPIES; ++i) {
     const int c = wave * COPIES + i;
     if (c < CA) {
-      const int block = min(tm * (BM / 32) + c / 3, p.MT - 1);
-      src[i] = p.pa + (((int64_t)kt0 * p.MT + block) * 3 + c % 3) * FRAG;
-      step[i] = (int64_t)p.MT * 3 * FRAG;
+      const int block = min(tm * (BM / 32) + c / PLANES, p.MT - 1);
+      src[i] = p.pa + (((int64_t)kt0 * p.MT + block) * PLANES + c % PLANES) * FRAG;
+      step[i] = (int64_t)p.MT * PLANES * FRAG;
     } else {
       const int block = min(tn * (BN / 32) + c - CA, p.NT - 1);
       src[i] = p.pb + ((int64_t)kt0 * p.NT + block) * FRAG;
@@ -219,8 +215,8 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
       const uint32_t dst = lds0 + stage * STAGE + (wave * COPIES + i) * FRAG;
       asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(src[i]), "{m0}"(dst) : "memory");
     }
-    // (behind the last fragment it is copied again, which keeps the count of copies in flight)
-    if (++copied < n_kt) {
+    // (behind the last stage it is copied again, which keeps the count of copies in flight)
+    if (++copied < stages) {
 #pragma unroll
       for (int i = 0; i < COPIES; ++i) src[i] += step[i];
     }
@@ -235,7 +231,7 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
   const int wm = wave / WN, wn = wave % WN;
   struct Frags {
-    bf16x8 a[TM][3], b[TN];
+    bf16x8 a[TM][PLANES], b[TN];
   };
   auto read = [&](int stage, Frags& f) {
     const char* at = lds + stage * STAGE + lane * 16;
@@ -244,48 +240,47 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int q = 0; q < 3; ++q)
-        f.a[i][q] = *reinterpret_cast<const bf16x8*>(at + ((wm * TM + i) * 3 + q) * FRAG);
+      for (int q = 0; q < PLANES; ++q)
+        f.a[i][q] = *reinterpret_cast<const bf16x8*>(at + ((wm * TM + i) * PLANES + q) * FRAG);
   };
   auto multiply = [&](const Frags& f) {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int q = 2; q >= 0; --q)
+      for (int q = PLANES - 1; q >= 0; --q)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i][q], f.b[j], acc[i][j], 0, 0, 0);
   };
+  int stage = 0;
   // Waits until this wave's reads have returned and its copies into the stage after this one have
   // landed, for all waves; then refills the stage just read.
-  auto advance = [&](int stage) {
+  auto advance = [&](int s) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((NS - 2) * COPIES) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" : : : "memory");
-    copy_next(stage);
+    copy_next(s);
+    stage = s == NS - 1 ? 0 : s + 1;
   };
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s) copy_next(s);
-  int stage = 0;
-  auto next = [&](int s) { return s == NS - 1 ? 0 : s + 1; };
   Frags even, odd;
   advance(NS - 1);
   read(0, even);
-  int kt = 0;
-  for (; kt + 2 <= n_kt; kt += 2) {
+  int s = 0;
+  for (; s + 2 <= stages; s += 2) {
     advance(stage);
-    stage = next(stage);
     read(stage, odd);
     multiply(even);
     advance(stage);
-    stage = next(stage);
     read(stage, even);
     multiply(odd);
   }
-  if (kt < n_kt) multiply(even);
+  if (s < stages) multiply(even);
   asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // no copy outlives the workgroup's LDS
 
-  // register r of a block: row 8 (r / 4) + 4 (lane / 32) + r mod 4, B's row lane mod 32
+  // register r of a block: row 8 (r / 4) + 4 (lane / 32) + r mod 4, B's row lane mod 32, which is
+  // column 4 q + j for row q + 8 j (pack_b)
   float* c = p.C + blockIdx.y * p.plane;
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -343,7 +338,7 @@ int64_t mx_gemm_scratch_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0) return 0;
   const WidePlan w = plan(M, N, K);
   if (!w.wide) return pad256(4 * K * N) + 4 * gemm_workspace_floats(M, N, K);
-  return w.KT * (3 * w.MT + w.NT) * FRAG + (w.slices > 1 ? 4 * w.slices * M * N : 0);
+  return w.KT * (PLANES * w.MT + w.NT) * FRAG + (w.slices > 1 ? 4 * w.slices * M * N : 0);
 }
 
 hipError_t launch_mx_gemm(const MxGemmParams& p, void* scratch, hipStream_t s) {
@@ -361,7 +356,7 @@ hipError_t launch_mx_gemm(const MxGemmParams& p, void* scratch, hipStream_t s) {
     return launch_gemm(g, reinterpret_cast<float*>(static_cast<char*>(scratch) + pad256(4 * p.K * p.N)), s);
   }
   char* pa = static_cast<char*>(scratch);
-  char* pb = pa + w.KT * w.MT * 3 * FRAG;
+  char* pb = pa + w.KT * w.MT * PLANES * FRAG;
   float* partial = reinterpret_cast<float*>(pb + w.KT * w.NT * FRAG);
   PackParams k{p.A, p.codes, p.scales, pa, pb, p.lda, p.M, p.N, p.K, w.MT, w.NT, (int)((p.M + 63) / 64)};
   const dim3 packs((unsigned)((w.KT + 1) / 2), (unsigned)(k.a_blocks + (p.N + 255) / 256));

@@ -29,15 +29,6 @@ __device__ __forceinline__ void store4(float* p, int rest, const float (&v)[4]) 
   }
 }
 
-// Maximum over the eight lanes that hold a block's 32 values: two quad permutations, then the
-// mirror image within eight lanes.
-__device__ __forceinline__ uint32_t block_largest(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, false));
-  return v;
-}
-
 // One group of 128 values for 32 lanes, four values a lane, U groups a lane and round.
 template <int F, bool KEEP, int U>
 __global__ void __launch_bounds__(256) mx_encode(const float* __restrict__ x, int64_t ldx,
@@ -65,7 +56,7 @@ __global__ void __launch_bounds__(256) mx_encode(const float* __restrict__ x, in
         // (an infinity or NaN of an e2m1 block takes the block; elsewhere it has a code)
         largest = max(largest, F != MX_E2M1 && b >= 0x7f800000u ? 0u : b);
       }
-      largest = block_largest(largest);
+      largest = mx_block_largest(largest);
       const bool lost = F == MX_E2M1 && largest >= 0x7f800000u;
       const uint32_t s = mx_scale_of<F>(largest);
       uint32_t w = mx_codes4<F, KEEP>(v[u], mx_reciprocal(s));

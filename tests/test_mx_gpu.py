@@ -204,11 +204,13 @@ PRODUCTS = [(1, 1, 1), (1, 5, 3), (3, 2, 40), (16, 16, 16), (33, 31, 32), (1, 10
             (64, 64, 64), (65, 130, 100), (128, 128, 512), (200, 10, 900), (255, 257, 333),
             (257, 513, 65), (512, 512, 512), (700, 390, 1025), (1024, 1030, 260), (130, 4100, 77),
             (1025, 1023, 1027)]
+# large tiles, whole and split along K
+LARGE_PRODUCTS = [(4100, 2100, 70), (4000, 2000, 300)]
 
 
 @pytest.mark.parametrize("trans_a", [False, True])
-@pytest.mark.parametrize("format", mx.FORMATS)
-@pytest.mark.parametrize("shape", PRODUCTS, ids=str)
+@pytest.mark.parametrize("format,shape", [(f, s) for s in PRODUCTS for f in mx.FORMATS]
+                         + [("e4m3", s) for s in LARGE_PRODUCTS], ids=str)
 def test_product_of_a_microscaled_operand(ctx, shape, format, trans_a):
     M, N, K = shape
     rng = np.random.default_rng(M + 7 * N + 31 * K)
@@ -309,12 +311,14 @@ def linear_room(X, W, bias, act, z):
 LINEARS = [(1, 1, 1), (1, 7, 33), (1, 300, 1000), (1, 1030, 4096), (2, 130, 128), (3, 64, 129),
            (4, 17, 600), (5, 33, 257), (15, 65, 64), (16, 1030, 300), (17, 16, 2100), (33, 100, 31),
            (64, 512, 1024), (100, 333, 200), (129, 127, 130), (256, 256, 512), (300, 1021, 617),
-           (1030, 520, 260)]
+           (1030, 520, 260), (16, 70, 1100), (3, 40, 6000)]
+# tiles in LDS: whole, split along K, and of 256
+LARGE_LINEARS = [(1030, 1031, 1033), (70, 2000, 8300), (4000, 3001, 200)]
 
 
 @pytest.mark.parametrize("x_format", mx.FORMATS)
 @pytest.mark.parametrize("w_format", mx.FORMATS)
-@pytest.mark.parametrize("shape", LINEARS, ids=str)
+@pytest.mark.parametrize("shape", LINEARS + LARGE_LINEARS, ids=str)
 def test_linear_layer_of_microscaled_weights(ctx, shape, w_format, x_format):
     M, N, K = shape
     rng = np.random.default_rng(3 * M + 5 * N + K)
@@ -331,8 +335,9 @@ def test_linear_layer_of_microscaled_weights(ctx, shape, w_format, x_format):
 
 def test_linear_layer_with_strides_and_without_depth(ctx):
     rng = np.random.default_rng(2)
-    for M, ldx in ((1, 200), (7, 203), (40, 201), (300, 207)):
-        N, K, ldy = 150, 190, 161
+    for M, ldx, N, ldy in ((1, 200, 150, 161), (7, 203, 150, 161), (40, 201, 150, 161),
+                           (300, 207, 150, 161), (2500, 203, 2501, 2511)):
+        K = 190
         wide = rng.standard_normal((M, ldx)).astype(np.float32)
         codes, scales, W = mx.stored(rng.standard_normal((N, K)), "e2m1")
         got = gpu_mx_linear(ctx, wide, (codes, scales), None, M, N, K, "e4m3", "e2m1", None, ldx, ldy)
@@ -348,10 +353,10 @@ def test_linear_layer_with_strides_and_without_depth(ctx):
 
 @pytest.mark.parametrize("x_format,w_format", [("e4m3", "e2m1"), ("e2m1", "e2m1"), ("e5m2", "e4m3"),
                                                ("e4m3", "e5m2")])
-@pytest.mark.parametrize("M", [1, 8, 40, 300])
-def test_linear_layer_with_infinities_and_nans(ctx, M, x_format, w_format):
+@pytest.mark.parametrize("M,N", [(1, 140), (8, 140), (40, 140), (300, 140), (2000, 2001)])
+def test_linear_layer_with_infinities_and_nans(ctx, M, N, x_format, w_format):
     rng = np.random.default_rng(M)
-    N, K = 140, 300
+    K = 300
     X = rng.standard_normal((M, K)).astype(np.float32)
     w = rng.standard_normal((N, K))
     w[5, 70] = np.nan  # (e2m1: its block of 32, all of row 5's results either way)
