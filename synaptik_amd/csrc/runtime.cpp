@@ -1108,9 +1108,14 @@ bool concurrency_enabled() {
 // Two-stream list schedule: step j goes beside the main chain (stream 1) when it does not
 // depend on the step currently at the tail of stream 0; a step waits (event) for every earlier
 // step on the other stream it depends on. Steps on one stream keep program order.
+// (iarg 0, 1, 2 of the matrix products are their extents M, N, K)
+bool is_product(const Step& st) {
+  const uint32_t op = st.rec.opcode;
+  return op == OP_GEMM || op == OP_MX_GEMM || op == OP_MX_LINEAR;
+}
 // A GEMM with at least 2^28 multiply-adds: enough tiles to occupy every CU on its own.
 bool large_gemm(const Step& st) {
-  if (st.rec.opcode != OP_GEMM) return false;
+  if (!is_product(st)) return false;
   const int64_t* a = st.rec.iarg;
   if (a[0] <= 0 || a[1] <= 0 || a[2] <= 0) return false;
   const double macs = (double)a[0] * (double)a[1] * (double)a[2];
@@ -1124,7 +1129,7 @@ bool large_gemm(const Step& st) {
 bool side_stream_pays(const Program& pr) {
   double macs = 0.0;
   for (const Step& st : pr.steps)
-    if (st.rec.opcode == OP_GEMM) {
+    if (is_product(st)) {
       const int64_t* a = st.rec.iarg;
       if (a[0] > 0 && a[1] > 0 && a[2] > 0) macs += (double)a[0] * (double)a[1] * (double)a[2];
     }
@@ -1993,6 +1998,7 @@ int32_t decode_image(const void* image, uint64_t image_bytes, Program* pr) {
   pr->n_outputs = (uint32_t)out_seen.size();
 
   uint64_t scratch_doubles = 0;
+  std::vector<uint64_t> step_doubles(h.n_steps, 0);  // each step's own
   pr->steps.resize(h.n_steps);
   for (uint32_t i = 0; i < h.n_steps; ++i) {
     if ((uint64_t)(end - p) < sizeof(StepRecord)) {
@@ -2007,8 +2013,9 @@ int32_t decode_image(const void* image, uint64_t image_bytes, Program* pr) {
     }
     st.payload.assign(p, p + st.rec.payload_bytes);
     p += padded;
-    const int32_t v = validate_step(pr->slots, i, st, &scratch_doubles);
+    const int32_t v = validate_step(pr->slots, i, st, &step_doubles[i]);
     if (v != SHK_HIP_STATUS_OK) return v;
+    scratch_doubles = std::max(scratch_doubles, step_doubles[i]);
     // codes of microscaled tensors are read 16 bytes at a time, scales in words of four
     auto aligned = [&](int32_t codes, int32_t scales) {
       pr->slot_alignment[codes] = std::max<uint8_t>(pr->slot_alignment[codes], 16);
@@ -2038,8 +2045,13 @@ int32_t decode_image(const void* image, uint64_t image_bytes, Program* pr) {
     launches |= step_launches(st.rec);
   }
   pr->publishes |= !launches;
+  // the side stream's scratch serves the steps that the plan puts there (the context stream's serves
+  // every step: the one-stream order runs them all on it)
   pr->scratch_side_off = off;
-  if (pr->side_steps > 0) off += ((scratch_doubles * 8 + 255) / 256) * 256;
+  uint64_t side_doubles = 0;
+  for (uint32_t i = 0; i < h.n_steps; ++i)
+    if (pr->stream_of[i] != 0) side_doubles = std::max(side_doubles, step_doubles[i]);
+  off += ((side_doubles * 8 + 255) / 256) * 256;
   pr->internal_offset.assign(h.n_slots, 0);
   for (uint32_t i = 0; i < h.n_slots; ++i) {
     if (pr->slots[i].kind != SLOT_INTERNAL) continue;

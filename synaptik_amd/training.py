@@ -24,7 +24,7 @@ from typing import Sequence
 import numpy as np
 
 from .native import HipBuffer, HipContext, HipProgram
-from .program import ProgramBuilder, Slot
+from .program import OUTPUT, ProgramBuilder, Slot
 
 ACTIVATIONS = (None, "relu", "tanh", "sigmoid")
 
@@ -208,8 +208,13 @@ def _optimizer_kind(opt) -> str:
     raise TypeError(f"unsupported optimizer {opt!r}")
 
 
+# formats that keep a hidden layer's outputs between the passes of a step
+CHECKPOINTS = (None, "e4m3", "e5m2")
+
+
 def lower_training_step(spec: MlpSpec, batch: int, optimizer, *, label_dtype: str = "i64",
-                        mode: str = GradientMode.RESET_AND_STEP, clear_accumulator: bool = False):
+                        mode: str = GradientMode.RESET_AND_STEP, clear_accumulator: bool = False,
+                        checkpoint: str | None = None):
     """Lowers one training step of `spec` at `batch` rows to a program image.
 
     Inputs (in order): W_1..W_L, b_1..b_L (current, read only), first-moment slots per tensor
@@ -224,7 +229,15 @@ def lower_training_step(spec: MlpSpec, batch: int, optimizer, *, label_dtype: st
     streaming pass after the backward sweep. The caller adopts the candidate set only when the run succeeds. Every mode is transactional: a
     non-finite accumulated candidate or optimizer intermediate leaves the current parameters,
     slots, accumulators and the counter unchanged.
+
+    checkpoint "e4m3" or "e5m2" keeps the hidden layers' outputs from the forward to the backward
+    pass as microscaled 8-bit values (ProgramBuilder.mx_encode with keep_nonzero, so that ReLU's
+    masks are exact) instead of binary32: 1.03 bytes a value instead of 4, and the forward and
+    backward passes then share two binary32 buffers each. The forward pass and the objective are
+    those of the uncompressed step; the gradients are those of the kept values.
     """
+    if checkpoint not in CHECKPOINTS:
+        raise ValueError(f"unsupported checkpoint format {checkpoint!r}")
     kind = _optimizer_kind(optimizer)
     pb = ProgramBuilder()
     lay = TrainingLayout()
@@ -259,6 +272,9 @@ def lower_training_step(spec: MlpSpec, batch: int, optimizer, *, label_dtype: st
         lay.y = pb.input(batch, label_dtype)
     lay.loss = pb.output(1)
 
+    if checkpoint is not None and L > 1:
+        _lower_checkpointed(pb, lay, spec, batch, optimizer, kind, mode, uses_acc, checkpoint)
+        return pb, lay
     # activations Y_l (internal); Y_0 is the input x
     acts = [lay.x] + [pb.internal(batch * l.fan_out) for l in spec.layers]
     # one cotangent buffer per layer: reusing a buffer two layers apart would make the input
@@ -295,14 +311,7 @@ def lower_training_step(spec: MlpSpec, batch: int, optimizer, *, label_dtype: st
         dx_done = L > 1
     else:
         pb.index_ce(acts[L], lay.y, lay.loss, batch, out_w, grad=dz[L - 1])
-    common = {}
-    if kind == "sgd":
-        common = dict(lr=optimizer.learning_rate, momentum=optimizer.momentum,
-                      dampening=optimizer.dampening, weight_decay=optimizer.weight_decay,
-                      nesterov=optimizer.nesterov, has_momentum_slot=has_first)
-    else:
-        common = dict(lr=optimizer.learning_rate, beta1=optimizer.beta1, beta2=optimizer.beta2,
-                      eps=optimizer.epsilon, weight_decay=optimizer.weight_decay)
+    common = _update_arguments(optimizer, kind)
     fuse_update = FUSE_OPTIMIZER and mode == GradientMode.RESET_AND_STEP
     # backward. The two-stream plan keeps a step on the main stream when it depends on the main
     # stream's latest step, so the emission order shapes the schedule: first the chain of input
@@ -336,13 +345,9 @@ def lower_training_step(spec: MlpSpec, batch: int, optimizer, *, label_dtype: st
     if head_loss is not None:
         pb.ce_head_loss(*head_loss)  # nothing waits on the objective but the commit
     if mode != GradientMode.RESET_AND_STEP:
-        # G = accumulator + G for every tensor, each candidate checked finite
-        acc_entries = [(g, g, a, None, g.count) for g, a in zip(lay.grads, lay.accum)]
-        for i in range(0, len(acc_entries), 16):
-            pb.optimizer(lay.counter, acc_entries[i:i + 16], kind="acc_sum", phase=0, lr=0.0)
+        _accumulate(pb, lay, "acc_sum", 0)  # G = accumulator + G
         if mode == GradientMode.ACCUMULATE:
-            for i in range(0, len(acc_entries), 16):
-                pb.optimizer(lay.counter, acc_entries[i:i + 16], kind="acc_commit", phase=1, lr=0.0)
+            _accumulate(pb, lay, "acc_commit", 1)
             return pb, lay
     # one staged pass: current set -> candidate set, failures flagged; then the counter
     params_next = lay.weights_next + [b for b in lay.biases_next if b is not None]
@@ -354,14 +359,134 @@ def lower_training_step(spec: MlpSpec, batch: int, optimizer, *, label_dtype: st
                         lay.second[j] if lay.second else None, params_next[j],
                         lay.first_next[j] if has_first else None,
                         lay.second_next[j] if lay.second else None, p.count))
-    for i in range(0, len(entries), 16):
-        pb.optimizer(lay.counter, entries[i:i + 16], kind=kind, phase=2, **common)
+    _staged_updates(pb, lay, entries, kind, common)
     if uses_acc:
-        acc_entries = [(g, g, a, None, g.count) for g, a in zip(lay.grads, lay.accum)]
-        for i in range(0, len(acc_entries), 16):
-            pb.optimizer(lay.counter, acc_entries[i:i + 16], kind="acc_clear", phase=1, lr=0.0)
+        _accumulate(pb, lay, "acc_clear", 1)
     pb.step_commit(lay.counter)
     return pb, lay
+
+
+def _update_arguments(optimizer, kind: str) -> dict:
+    if kind == "sgd":
+        return dict(lr=optimizer.learning_rate, momentum=optimizer.momentum,
+                    dampening=optimizer.dampening, weight_decay=optimizer.weight_decay,
+                    nesterov=optimizer.nesterov, has_momentum_slot=optimizer.momentum != 0.0)
+    return dict(lr=optimizer.learning_rate, beta1=optimizer.beta1, beta2=optimizer.beta2,
+                eps=optimizer.epsilon, weight_decay=optimizer.weight_decay)
+
+
+def _lower_checkpointed(pb: ProgramBuilder, lay: TrainingLayout, spec: MlpSpec, batch: int,
+                        optimizer, kind: str, mode: str, uses_acc: bool, checkpoint: str) -> None:
+    """The steps of lower_training_step with the hidden outputs kept in 8 bits. Layers are taken
+    one after the other in both passes: the forward pass moves through two binary32 buffers, the
+    backward pass through two for the cotangents and, when the step updates at once, one for the
+    weight gradient under way."""
+    L, layers = len(spec.layers), spec.layers
+    if layers[-1].activation is not None:
+        raise ValueError("the loss heads are lowered for an identity output layer "
+                         "(cross-entropy consumes raw logits)")
+    steps_at_once = mode == GradientMode.RESET_AND_STEP
+    common = _update_arguments(optimizer, kind)
+    params = lay.weights + [b for b in lay.biases if b is not None]
+    bias_at = {}  # layer -> its bias's ordinal among the parameters
+    for i, b in enumerate(lay.biases):
+        if b is not None:
+            bias_at[i] = L + len(bias_at)
+    params_next = lay.weights_next + [b for b in lay.biases_next if b is not None]
+
+    def entry(j, grad):
+        return (params[j], grad, lay.first[j] if lay.first else None,
+                lay.second[j] if lay.second else None, params_next[j],
+                lay.first_next[j] if lay.first else None,
+                lay.second_next[j] if lay.second else None, params[j].count)
+
+    hidden = max(l.fan_out for l in layers[:-1])
+    out_w = layers[-1].fan_out
+    moving = [pb.internal(batch * hidden) for _ in range(min(2, L - 1))]
+    kept = [pb.mx_tensor(batch, l.fan_out, checkpoint) for l in layers[:-1]]
+    cotangent = [pb.internal(batch * max(hidden, out_w)) for _ in range(2)]
+    if steps_at_once:
+        one = pb.internal(max(l.fan_in * l.fan_out for l in layers[1:]))
+        gW = [None] + [one] * (L - 1)  # (the first layer's update is fused into its product)
+    else:
+        gW = [pb.internal(l.fan_in * l.fan_out) for l in layers]
+    gb = [pb.internal(l.fan_out) if l.bias else None for l in layers]
+    lay.grads = gW + [g for g in gb if g is not None]
+
+    # forward
+    cur = lay.x
+    for i, l in enumerate(layers[:-1]):
+        dst = moving[i % 2]
+        pb.gemm(cur, lay.weights[i], dst, batch, l.fan_out, l.fan_in, trans_b=True,
+                bias=lay.biases[i], act=l.activation)
+        pb.mx_encode(dst, kept[i], batch, l.fan_out, format=checkpoint, keep_nonzero=True)
+        cur = dst
+    # objective and its cotangent (g = 1)
+    last, dz = layers[-1], cotangent[(L - 1) % 2]
+    head_loss = None
+    if FUSE_CE_HEAD and spec.loss == "ce" and out_w <= 16:
+        row_loss = pb.internal(batch)
+        pb.ce_head(cur, lay.weights[L - 1], lay.y, dz, row_loss, batch, last.fan_in, out_w,
+                   bias=lay.biases[L - 1])
+        head_loss = (row_loss, lay.loss, batch)
+    else:
+        out = pb.internal(batch * out_w)
+        pb.gemm(cur, lay.weights[L - 1], out, batch, out_w, last.fan_in, trans_b=True,
+                bias=lay.biases[L - 1])
+        if spec.loss == "mse":
+            pb.mse(out, lay.y, lay.loss, batch * out_w, grad=dz, reduction=spec.reduction)
+        else:
+            pb.index_ce(out, lay.y, lay.loss, batch, out_w, grad=dz)
+    # backward: each layer's weight and bias gradients, then the cotangent of the layer below
+    if gb[L - 1] is not None:
+        pb.colsum(dz, gb[L - 1], batch, out_w)
+    for i in reversed(range(1, L)):
+        l, dz, below = layers[i], cotangent[i % 2], cotangent[(i - 1) % 2]
+        pb.mx_gemm(dz, kept[i - 1], gW[i], l.fan_out, l.fan_in, batch, format=checkpoint,
+                   trans_a=True)
+        if steps_at_once:
+            pb.optimizer(lay.counter, [entry(i, gW[i])], kind=kind, phase=2, **common)
+        pb.gemm(dz, lay.weights[i], below, batch, l.fan_in, l.fan_out)
+        pb.mx_act_grad(below, kept[i - 1], below, batch, l.fan_in, act=layers[i - 1].activation,
+                       format=checkpoint, colsum=gb[i - 1])
+    first = layers[0]
+    if steps_at_once:
+        e = entry(0, None)
+        pb.gemm_update(cotangent[0], lay.x, first.fan_out, first.fan_in, batch, lay.counter,
+                       (e[0], e[2], e[3], e[4], e[5], e[6]), kind=kind, trans_a=True, **common)
+    else:
+        pb.gemm(cotangent[0], lay.x, gW[0], first.fan_out, first.fan_in, batch, trans_a=True)
+    if head_loss is not None:
+        pb.ce_head_loss(*head_loss)
+    if not steps_at_once:
+        _accumulate(pb, lay, "acc_sum", 0)
+        if mode == GradientMode.ACCUMULATE:
+            _accumulate(pb, lay, "acc_commit", 1)
+            return
+        _staged_updates(pb, lay, [entry(j, lay.grads[j]) for j in range(len(params))], kind, common)
+    else:
+        _staged_updates(pb, lay, [entry(j, gb[i]) for i, j in bias_at.items()], kind, common)
+    if uses_acc:
+        _accumulate(pb, lay, "acc_clear", 1)
+    pb.step_commit(lay.counter)
+
+
+def _staged_updates(pb: ProgramBuilder, lay: TrainingLayout, entries: list, kind: str,
+                    common: dict) -> None:
+    """One staged pass over the entries: current set -> candidate set, failures flagged."""
+    for i in range(0, len(entries), 16):
+        pb.optimizer(lay.counter, entries[i:i + 16], kind=kind, phase=2, **common)
+
+
+def _accumulate(pb: ProgramBuilder, lay: TrainingLayout, kind: str, phase: int) -> None:
+    """An accumulator pass over every tensor: the sum (each candidate checked finite), its commit
+    or the clear."""
+    params = lay.weights + [b for b in lay.biases if b is not None]
+    # the clear of a step that updates at once has no stored gradient: the accumulator stands in
+    entries = [(g if g is not None and g.count == p.count else a,) * 2 + (a, None, p.count)
+               for g, a, p in zip(lay.grads, lay.accum, params)]
+    for i in range(0, len(entries), 16):
+        pb.optimizer(lay.counter, entries[i:i + 16], kind=kind, phase=phase, lr=0.0)
 
 
 def lower_forward(spec: MlpSpec, batch: int):
@@ -378,6 +503,60 @@ def lower_forward(spec: MlpSpec, batch: int):
                 act=l.activation)
         cur = dst
     return pb
+
+
+def lower_mx_weights(spec: MlpSpec, format: str = "e2m1"):
+    """Encodes a chain's weights for lower_mx_forward: inputs W_1..W_L; outputs codes and scales of
+    W_1, of W_2, and so on."""
+    pb = ProgramBuilder()
+    for l in spec.layers:
+        W = pb.input(l.fan_in * l.fan_out)
+        pb.mx_encode(W, pb.mx_tensor(l.fan_out, l.fan_in, format, "output"), l.fan_out, l.fan_in,
+                     format=format)
+    return pb
+
+
+def lower_mx_forward(spec: MlpSpec, batch: int, *, weights: str = "e2m1", activations: str = "e4m3"):
+    """Inference program of microscaled weights: inputs codes and scales of W_1..W_L (as
+    lower_mx_weights gives them), b_1..b_L, x; output prediction. Each layer's input is encoded in
+    the format `activations` on the way; sums, biases and activation functions are those of
+    lower_forward."""
+    pb = ProgramBuilder()
+    Ws = [pb.mx_tensor(l.fan_out, l.fan_in, weights, "input") for l in spec.layers]
+    bs = [pb.input(l.fan_out) if l.bias else None for l in spec.layers]
+    x = pb.input(batch * spec.layers[0].fan_in)
+    out = pb.output(batch * spec.layers[-1].fan_out)
+    cur = x
+    for i, l in enumerate(spec.layers):
+        dst = out if i == len(spec.layers) - 1 else pb.internal(batch * l.fan_out)
+        pb.mx_linear(cur, Ws[i], dst, batch, l.fan_out, l.fan_in, x_format=activations,
+                     w_format=weights, bias=bs[i], act=l.activation)
+        cur = dst
+    return pb
+
+
+def encode_mx_weights(ctx: HipContext, spec: MlpSpec, weights, format: str = "e2m1") -> list:
+    """A chain's weights (host arrays or buffers of the context, [out, in]) as the buffers that
+    lower_mx_forward's programs take first: codes and scales of W_1, of W_2, and so on. The bytes
+    of a weight come down from 4 to 0.53 (e2m1) or 1.03."""
+    if len(weights) != len(spec.layers):
+        raise ValueError("one weight matrix per layer is required")
+    bufs = []
+    for w, l in zip(weights, spec.layers):
+        if not isinstance(w, HipBuffer):
+            w = np.asarray(w, np.float32)
+            if w.shape != (l.fan_out, l.fan_in):
+                raise ValueError(f"weight shape {w.shape} does not match ({l.fan_out}, {l.fan_in})")
+            w = ctx.upload(w)
+        bufs.append(w)
+    pb = lower_mx_weights(spec, format)
+    outs = [ctx.buffer(s.nbytes) for s in pb.slots if s.kind == OUTPUT]
+    prog = HipProgram(ctx, pb.image())
+    try:
+        prog.run(bufs, outs)
+    finally:
+        prog.close()
+    return outs
 
 
 # ---- session ----
@@ -448,12 +627,13 @@ class HipTrainingSession:
     and writes the other, and the session adopts the written set only when the run succeeds."""
 
     def __init__(self, ctx: HipContext, spec: MlpSpec, weights, biases, optimizer, batch: int,
-                 *, label_dtype: str = "i64"):
+                 *, label_dtype: str = "i64", checkpoint: str | None = None):
         self.ctx = ctx
         self.spec = spec
         self.batch = batch
         self.optimizer = optimizer
         self.label_dtype = label_dtype
+        self.checkpoint = checkpoint  # see lower_training_step
         self._programs: dict[tuple, tuple[HipProgram, TrainingLayout]] = {}
         self._bindings: dict[tuple, object] = {}  # prepared handle arrays of the plain step
         self.program, lay = self._program(GradientMode.RESET_AND_STEP, False)
@@ -503,7 +683,7 @@ class HipTrainingSession:
         if key not in self._programs:
             pb, lay = lower_training_step(self.spec, self.batch, self.optimizer,
                                           label_dtype=self.label_dtype, mode=mode,
-                                          clear_accumulator=clear)
+                                          clear_accumulator=clear, checkpoint=self.checkpoint)
             self._programs[key] = (HipProgram(self.ctx, pb.image()), lay)
         return self._programs[key]
 
