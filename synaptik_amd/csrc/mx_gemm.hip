@@ -15,8 +15,6 @@
 namespace shk {
 namespace {
 
-int64_t pad256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-
 // ---- operands as matrix-instruction fragments ----
 // v_mfma_f32_32x32x16_bf16 takes from lane l the eight values k = 8 (l / 32) .. + 7 of row l mod 32.
 // Both operands are laid out as the 1 KB fragments it takes, 16 bytes a lane: fragment (kt, block,
@@ -41,18 +39,23 @@ struct Planes {
   uintx4 hi, mid, lo;
 };
 __device__ __forceinline__ Planes split8(const float (&v)[8]) {
-  uint32_t h[8], m[8], l[8];
+  uint32_t h[8], m[8], l[8], largest = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t b = __float_as_uint(v[i]);
-    h[i] = b & 0xffff0000u;
-    const float r = v[i] - __uint_as_float(h[i]);
-    m[i] = __float_as_uint(r) & 0xffff0000u;
-    l[i] = __float_as_uint(r - __uint_as_float(m[i]));
-    if (!is_finite(v[i])) {
-      h[i] = v[i] != v[i] ? b | 0x00400000u : b;
-      m[i] = l[i] = 0;
-    }
+    largest = max(largest, b & 0x7fffffffu);
+    h[i] = b;  // (its high half is cut out below)
+    const float r = v[i] - __uint_as_float(b & 0xffff0000u);
+    m[i] = __float_as_uint(r);
+    l[i] = __float_as_uint(r - __uint_as_float(m[i] & 0xffff0000u));
+  }
+  if (largest >= 0x7f800000u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!is_finite(v[i])) {
+        h[i] |= v[i] != v[i] ? 0x00400000u : 0u;
+        m[i] = l[i] = 0;
+      }
   }
   Planes p;
 #pragma unroll
@@ -102,6 +105,29 @@ __device__ __forceinline__ void pack_a_n(const float* __restrict__ a, int64_t ld
   put_planes(frag_at(pa, octet, m, MT, PLANES), split8(v));
 }
 
+// Four columns' codes of eight k (a word of four a k, and the scale) as the eight values of each
+// column.
+template <int F>
+__device__ __forceinline__ void fragments_of4(const uint32_t (&w)[8], const uint32_t (&scale)[8],
+                                              bf16x8 (&out)[4]) {
+  uint32_t lo[8], hi[8];  // columns 0, 1 and 2, 3
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo[i] = mx_values2<F, 0>(w[i], mx_scale_operand(scale[i]));
+    hi[i] = mx_values2<F, 1>(w[i], mx_scale_operand(scale[i]));
+  }
+  uintx4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[0][i] = __builtin_amdgcn_perm(lo[2 * i + 1], lo[2 * i], 0x05040100u);
+    v[1][i] = __builtin_amdgcn_perm(lo[2 * i + 1], lo[2 * i], 0x07060302u);
+    v[2][i] = __builtin_amdgcn_perm(hi[2 * i + 1], hi[2 * i], 0x05040100u);
+    v[3][i] = __builtin_amdgcn_perm(hi[2 * i + 1], hi[2 * i], 0x07060302u);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] = __builtin_bit_cast(bf16x8, v[j]);
+}
+
 // B's codes [K, N] as bfloat16 fragments: a lane takes four columns 4 q .. 4 q + 3 of a block and
 // eight k. Column 4 q + j is the fragment's row q + 8 j, so that eight lanes write 128 contiguous
 // bytes; the epilogue puts the columns back.
@@ -113,7 +139,7 @@ __device__ __forceinline__ void pack_b(const uint8_t* __restrict__ codes,
   const int64_t n = (bn * 64 + (threadIdx.x & 63)) * 4;
   const int64_t octet = bk * 4 + (threadIdx.x >> 6), k = 8 * octet;
   if (n >= N || (octet >> 1) >= (K + 15) / 16) return;
-  uint32_t w[8], sc[8], b[8][4];
+  uint32_t w[8], sc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t row = k + i < K ? k + i : K - 1;
@@ -121,21 +147,13 @@ __device__ __forceinline__ void pack_b(const uint8_t* __restrict__ codes,
     sc[i] = scales[row * G * 4 + n / 32];
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float f = mx_factor(sc[i]);
-    float v[4];
-    mx_values4<F>(w[i], v);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) b[i][j] = k + i < K ? __float_as_uint(v[j] * f) : 0u;
-  }
+  for (int i = 0; i < 8; ++i)
+    if (k + i >= K) w[i] = 0, sc[i] = 127;
+  bf16x8 out[4];
+  fragments_of4<F>(w, sc, out);
   char* at = frag_at(pb, octet, n / 32 * 32 + (n & 31) / 4, NT, 1);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uintx4 q;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = high_halves(b[2 * i][j], b[2 * i + 1][j]);
-    *reinterpret_cast<uintx4*>(at + 8 * 16 * j) = q;
-  }
+  for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8*>(at + 8 * 16 * j) = out[j];
 }
 
 // Both operands in one launch: workgroup (bk, y) packs 32 k of 64 rows of A, then of 256 columns
@@ -146,7 +164,7 @@ struct PackParams {
   const uint8_t* scales;
   char* pa;
   char* pb;
-  int64_t lda, M, N, K, MT, NT;
+  int64_t lda, M, N, K, G, MT, NT;
   int a_blocks;
 };
 template <int F, bool TA>
@@ -155,8 +173,7 @@ __global__ void __launch_bounds__(256) mx_pack(PackParams p) {
     if (TA) pack_a_t(p.A, p.lda, p.pa, p.M, p.K, p.MT, blockIdx.x, blockIdx.y);
     else pack_a_n(p.A, p.lda, p.pa, p.M, p.K, p.MT, blockIdx.x, blockIdx.y);
   } else {
-    pack_b<F>(p.codes, p.scales, p.pb, p.N, p.K, (p.N + MX_GROUP - 1) / MX_GROUP, p.NT, blockIdx.x,
-              blockIdx.y - p.a_blocks);
+    pack_b<F>(p.codes, p.scales, p.pb, p.N, p.K, p.G, p.NT, blockIdx.x, blockIdx.y - p.a_blocks);
   }
 }
 
@@ -297,7 +314,7 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
 }
 
 // The sum over the slices of a product split along K, in slice order.
-__global__ void __launch_bounds__(256) mx_wide_sum(const float* __restrict__ partial, int64_t plane,
+__global__ void __launch_bounds__(256) mx_gemm_sum(const float* __restrict__ partial, int64_t plane,
                                                    int slices, float* __restrict__ C, int64_t ldc,
                                                    int64_t N) {
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < plane; e += (int64_t)gridDim.x * 256) {
@@ -308,80 +325,245 @@ __global__ void __launch_bounds__(256) mx_wide_sum(const float* __restrict__ par
   }
 }
 
-// (the packing grids' second dimension)
-constexpr int64_t kMaxRows = 1 << 20;
+// ---- small products: operands straight into registers ----
+// A workgroup gives 16 MB rows and 64 columns; its waves take every W-th chunk of 32 k and their sums
+// are added in wave order. v_mfma_f32_16x16x32_bf16 takes from lane l the eight values k = 8 (l / 16)
+// .. + 7 of row or column l mod 16: the lane loads them of MB rows of A, splits them, and of four
+// columns of B (4 (l mod 16) + j is column l mod 16 of product j), whose codes lie four to a word, a
+// word for each k.
+template <bool TA>
+__device__ __forceinline__ void load_a8(const float* __restrict__ a, int64_t lda, int64_t m, int64_t k,
+                                        int64_t K, float (&v)[8]) {
+  if constexpr (TA) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? a[(k + i) * lda + m] : 0.0f;
+  } else if (k + 8 <= K) {
+    const float* src = a + m * lda + k;
+    const float4u x = *reinterpret_cast<const float4u*>(src), y = *reinterpret_cast<const float4u*>(src + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = x[i]; v[4 + i] = y[i]; }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? a[m * lda + k + i] : 0.0f;
+  }
+}
 
-struct WidePlan {
-  bool wide;
-  int tile, slices, chunk;
-  int64_t KT, MT, NT;
+struct DirectParams {
+  const float* A;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  float* C;  // or the partial sums [slices][M][N] of a product split along K
+  int64_t lda, ldc, plane, K, G;
+  int M, N, chunks, per_slice, row_tiles;
 };
-WidePlan plan(int64_t M, int64_t N, int64_t K) {
-  WidePlan w{};
-  w.KT = (K + 15) / 16;
-  w.MT = (M + 31) / 32;
-  w.NT = (N + 31) / 32;
-  auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-  w.wide = M >= 64 && N >= 64 && K >= 64 && (double)M * N * K >= (double)(1 << 27) &&
-           M <= kMaxRows && N <= kMaxRows;
-  w.tile = tiles(256) >= 128 ? 256 : 128;
-  const int64_t t = tiles(w.tile);
-  const int64_t s = t >= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(256 / t, w.KT / 8));
-  w.chunk = (int)((w.KT + s - 1) / s);
-  w.slices = w.chunk > 0 ? (int)((w.KT + w.chunk - 1) / w.chunk) : 1;
+template <int F, bool TA, int MB>
+__global__ void __launch_bounds__(512) mx_direct(DirectParams p) {
+  extern __shared__ __align__(16) float sums[];  // [waves][MB][4][64][4]
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int64_t n = (int64_t)(blockIdx.x / p.row_tiles) * 64 + 4 * c;
+  const int64_t m0 = (int64_t)(blockIdx.x % p.row_tiles) * (16 * MB);
+  const int last = min(p.chunks, (int)(blockIdx.y + 1) * p.per_slice);
+  floatx4 acc[MB][4];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int t = blockIdx.y * p.per_slice + wave; t < last; t += waves) {
+    const int64_t k = (int64_t)t * 32 + 8 * q;
+    uint32_t w[8], s[8];
+    float a[MB][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // (behind K the last row again, against zeros of A)
+      const int64_t row = min(k + i, p.K - 1);
+      w[i] = mx_load4<F>(p.codes, row * p.G * 32 + n / 4);
+      s[i] = p.scales[row * p.G * 4 + n / 32];
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+      load_a8<TA>(p.A, p.lda, min(m0 + 16 * i + c, (int64_t)p.M - 1), k, p.K, a[i]);
+    bf16x8 b[4];
+    fragments_of4<F>(w, s, b);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      const Planes x = split8(a[i]);
+      const bf16x8 parts[PLANES] = {__builtin_bit_cast(bf16x8, x.lo), __builtin_bit_cast(bf16x8, x.mid),
+                                    __builtin_bit_cast(bf16x8, x.hi)};
+#pragma unroll
+      for (int h = 0; h < PLANES; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(parts[h], b[j], acc[i][j], 0, 0, 0);
+    }
+  }
+  // register r of a lane: row 4 q + r, so that it holds four columns of four rows
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<floatx4*>(sums + (((wave * MB + i) * 4 + r) * 64 + lane) * 4) =
+          floatx4{acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]};
+  __syncthreads();
+  float* out = p.C + blockIdx.y * p.plane;
+  const int64_t n0 = (int64_t)(blockIdx.x / p.row_tiles) * 64;
+  for (int e = threadIdx.x; e < MB * 256; e += blockDim.x) {
+    floatx4 v = *reinterpret_cast<const floatx4*>(sums + e * 4);
+    for (int x = 1; x < waves; ++x) v += *reinterpret_cast<const floatx4*>(sums + (x * MB * 256 + e) * 4);
+    const int64_t row = m0 + (e >> 8) * 16 + ((e & 63) >> 4) * 4 + ((e >> 6) & 3);
+    const int64_t col = n0 + 4 * (e & 15);
+    if (row >= p.M) continue;
+    float* dst = out + row * p.ldc + col;
+    if (col + 4 <= p.N) {
+      *reinterpret_cast<float4u*>(dst) = float4u{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < p.N) dst[j] = v[j];
+    }
+  }
+}
+
+// How a product runs (us on MI355X, e4m3, a synchronous run's 13 us included):
+//   * straight into registers up to 5 * 2^28 multiply-adds (1024^3 30.0, packed 34.5; 500x1021x1531
+//     30.5 against 33.3; but 1500x1500x1000 52 against 46), and whatever the depth for up to 64 rows
+//     or 128 columns, where packing the other operand costs most (64x8192x8192 73 against 93,
+//     4096x128x4096 44 against 76; 128 rows, 128x4096x4096, 47 against 45); two row fragments a
+//     workgroup from 2^28 on (64x4096x4096 35 against 41 with one, but 300x300x1000 22.2 against 21.7);
+//   * packed on tiles of 256 when there is one for every CU (8192x8192x500 206 against 213 on tiles
+//     of 128; 4000x2900x2048, 192 tiles, 160 against 147).
+// Either is split along K into as many slices as bring 512 (256 tiles) workgroups, of at least two
+// chunks of 32 k a wave (eight fragments): 16x4096x4096 27 in eight, packed 1024^3 34.5 in four and
+// 40.5 whole.
+struct ProductPlan {
+  bool direct;
+  int mb, waves;            // direct: row fragments and waves a workgroup
+  int tile;                 // packed: its edge
+  int slices, chunk;        // chunk: chunks of 32 k, or fragments, of a slice
+  int64_t KT, MT, NT;       // packed: fragments along K, blocks of A and of B
+};
+ProductPlan plan(int64_t M, int64_t N, int64_t K) {
+  ProductPlan w{};
+  const double work = (double)M * (double)N * (double)K;
+  int64_t units, s;
+  if (work <= 5.0 * (1 << 28) || M <= 64 || N <= 128) {
+    w.direct = true;
+    w.mb = work >= (double)(1 << 28) ? 2 : 1;
+    units = (K + 31) / 32;
+    w.waves = (int)std::min<int64_t>(8, units);
+    const int64_t t = ((N + 63) / 64) * ((M + 16 * w.mb - 1) / (16 * w.mb));
+    s = std::min(512 / t, units / (2 * w.waves));
+  } else {
+    w.KT = units = (K + 15) / 16;
+    w.MT = (M + 31) / 32;
+    w.NT = (N + 31) / 32;
+    auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+    w.tile = tiles(256) >= 256 ? 256 : 128;
+    s = std::min(256 / tiles(w.tile), units / 8);
+  }
+  s = std::max<int64_t>(1, s);
+  w.chunk = (int)((units + s - 1) / s);
+  w.slices = (int)((units + w.chunk - 1) / w.chunk);
   return w;
+}
+
+// Rows and columns that one set of launches takes (grid dimensions); a multiple of a group.
+constexpr int64_t MAX_EXTENT = 1 << 20;
+
+int64_t piece_scratch_bytes(int64_t M, int64_t N, int64_t K) {
+  const ProductPlan w = plan(M, N, K);
+  return w.KT * (PLANES * w.MT + w.NT) * FRAG + (w.slices > 1 ? 4 * w.slices * M * N : 0);
+}
+
+// p.N columns of a B whose rows have G groups.
+hipError_t launch_piece(const MxGemmParams& p, int64_t G, void* scratch, hipStream_t s) {
+  const ProductPlan w = plan(p.M, p.N, p.K);
+  char* pa = static_cast<char*>(scratch);
+  char* pb = pa + w.KT * w.MT * PLANES * FRAG;
+  float* partial = reinterpret_cast<float*>(pb + w.KT * w.NT * FRAG);
+  float* sums = w.slices > 1 ? partial : p.C;
+  const int64_t ld_sums = w.slices > 1 ? p.N : p.ldc, plane = p.M * p.N;
+  if (w.direct) {
+    DirectParams d{};
+    d.A = p.A; d.codes = p.codes; d.scales = p.scales; d.C = sums;
+    d.lda = p.lda; d.ldc = ld_sums; d.plane = plane; d.K = p.K; d.G = G;
+    d.M = (int)p.M; d.N = (int)p.N; d.chunks = (int)((p.K + 31) / 32); d.per_slice = w.chunk;
+    d.row_tiles = (int)((p.M + 16 * w.mb - 1) / (16 * w.mb));
+    const dim3 grid((unsigned)((p.N + 63) / 64 * d.row_tiles), (unsigned)w.slices), block(64 * w.waves);
+    mx_with_format(p.format, [&](auto f) {
+      constexpr int F = decltype(f)::value;
+      auto go = [&](auto ta, auto mb) {
+        constexpr int MB = decltype(mb)::value;
+        hipLaunchKernelGGL((mx_direct<F, decltype(ta)::value, MB>), grid, block, w.waves * MB * 4096, s, d);
+      };
+      auto by_rows = [&](auto ta) {
+        if (w.mb == 1) go(ta, std::integral_constant<int, 1>());
+        else go(ta, std::integral_constant<int, 2>());
+      };
+      if (p.transA) by_rows(std::true_type());
+      else by_rows(std::false_type());
+    });
+  } else {
+    PackParams k{p.A, p.codes, p.scales, pa, pb, p.lda, p.M, p.N, p.K, G, w.MT, w.NT, (int)((p.M + 63) / 64)};
+    const dim3 packs((unsigned)((w.KT + 1) / 2), (unsigned)(k.a_blocks + (p.N + 255) / 256));
+    mx_with_format(p.format, [&](auto f) {
+      constexpr int F = decltype(f)::value;
+      if (p.transA) hipLaunchKernelGGL((mx_pack<F, true>), packs, dim3(256), 0, s, k);
+      else hipLaunchKernelGGL((mx_pack<F, false>), packs, dim3(256), 0, s, k);
+    });
+    WideParams q{};
+    q.pa = pa; q.pb = pb; q.C = sums;
+    q.ldc = ld_sums; q.plane = plane;
+    q.M = (int)p.M; q.N = (int)p.N;
+    q.KT = (int)w.KT; q.MT = (int)w.MT; q.NT = (int)w.NT;
+    q.tiles_m = (int)((p.M + w.tile - 1) / w.tile);
+    q.tiles_n = (int)((p.N + w.tile - 1) / w.tile);
+    q.chunk = w.chunk;
+    const dim3 grid((unsigned)(q.tiles_m * q.tiles_n), (unsigned)w.slices);
+    if (w.tile == 256) hipLaunchKernelGGL((mx_wide<256, 256, 4, 2, 4>), grid, dim3(512), 0, s, q);
+    else hipLaunchKernelGGL((mx_wide<128, 128, 4, 2, 4>), grid, dim3(512), 0, s, q);
+  }
+  if (w.slices > 1)
+    hipLaunchKernelGGL(mx_gemm_sum, dim3((unsigned)std::min<int64_t>(8192, (plane + 255) / 256)), dim3(256),
+                       0, s, partial, plane, w.slices, p.C, p.ldc, p.N);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t mx_gemm_scratch_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0) return 0;
-  const WidePlan w = plan(M, N, K);
-  if (!w.wide) return pad256(4 * K * N) + 4 * gemm_workspace_floats(M, N, K);
-  return w.KT * (PLANES * w.MT + w.NT) * FRAG + (w.slices > 1 ? 4 * w.slices * M * N : 0);
+  if (K == 0) return 4 * gemm_workspace_floats(M, N, K);
+  int64_t bytes = 0;  // whole pieces and the last ones
+  for (int64_t m : {std::min(M, MAX_EXTENT), M % MAX_EXTENT})
+    for (int64_t n : {std::min(N, MAX_EXTENT), N % MAX_EXTENT})
+      if (m > 0 && n > 0) bytes = std::max(bytes, piece_scratch_bytes(m, n, K));
+  return bytes;
 }
 
-hipError_t launch_mx_gemm(const MxGemmParams& p, void* scratch, hipStream_t s) {
-  if (p.M <= 0 || p.N <= 0) return hipSuccess;
-  const WidePlan w = plan(p.M, p.N, p.K);
-  if (!w.wide) {
-    float* b = static_cast<float*>(scratch);
-    const hipError_t e = launch_mx_decode(p.codes, p.scales, b, p.N, p.K, p.N, p.format, s);
-    if (e != hipSuccess) return e;
+hipError_t launch_mx_gemm(const MxGemmParams& in, void* scratch, hipStream_t s) {
+  if (in.M <= 0 || in.N <= 0) return hipSuccess;
+  if (in.K == 0) {  // no products: zeros
     GemmParams g{};
-    g.A = p.A; g.B = b; g.C = p.C;
-    g.M = p.M; g.N = p.N; g.K = p.K;
-    g.lda = p.lda; g.ldb = p.N; g.ldc = p.ldc;
-    g.transA = p.transA;
-    return launch_gemm(g, reinterpret_cast<float*>(static_cast<char*>(scratch) + pad256(4 * p.K * p.N)), s);
+    g.A = g.B = in.A;
+    g.C = in.C;
+    g.M = in.M; g.N = in.N;
+    g.ldc = in.ldc;
+    return launch_gemm(g, static_cast<float*>(scratch), s);
   }
-  char* pa = static_cast<char*>(scratch);
-  char* pb = pa + w.KT * w.MT * PLANES * FRAG;
-  float* partial = reinterpret_cast<float*>(pb + w.KT * w.NT * FRAG);
-  PackParams k{p.A, p.codes, p.scales, pa, pb, p.lda, p.M, p.N, p.K, w.MT, w.NT, (int)((p.M + 63) / 64)};
-  const dim3 packs((unsigned)((w.KT + 1) / 2), (unsigned)(k.a_blocks + (p.N + 255) / 256));
-  mx_with_format(p.format, [&](auto f) {
-    constexpr int F = decltype(f)::value;
-    if (p.transA) hipLaunchKernelGGL((mx_pack<F, true>), packs, dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((mx_pack<F, false>), packs, dim3(256), 0, s, k);
-  });
-  WideParams q{};
-  q.pa = pa; q.pb = pb;
-  q.C = w.slices > 1 ? partial : p.C;
-  q.ldc = w.slices > 1 ? p.N : p.ldc;
-  q.plane = p.M * p.N;
-  q.M = (int)p.M; q.N = (int)p.N;
-  q.KT = (int)w.KT; q.MT = (int)w.MT; q.NT = (int)w.NT;
-  q.tiles_m = (int)((p.M + w.tile - 1) / w.tile);
-  q.tiles_n = (int)((p.N + w.tile - 1) / w.tile);
-  q.chunk = w.chunk;
-  const dim3 grid((unsigned)(q.tiles_m * q.tiles_n), (unsigned)w.slices);
-  if (w.tile == 256) hipLaunchKernelGGL((mx_wide<256, 256, 4, 2, 4>), grid, dim3(512), 0, s, q);
-  else hipLaunchKernelGGL((mx_wide<128, 128, 2, 2, 4>), grid, dim3(256), 0, s, q);
-  if (w.slices > 1)
-    hipLaunchKernelGGL(mx_wide_sum, dim3((unsigned)std::min<int64_t>(8192, (q.plane + 255) / 256)),
-                       dim3(256), 0, s, partial, q.plane, w.slices, p.C, p.ldc, p.N);
-  return hipGetLastError();
+  for (int64_t m = 0; m < in.M; m += MAX_EXTENT)
+    for (int64_t n = 0; n < in.N; n += MAX_EXTENT) {
+      MxGemmParams p = in;
+      p.M = std::min(MAX_EXTENT, in.M - m);
+      p.N = std::min(MAX_EXTENT, in.N - n);
+      p.A += in.transA ? m : m * in.lda;
+      p.codes += n / MX_GROUP * mx_group_bytes(in.format);
+      p.scales += n / MX_BLOCK;
+      p.C += m * in.ldc + n;
+      const hipError_t e = launch_piece(p, mx_groups(in.N), scratch, s);
+      if (e != hipSuccess) return e;
+    }
+  return hipSuccess;
 }
 
 }  // namespace shk

@@ -46,21 +46,6 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
   return F == MX_E2M1 && largest >= 0x7f800000u ? 255u : mx_scale_of<F>(largest);
 }
 
-// Two values as bfloat16, by the conversion that scales (exact, and NaN under the scale 255): those
-// of the low or high half of a word of four 8-bit codes, or of byte PART of a word of eight e2m1
-// codes.
-template <int F, int PART>
-__device__ __forceinline__ uint32_t values2(uint32_t w, float scale) {
-  if constexpr (F == MX_E2M1)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, PART));
-  else if constexpr (F == MX_E4M3)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, PART != 0));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, scale, PART != 0));
-}
-// The scale operand of a byte: the conversion reads its exponent, and NaN in an infinity's.
-__device__ __forceinline__ float scale_operand(uint32_t s) { return __uint_as_float(s << 23); }
-
 // A block of 32 codes; eight(i): its values 8 i .. 8 i + 7.
 template <int F>
 struct Codes {
@@ -76,11 +61,11 @@ struct Codes {
   __device__ __forceinline__ bf16x8 eight(int i, float scale) const {
     uintx4 r;
     if constexpr (F == MX_E2M1)
-      r = uintx4{values2<F, 0>(w[i], scale), values2<F, 1>(w[i], scale), values2<F, 2>(w[i], scale),
-                 values2<F, 3>(w[i], scale)};
+      r = uintx4{mx_values2<F, 0>(w[i], scale), mx_values2<F, 1>(w[i], scale), mx_values2<F, 2>(w[i], scale),
+                 mx_values2<F, 3>(w[i], scale)};
     else
-      r = uintx4{values2<F, 0>(w[2 * i], scale), values2<F, 1>(w[2 * i], scale),
-                 values2<F, 0>(w[2 * i + 1], scale), values2<F, 1>(w[2 * i + 1], scale)};
+      r = uintx4{mx_values2<F, 0>(w[2 * i], scale), mx_values2<F, 1>(w[2 * i], scale),
+                 mx_values2<F, 0>(w[2 * i + 1], scale), mx_values2<F, 1>(w[2 * i + 1], scale)};
     return __builtin_bit_cast(bf16x8, r);
   }
 };
@@ -130,7 +115,7 @@ __device__ __forceinline__ void encode_rows(const LinearParams& p, char* lds) {
     const uint32_t s = scale_byte<FX>(mx_block_largest(largest));
     // (a lost block's reciprocal is of no account: its scale makes it NaN)
     const uint32_t c = mx_codes4<FX, false>(v, mx_reciprocal(min(s, 254u)));
-    const uint2 out = {values2<FX, 0>(c, scale_operand(s)), values2<FX, 1>(c, scale_operand(s))};
+    const uint2 out = {mx_values2<FX, 0>(c, mx_scale_operand(s)), mx_values2<FX, 1>(c, mx_scale_operand(s))};
     reinterpret_cast<uint2*>(lds)[t * 32 + q] = out;
   }
 }
@@ -179,7 +164,7 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (g0 + u * waves >= p.G) break;
-      const float wf = scale_operand(ws[u]);
+      const float wf = mx_scale_operand(ws[u]);
       bf16x8 a[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = w[u].eight(i, wf);
@@ -191,7 +176,7 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
       } else {
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-          const float xf = scale_operand(xs[u][i]);
+          const float xf = mx_scale_operand(xs[u][i]);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], x[u][i].eight(j, xf), acc[i], 0, 0, 0);
@@ -408,9 +393,9 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_linear_tile(TileParams t) {
     } else {
       float sx[TM], sw[TN];
 #pragma unroll
-      for (int i = 0; i < TM; ++i) sx[i] = scale_operand((s.x[i] >> (16 * H)) & 0xffu);
+      for (int i = 0; i < TM; ++i) sx[i] = mx_scale_operand((s.x[i] >> (16 * H)) & 0xffu);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) sw[j] = scale_operand((s.w[j] >> (16 * H)) & 0xffu);
+      for (int j = 0; j < TN; ++j) sw[j] = mx_scale_operand((s.w[j] >> (16 * H)) & 0xffu);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         bf16x8 a[TM], b[TN];

@@ -11,6 +11,21 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
+// Two values as bfloat16, by the conversion that scales (exact, and NaN under the scale 255): those
+// of the low or high half of a word of four 8-bit codes, or of byte PART of a word of eight e2m1
+// codes.
+template <int F, int PART>
+__device__ __forceinline__ uint32_t mx_values2(uint32_t w, float scale) {
+  if constexpr (F == MX_E2M1)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, PART));
+  else if constexpr (F == MX_E4M3)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, PART != 0));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, scale, PART != 0));
+}
+// The scale operand of a byte: the conversion reads its exponent, and NaN in an infinity's.
+__device__ __forceinline__ float mx_scale_operand(uint32_t s) { return __uint_as_float(s << 23); }
+
 // Workgroup -> tile: tiles in bands of four rows of tiles, and each of the eight XCDs (workgroups
 // go to them in turn) a contiguous run of that order, so that an XCD's second-level cache serves
 // few rows and columns of tiles.
