@@ -97,15 +97,17 @@ __global__ void __launch_bounds__(256) mx_decode(const uint8_t* __restrict__ cod
   }
 }
 
-// dZ = act_grad(dY, Y) from Y's codes, and with `partial` the column sums of this workgroup's
-// rows in binary64 (row blockIdx.y of [gridDim.y, C]). A workgroup takes 256 columns and `rows`
-// rows, its four waves every fourth one; dy and dz may be the same memory.
+// dZ = act_grad(dY, Y) from Y's codes, and the column sums of this workgroup's rows in binary64:
+// PARTIAL as row blockIdx.y of [gridDim.y, C], WHOLE (one row of workgroups) rounded into the
+// result. A workgroup takes 256 columns and `rows` rows, its four waves every fourth one; dy and dz
+// may be the same memory.
 constexpr int AG_COLS = 256, AG_UNROLL = 4;
-template <int F, int ACT, bool SUM>
+enum Sums { NO_SUMS, PARTIAL, WHOLE };
+template <int F, int ACT, int SUMS>
 __global__ void __launch_bounds__(256) mx_act_grad(const float* dy, int64_t ldy,
                                                    const uint8_t* __restrict__ codes,
                                                    const uint8_t* __restrict__ scales, float* dz,
-                                                   int64_t ldz, double* __restrict__ partial,
+                                                   int64_t ldz, void* __restrict__ sums,
                                                    int64_t R, int C, int64_t G, int64_t rows) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t c = (int64_t)blockIdx.x * AG_COLS + 4 * lane;
@@ -133,13 +135,13 @@ __global__ void __launch_bounds__(256) mx_act_grad(const float* dy, int64_t ldy,
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           g[u][i] = act_grad(ACT, g[u][i], y[i] * f);
-          if (SUM) sum[i] += (double)g[u][i];
+          if (SUMS != NO_SUMS) sum[i] += (double)g[u][i];
         }
         store4(dz + r * ldz + c, rest, g[u]);
       }
     }
   }
-  if constexpr (SUM) {
+  if constexpr (SUMS != NO_SUMS) {
     __shared__ double wave_sums[3][AG_COLS];
     if (w > 0) {
 #pragma unroll
@@ -147,21 +149,26 @@ __global__ void __launch_bounds__(256) mx_act_grad(const float* dy, int64_t ldy,
     }
     __syncthreads();
     if (w == 0) {
-      double* out = partial + (int64_t)blockIdx.y * C + c;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = 4 * lane + i;
-        if (i < rest) out[i] = ((sum[i] + wave_sums[0][j]) + wave_sums[1][j]) + wave_sums[2][j];
+        const double v = ((sum[i] + wave_sums[0][j]) + wave_sums[1][j]) + wave_sums[2][j];
+        if (i >= rest) continue;
+        if (SUMS == WHOLE) static_cast<float*>(sums)[c + i] = (float)v;
+        else static_cast<double*>(sums)[(int64_t)blockIdx.y * C + c + i] = v;
       }
     }
   }
 }
 
 // Rows a workgroup of mx_act_grad takes: 16 (four a wave, all in flight at once), more when that
-// would be over 2048 workgroups.
+// would be over 1024 workgroups (4096x4096 with sums, a run of 13 us included: 46.4 / 44.0 / 47.5 /
+// 50.6 us for 512 / 1024 / 2048 / 4096 workgroups; 26 us for 145 MB are 5.6 TB/s), and up to 64
+// rows one workgroup, which then needs no second launch for the sums.
 int64_t act_grad_rows(int64_t R, int64_t C) {
+  if (R <= 64) return 64;
   const int64_t strips = (C + AG_COLS - 1) / AG_COLS;
-  const int64_t slabs = std::max<int64_t>(1, 2048 / strips);
+  const int64_t slabs = std::max<int64_t>(1, 1024 / strips);
   const int64_t rows = (R + slabs - 1) / slabs;
   return std::max<int64_t>(16, (rows + 15) / 16 * 16);
 }
@@ -233,12 +240,13 @@ hipError_t launch_mx_act_grad(const float* dy, int64_t ldy, const uint8_t* codes
       constexpr int F = decltype(f)::value;
       auto go = [&](auto a) {
         constexpr int ACT = decltype(a)::value;
-        if (colsum != nullptr)
-          hipLaunchKernelGGL((mx_act_grad<F, ACT, true>), grid, dim3(256), 0, s, dy, ldy, codes, scales,
-                             dz, ldz, partial, R, (int)C, G, rows);
-        else
-          hipLaunchKernelGGL((mx_act_grad<F, ACT, false>), grid, dim3(256), 0, s, dy, ldy, codes,
-                             scales, dz, ldz, partial, R, (int)C, G, rows);
+        auto with = [&](auto sums, void* to) {
+          hipLaunchKernelGGL((mx_act_grad<F, ACT, decltype(sums)::value>), grid, dim3(256), 0, s, dy, ldy,
+                             codes, scales, dz, ldz, to, R, (int)C, G, rows);
+        };
+        if (colsum == nullptr) with(std::integral_constant<int, NO_SUMS>(), nullptr);
+        else if (slabs == 1) with(std::integral_constant<int, WHOLE>(), colsum);
+        else with(std::integral_constant<int, PARTIAL>(), partial);
       };
       switch (act) {
         case ACT_RELU: go(std::integral_constant<int, ACT_RELU>()); break;
@@ -250,7 +258,7 @@ hipError_t launch_mx_act_grad(const float* dy, int64_t ldy, const uint8_t* codes
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (colsum == nullptr) return hipSuccess;
+  if (colsum == nullptr || slabs == 1) return hipSuccess;
   return launch_colsum_finish(partial, colsum, slabs, C, s);
 }
 

@@ -128,7 +128,7 @@ def test_rows_further_apart_than_their_width(ctx):
 @pytest.mark.parametrize("act", [None, "relu", "tanh", "sigmoid"])
 @pytest.mark.parametrize("shape,format", [((1, 1), "e4m3"), ((2, 5), "e5m2"), ((16, 256), "e4m3"),
                                           ((17, 257), "e2m1"), ((300, 130), "e4m3"),
-                                          ((1, 3001), "e5m2"), ((70000, 3), "e4m3"),
+                                          ((64, 70), "e4m3"), ((65, 70), "e4m3"), ((1, 3001), "e5m2"), ((70000, 3), "e4m3"),
                                           ((1000, 1100), "e4m3")], ids=str)
 def test_activation_gradient_from_a_checkpoint(ctx, shape, format, act):
     R, C = shape
@@ -224,7 +224,7 @@ def test_product_of_a_microscaled_operand(ctx, shape, format, trans_a):
 
 
 @pytest.mark.parametrize("trans_a", [False, True])
-@pytest.mark.parametrize("size", [40, 520])
+@pytest.mark.parametrize("size", [40, 520, 1201])
 def test_product_keeps_every_bit_of_the_wide_operand(ctx, size, trans_a):
     """One nonzero a row of A: each result is a single product, off by the rounding of the few
     additions of its exact parts (three, each cut off at worst: 6 u)."""
@@ -239,9 +239,21 @@ def test_product_keeps_every_bit_of_the_wide_operand(ctx, size, trans_a):
 
 
 @pytest.mark.parametrize("trans_a", [False, True])
+def test_products_longer_than_a_piece(ctx, trans_a):
+    """More rows, and more columns, than one set of launches takes."""
+    rng = np.random.default_rng(1)
+    for M, N, K in (((1 << 20) + 37, 5, 6), (3, (1 << 20) + 200, 2)):
+        A = rng.standard_normal((M, K)).astype(np.float32)
+        codes, scales, B = mx.stored(rng.standard_normal((K, N)), "e2m1")
+        got = gpu_mx_gemm(ctx, A.T if trans_a else A, codes, scales, M, N, K, "e2m1", trans_a)
+        A = A.astype(np.float64)
+        assert (np.abs(got - A @ B) <= 2 * (3 * K + 1) * U * (np.abs(A) @ np.abs(B))).all()
+
+
+@pytest.mark.parametrize("trans_a", [False, True])
 def test_product_with_strides_and_a_matrix_of_no_depth(ctx, trans_a):
     rng = np.random.default_rng(11)
-    for M, N, K, pad_a, ldc in ((45, 70, 130, 9, 77), (600, 530, 520, 3, 531)):
+    for M, N, K, pad_a, ldc in ((45, 70, 130, 9, 77), (600, 530, 520, 3, 531), (1150, 1290, 1203, 5, 1295)):
         shape = (K, M) if trans_a else (M, K)
         wide = rng.standard_normal((shape[0], shape[1] + pad_a)).astype(np.float32)
         A = wide[:, :shape[1]]
@@ -254,7 +266,7 @@ def test_product_with_strides_and_a_matrix_of_no_depth(ctx, trans_a):
     assert np.array_equal(got, np.zeros((5, 6), np.float32))
 
 
-@pytest.mark.parametrize("size", [48, 560])
+@pytest.mark.parametrize("size", [48, 560, 1209])
 def test_product_with_infinities_and_nans(ctx, size):
     """A value that is not finite makes every result that it contributes to not finite, and no
     other; a masked sample's row of zeros gives zeros."""
@@ -333,6 +345,28 @@ def test_linear_layer_of_microscaled_weights(ctx, shape, w_format, x_format):
     assert (np.abs(got - mx.activate(act, z)) <= linear_room(Xq, W, b, act, z)).all()
 
 
+@pytest.mark.parametrize("x_format", mx.FORMATS)
+@pytest.mark.parametrize("w_format", mx.FORMATS)
+@pytest.mark.parametrize("shape", [(3, 50, 700), (40, 50, 700), (1100, 1050, 1000)], ids=str)
+def test_linear_layer_of_blocks_of_different_sizes(ctx, shape, w_format, x_format):
+    """Blocks 24 binades apart beside each other, on both sides: the small ones' products still count
+    to binary32 where the large ones of the other side are small or zero."""
+    M, N, K = shape
+    rng = np.random.default_rng(K + M)
+    blocks = -(-K // 32)
+
+    def spread(rows):
+        f = np.exp2(rng.choice([-24, -12, 0], (rows, blocks))) * (rng.random((rows, blocks)) < 0.7)
+        return rng.standard_normal((rows, K)) * np.repeat(f, 32, axis=1)[:, :K]
+
+    X = spread(M).astype(np.float32)
+    codes, scales, W = mx.stored(spread(N), w_format)
+    Xq = mx.stored(X, x_format)[2]
+    got = gpu_mx_linear(ctx, X, (codes, scales), None, M, N, K, x_format, w_format, None)
+    z = Xq @ W.T
+    assert (np.abs(got - z) <= linear_room(Xq, W, np.zeros(N), None, z)).all()
+
+
 def test_linear_layer_with_strides_and_without_depth(ctx):
     rng = np.random.default_rng(2)
     for M, ldx, N, ldy in ((1, 200, 150, 161), (7, 203, 150, 161), (40, 201, 150, 161),
@@ -349,6 +383,18 @@ def test_linear_layer_with_strides_and_without_depth(ctx):
     for M in (1, 40):
         got = gpu_mx_linear(ctx, np.zeros(0, np.float32), (e, e), bias, M, 9, 0, "e4m3", "e2m1", "relu")
         assert np.array_equal(got, np.tile(np.maximum(bias, 0), (M, 1)))
+
+
+def test_linear_layers_longer_than_a_piece(ctx):
+    rng = np.random.default_rng(6)
+    for M, N, K in (((1 << 20) + 37, 3, 8), (2, (1 << 20) + 70, 5)):
+        X = rng.standard_normal((M, K)).astype(np.float32)
+        codes, scales, W = mx.stored(rng.standard_normal((N, K)), "e4m3")
+        bias = rng.standard_normal(N).astype(np.float32)
+        got = gpu_mx_linear(ctx, X, (codes, scales), bias, M, N, K, "e4m3", "e4m3", "relu")
+        Xq = mx.stored(X, "e4m3")[2]
+        z = Xq @ W.T + bias
+        assert (np.abs(got - np.maximum(z, 0)) <= linear_room(Xq, W, bias, "relu", z)).all()
 
 
 @pytest.mark.parametrize("x_format,w_format", [("e4m3", "e2m1"), ("e2m1", "e2m1"), ("e5m2", "e4m3"),
