@@ -8,6 +8,9 @@
 // of three bfloat16 products whose terms are exact, accumulated in binary32: what a binary32
 // product gives (each term rounded no more often), at a third of the bfloat16 matrix cores' rate
 // instead of the binary32 ones', 5.3 times as fast (2.5 / 3 against 0.157 PFLOP/s).
+// The matrix cores read subnormal bfloat16 values as zeros, so a value of A counts with an error
+// below 2^-126, the smallest normal binary32 value: the first part that is read as zero is below
+// it, and so is all that the part leads. (B's values are normal: scales start at 2^-110.)
 #include <algorithm>
 
 #include "mx_tiles.h"

@@ -238,6 +238,25 @@ def test_product_keeps_every_bit_of_the_wide_operand(ctx, size, trans_a):
     assert (np.abs(got - want) <= 6 * U * np.abs(want)).all()
 
 
+@pytest.mark.parametrize("size", [40, 520, 1201])
+def test_product_of_the_smallest_wide_values(ctx, size):
+    """Wide values down to the least subnormal one, against large microscaled values.
+
+    The matrix cores read subnormal bfloat16 values as zeros. Of a wide value's three exact parts,
+    each the leading eight bits of what the ones before it leave, those read as zeros are the last
+    ones; the first of them is below 2^-126, so what it leads, the sum of it and the ones behind it,
+    is too (2^-126 has one bit: a remainder of at least 2^-126 leads with at least 2^-126). A wide
+    value therefore counts with an error below 2^-126."""
+    rng = np.random.default_rng(size)
+    M = N = K = size
+    A = np.ldexp(rng.integers(-(1 << 24), 1 << 24, (M, K)), rng.integers(-149, -130, (M, 1))).astype(np.float32)
+    codes, scales, B = mx.stored(np.ldexp(rng.standard_normal((K, N)), 100), "e4m3")
+    room = 2 * (3 * K + 1) * U * (np.abs(A).astype(np.float64) @ np.abs(B)) + 2.0 ** -126 * np.abs(B).sum(0)
+    for trans_a in (False, True):
+        got = gpu_mx_gemm(ctx, A.T if trans_a else A, codes, scales, M, N, K, "e4m3", trans_a)
+        assert (np.abs(got - A.astype(np.float64) @ B) <= room).all()
+
+
 @pytest.mark.parametrize("trans_a", [False, True])
 def test_products_longer_than_a_piece(ctx, trans_a):
     """More rows, and more columns, than one set of launches takes."""
