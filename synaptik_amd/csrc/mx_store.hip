@@ -99,35 +99,36 @@ __global__ void __launch_bounds__(256) mx_decode(const uint8_t* __restrict__ cod
 
 // dZ = act_grad(dY, Y) from Y's codes, and the column sums of this workgroup's rows in binary64:
 // PARTIAL as row blockIdx.y of [gridDim.y, C], WHOLE (one row of workgroups) rounded into the
-// result. A workgroup takes 256 columns and `rows` rows, its four waves every fourth one; dy and dz
-// may be the same memory.
-constexpr int AG_COLS = 256, AG_UNROLL = 4;
+// result. A workgroup takes 4 Q columns and `rows` rows, Q lanes a row: 256 columns and four rows at
+// once where its sums are partial, 32 columns (one line of memory) and 128 rows at once where they
+// are whole. dy and dz may be the same memory.
+constexpr int AG_UNROLL = 4;
 enum Sums { NO_SUMS, PARTIAL, WHOLE };
 template <int F, int ACT, int SUMS>
-__global__ void __launch_bounds__(256) mx_act_grad(const float* dy, int64_t ldy,
-                                                   const uint8_t* __restrict__ codes,
-                                                   const uint8_t* __restrict__ scales, float* dz,
-                                                   int64_t ldz, void* __restrict__ sums,
-                                                   int64_t R, int C, int64_t G, int64_t rows) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * AG_COLS + 4 * lane;
+__global__ void __launch_bounds__(SUMS == WHOLE ? 1024 : 256)
+    mx_act_grad(const float* dy, int64_t ldy, const uint8_t* __restrict__ codes,
+                const uint8_t* __restrict__ scales, float* dz, int64_t ldz, void* __restrict__ sums,
+                int64_t R, int C, int64_t G, int64_t rows) {
+  constexpr int Q = SUMS == WHOLE ? 8 : 64, AT_ONCE = SUMS == WHOLE ? 128 : 4;
+  const int quad = threadIdx.x % Q, w = threadIdx.x / Q;
+  const int64_t c = (int64_t)blockIdx.x * (4 * Q) + 4 * quad;
   const int rest = (int)min((int64_t)4, C - c);
   const int64_t last = min(R, ((int64_t)blockIdx.y + 1) * rows);
   double sum[4] = {0.0, 0.0, 0.0, 0.0};
   if (rest > 0) {
-    for (int64_t r0 = (int64_t)blockIdx.y * rows + w; r0 < last; r0 += 4 * AG_UNROLL) {
+    for (int64_t r0 = (int64_t)blockIdx.y * rows + w; r0 < last; r0 += AT_ONCE * AG_UNROLL) {
       float g[AG_UNROLL][4];
       uint32_t code[AG_UNROLL], s[AG_UNROLL];
 #pragma unroll
       for (int u = 0; u < AG_UNROLL; ++u) {
-        const int64_t r = min(r0 + 4 * u, last - 1);
+        const int64_t r = min(r0 + AT_ONCE * u, last - 1);
         load4(dy + r * ldy + c, rest, g[u]);
         code[u] = mx_load4<F>(codes, r * G * 32 + c / 4);
         s[u] = scales[r * G * 4 + c / 32];
       }
 #pragma unroll
       for (int u = 0; u < AG_UNROLL; ++u) {
-        const int64_t r = r0 + 4 * u;
+        const int64_t r = r0 + AT_ONCE * u;
         if (r >= last) break;
         const float f = mx_factor(s[u]);
         float y[4];
@@ -142,33 +143,42 @@ __global__ void __launch_bounds__(256) mx_act_grad(const float* dy, int64_t ldy,
     }
   }
   if constexpr (SUMS != NO_SUMS) {
-    __shared__ double wave_sums[3][AG_COLS];
-    if (w > 0) {
+    // the rows of a wave, then the waves in order
+    constexpr int WAVES = SUMS == WHOLE ? 16 : 4;
+    __shared__ double wave_sums[WAVES][4 * Q];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) wave_sums[w - 1][4 * lane + i] = sum[i];
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int o = Q; o < 64; o *= 2) sum[i] += __shfl_xor(sum[i], o, 64);
+    }
+    if ((threadIdx.x & 63) < Q) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wave_sums[threadIdx.x >> 6][4 * quad + i] = sum[i];
     }
     __syncthreads();
-    if (w == 0) {
+    const int64_t col = (int64_t)blockIdx.x * (4 * Q) + threadIdx.x;
+    if (threadIdx.x < 4 * Q && col < C) {
+      double v = wave_sums[0][threadIdx.x];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 4 * lane + i;
-        const double v = ((sum[i] + wave_sums[0][j]) + wave_sums[1][j]) + wave_sums[2][j];
-        if (i >= rest) continue;
-        if (SUMS == WHOLE) static_cast<float*>(sums)[c + i] = (float)v;
-        else static_cast<double*>(sums)[(int64_t)blockIdx.y * C + c + i] = v;
-      }
+      for (int i = 1; i < WAVES; ++i) v += wave_sums[i][threadIdx.x];
+      if (SUMS == WHOLE) static_cast<float*>(sums)[col] = (float)v;
+      else static_cast<double*>(sums)[(int64_t)blockIdx.y * C + col] = v;
     }
   }
 }
 
-// Rows a workgroup of mx_act_grad takes: 16 (four a wave, all in flight at once), more when that
-// would be over 1024 workgroups (4096x4096 with sums, a run of 13 us included: 46.4 / 44.0 / 47.5 /
-// 50.6 us for 512 / 1024 / 2048 / 4096 workgroups; 26 us for 145 MB are 5.6 TB/s), and up to 64
-// rows one workgroup, which then needs no second launch for the sums.
+// Whether one workgroup takes all rows of its columns, whose sums then need no second launch (us, a
+// run's 11 included: 500x4096 17.2 against 18.8, 1024x1000 18.5 against 19.5, 1024x4096 22.5 either
+// way, but 2048x1000 28.0 against 22.4).
+bool whole_sums(int64_t R) { return R <= 1024; }
+
+// Rows a workgroup takes otherwise: 16 (four a wave, all in flight at once) or as many as make 64
+// slabs of rows, whose sums the second launch reads fastest (4096x1000 24.7 us, with 32 / 128 / 256
+// slabs 27.2 / 25.8 / 30.7; 4096x4096 41.5: 26 us for 145 MB are 5.6 TB/s), or 1024 workgroups where
+// there are few columns and the slabs so many that their sums are folded in two launches (8192x200
+// 20.5 against 26.0).
 int64_t act_grad_rows(int64_t R, int64_t C) {
-  if (R <= 64) return 64;
-  const int64_t strips = (C + AG_COLS - 1) / AG_COLS;
-  const int64_t slabs = std::max<int64_t>(1, 1024 / strips);
+  const int64_t strips = (C + 255) / 256, slabs = R > 4096 && strips <= 2 ? 1024 / strips : 64;
   const int64_t rows = (R + slabs - 1) / slabs;
   return std::max<int64_t>(16, (rows + 15) / 16 * 16);
 }
@@ -223,7 +233,7 @@ hipError_t launch_mx_decode(const uint8_t* codes, const uint8_t* scales, float* 
 }
 
 int64_t mx_act_grad_partial_doubles(int64_t R, int64_t C) {
-  if (R <= 0 || C <= 0) return 0;
+  if (R <= 0 || C <= 0 || whole_sums(R)) return 0;
   const int64_t rows = act_grad_rows(R, C);
   return (R + rows - 1) / rows * C;
 }
@@ -232,20 +242,22 @@ hipError_t launch_mx_act_grad(const float* dy, int64_t ldy, const uint8_t* codes
                               const uint8_t* scales, float* dz, int64_t ldz, float* colsum, int64_t R,
                               int64_t C, int format, int act, double* partial, hipStream_t s) {
   if (C <= 0) return hipSuccess;
-  const int64_t G = mx_groups(C), rows = act_grad_rows(R, C);
-  const int64_t slabs = (R + rows - 1) / rows;
+  const bool whole = colsum != nullptr && whole_sums(R);
+  const int64_t G = mx_groups(C), rows = whole ? R : act_grad_rows(R, C);
+  const int64_t slabs = whole ? 1 : (R + rows - 1) / rows;
   if (slabs > 0) {
-    const dim3 grid((unsigned)((C + AG_COLS - 1) / AG_COLS), (unsigned)slabs);
     mx_with_format(format, [&](auto f) {
       constexpr int F = decltype(f)::value;
       auto go = [&](auto a) {
         constexpr int ACT = decltype(a)::value;
         auto with = [&](auto sums, void* to) {
-          hipLaunchKernelGGL((mx_act_grad<F, ACT, decltype(sums)::value>), grid, dim3(256), 0, s, dy, ldy,
-                             codes, scales, dz, ldz, to, R, (int)C, G, rows);
+          constexpr int SUMS = decltype(sums)::value, COLS = SUMS == WHOLE ? 32 : 256;
+          hipLaunchKernelGGL((mx_act_grad<F, ACT, SUMS>), dim3((unsigned)((C + COLS - 1) / COLS), (unsigned)slabs),
+                             dim3(SUMS == WHOLE ? 1024 : 256), 0, s, dy, ldy, codes, scales, dz, ldz, to, R,
+                             (int)C, G, rows);
         };
         if (colsum == nullptr) with(std::integral_constant<int, NO_SUMS>(), nullptr);
-        else if (slabs == 1) with(std::integral_constant<int, WHOLE>(), colsum);
+        else if (whole) with(std::integral_constant<int, WHOLE>(), colsum);
         else with(std::integral_constant<int, PARTIAL>(), partial);
       };
       switch (act) {
@@ -258,7 +270,7 @@ hipError_t launch_mx_act_grad(const float* dy, int64_t ldy, const uint8_t* codes
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (colsum == nullptr || slabs == 1) return hipSuccess;
+  if (colsum == nullptr || whole) return hipSuccess;
   return launch_colsum_finish(partial, colsum, slabs, C, s);
 }
 
