@@ -545,12 +545,22 @@ hipError_t launch(const LinearParams& p, const Plan& w, char* scratch, hipStream
     if (r == ROWS_INLINE)
       hipLaunchKernelGGL((mx_linear_rows<FX, FW, 1, true, 1>), dim3((p.N + 15) / 16), block,
                          waves * 1024 + (size_t)p.M * G * 256, s, p);
-    else if (p.M <= 16)
-      hipLaunchKernelGGL((mx_linear_rows<FX, FW, 1, false, 1>), dim3((p.N + 15) / 16), block, waves * 1024,
-                         s, p);
-    else
-      hipLaunchKernelGGL((mx_linear_rows<FX, FW, 4, false, 1>), dim3((p.N + 15) / 16, (p.M + 63) / 64),
-                         block, waves * 4096, s, p);
+    else {
+      auto go = [&](auto mb) {
+        constexpr int MB = decltype(mb)::value;
+        hipLaunchKernelGGL((mx_linear_rows<FX, FW, MB, false, 1>),
+                           dim3((p.N + 15) / 16, (p.M + 16 * MB - 1) / (16 * MB)), block, waves * MB * 1024, s, p);
+      };
+      // as many row fragments as leave three quarters of the CUs a workgroup (48x4096x4096 28.6 us
+      // with four, 30.2 with two, 31.4 with one; 128x1024x2048 24.3, 21.5, 22.5; 64x1024x4096 30.6,
+      // 25.1, 22.2)
+      auto enough = [&](int mb) {
+        return p.M > 8 * mb && (int64_t)((p.N + 15) / 16) * ((p.M + 16 * mb - 1) / (16 * mb)) >= 192;
+      };
+      if (enough(4)) go(std::integral_constant<int, 4>());
+      else if (enough(2)) go(std::integral_constant<int, 2>());
+      else go(std::integral_constant<int, 1>());
+    }
     return hipGetLastError();
   }
   PrepareParams k{};
