@@ -186,7 +186,8 @@ struct WideParams {
   const char* pb;
   float* C;        // or the partial sums [slices][M][N] of a product split along K
   int64_t ldc, plane;
-  int M, N, KT, MT, NT;
+  int M, N, KT, MT, NT;         // MT, NT: blocks of the packed operands
+  int blocks_m;                 // blocks of A from pa on
   int tiles_m, tiles_n, chunk;  // chunk: fragments along K of a slice
 };
 
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
   for (int i = 0; i < COPIES; ++i) {
     const int c = wave * COPIES + i;
     if (c < CA) {
-      const int block = min(tm * (BM / 32) + c / PLANES, p.MT - 1);
+      const int block = min(tm * (BM / 32) + c / PLANES, p.blocks_m - 1);
       src[i] = p.pa + (((int64_t)kt0 * p.MT + block) * PLANES + c % PLANES) * FRAG;
       step[i] = (int64_t)p.MT * PLANES * FRAG;
     } else {
@@ -433,15 +434,17 @@ __global__ void __launch_bounds__(512) mx_direct(DirectParams p) {
 //     or 128 columns, where packing the other operand costs most (64x8192x8192 73 against 93,
 //     4096x128x4096 44 against 76; 128 rows, 128x4096x4096, 47 against 45); two row fragments a
 //     workgroup from 2^28 on (64x4096x4096 35 against 41 with one, but 300x300x1000 22.2 against 21.7);
-//   * packed on tiles of 256 when there is one for every CU (8192x8192x500 206 against 213 on tiles
-//     of 128; 4000x2900x2048, 192 tiles, 160 against 147).
+//   * packed on tiles of 256, of 128, or the rows of as many rounds of 256 CUs as tiles of 256 fill and
+//     then the others on tiles of 128, whichever takes the fewest rounds; a tile of 256 takes 3.6 times
+//     one of 128 (4096^3 342 on 256, 368 on 128; 4000x2900x2048, 192 tiles, 155 against 148;
+//     4096x5120x2048, 320 tiles, 284, 250 and mixed 229; 5000x4000x2000 277, 232 and 224).
 // Either is split along K into as many slices as bring 512 (256 tiles) workgroups, of at least two
 // chunks of 32 k a wave (eight fragments): 16x4096x4096 27 in eight, packed 1024^3 34.5 in four and
 // 40.5 whole.
 struct ProductPlan {
   bool direct;
   int mb, waves;            // direct: row fragments and waves a workgroup
-  int tile;                 // packed: its edge
+  int large;                // packed: rows of tiles of 256, ahead of those of 128
   int slices, chunk;        // chunk: chunks of 32 k, or fragments, of a slice
   int64_t KT, MT, NT;       // packed: fragments along K, blocks of A and of B
 };
@@ -460,9 +463,14 @@ ProductPlan plan(int64_t M, int64_t N, int64_t K) {
     w.KT = units = (K + 15) / 16;
     w.MT = (M + 31) / 32;
     w.NT = (N + 31) / 32;
-    auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-    w.tile = tiles(256) >= 256 ? 256 : 128;
-    s = std::min(256 / tiles(w.tile), units / 8);
+    auto tiles = [&](int64_t m, int64_t t) { return std::max<int64_t>(0, (m + t - 1) / t) * ((N + t - 1) / t); };
+    const int64_t strips = (M + 255) / 256, whole = tiles(M, 256) / 256 * 256 / tiles(1, 256);
+    double least = 1e300;
+    for (int64_t m : {(int64_t)0, whole, strips}) {  // rounds, in tiles of 128
+      const double t = 3.6 * (double)((m * tiles(1, 256) + 255) / 256) + (double)((tiles(M - 256 * m, 128) + 255) / 256);
+      if (t < least) least = t, w.large = (int)m;
+    }
+    s = w.large ? 1 : std::min(256 / tiles(M, 128), units / 8);
   }
   s = std::max<int64_t>(1, s);
   w.chunk = (int)((units + s - 1) / s);
@@ -515,16 +523,26 @@ hipError_t launch_piece(const MxGemmParams& p, int64_t G, void* scratch, hipStre
       else hipLaunchKernelGGL((mx_pack<F, false>), packs, dim3(256), 0, s, k);
     });
     WideParams q{};
-    q.pa = pa; q.pb = pb; q.C = sums;
+    q.pb = pb;
     q.ldc = ld_sums; q.plane = plane;
-    q.M = (int)p.M; q.N = (int)p.N;
+    q.N = (int)p.N;
     q.KT = (int)w.KT; q.MT = (int)w.MT; q.NT = (int)w.NT;
-    q.tiles_m = (int)((p.M + w.tile - 1) / w.tile);
-    q.tiles_n = (int)((p.N + w.tile - 1) / w.tile);
     q.chunk = w.chunk;
-    const dim3 grid((unsigned)(q.tiles_m * q.tiles_n), (unsigned)w.slices);
-    if (w.tile == 256) hipLaunchKernelGGL((mx_wide<256, 256, 4, 2, 4>), grid, dim3(512), 0, s, q);
-    else hipLaunchKernelGGL((mx_wide<128, 128, 4, 2, 4>), grid, dim3(512), 0, s, q);
+    auto go = [&](auto tile, int64_t row0, int64_t rows) {
+      constexpr int T = decltype(tile)::value;
+      if (rows <= 0) return;
+      q.pa = pa + row0 / 32 * PLANES * FRAG;
+      q.C = sums + row0 * ld_sums;
+      q.M = (int)rows;
+      q.blocks_m = (int)(w.MT - row0 / 32);
+      q.tiles_m = (int)((rows + T - 1) / T);
+      q.tiles_n = (int)((p.N + T - 1) / T);
+      hipLaunchKernelGGL((mx_wide<T, T, 4, 2, 4>), dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)w.slices),
+                         dim3(512), 0, s, q);
+    };
+    const int64_t large = std::min(p.M, 256 * (int64_t)w.large);
+    go(std::integral_constant<int, 256>(), 0, large);
+    go(std::integral_constant<int, 128>(), large, p.M - large);
   }
   if (w.slices > 1)
     hipLaunchKernelGGL(mx_gemm_sum, dim3((unsigned)std::min<int64_t>(8192, (plane + 255) / 256)), dim3(256),

@@ -129,7 +129,8 @@ def test_rows_further_apart_than_their_width(ctx):
 @pytest.mark.parametrize("shape,format", [((1, 1), "e4m3"), ((2, 5), "e5m2"), ((16, 256), "e4m3"),
                                           ((17, 257), "e2m1"), ((300, 130), "e4m3"),
                                           ((64, 70), "e4m3"), ((65, 70), "e4m3"), ((1, 3001), "e5m2"), ((70000, 3), "e4m3"),
-                                          ((1000, 1100), "e4m3")], ids=str)
+                                          ((1000, 1100), "e4m3"), ((1025, 300), "e5m2"), ((1500, 513), "e4m3"),
+                                          ((5000, 600), "e5m2")], ids=str)
 def test_activation_gradient_from_a_checkpoint(ctx, shape, format, act):
     R, C = shape
     rng = np.random.default_rng(R + C)
@@ -204,8 +205,8 @@ PRODUCTS = [(1, 1, 1), (1, 5, 3), (3, 2, 40), (16, 16, 16), (33, 31, 32), (1, 10
             (64, 64, 64), (65, 130, 100), (128, 128, 512), (200, 10, 900), (255, 257, 333),
             (257, 513, 65), (512, 512, 512), (700, 390, 1025), (1024, 1030, 260), (130, 4100, 77),
             (1025, 1023, 1027)]
-# large tiles, whole and split along K
-LARGE_PRODUCTS = [(4100, 2100, 70), (4000, 2000, 300)]
+# small tiles whole and split along K, large tiles, and large tiles ahead of small ones
+LARGE_PRODUCTS = [(4100, 2100, 70), (4000, 2000, 300), (1600, 1500, 600), (4100, 2100, 200), (4000, 4050, 90), (4600, 4000, 90)]
 
 
 @pytest.mark.parametrize("trans_a", [False, True])
@@ -342,7 +343,7 @@ def linear_room(X, W, bias, act, z):
 LINEARS = [(1, 1, 1), (1, 7, 33), (1, 300, 1000), (1, 1030, 4096), (2, 130, 128), (3, 64, 129),
            (4, 17, 600), (5, 33, 257), (15, 65, 64), (16, 1030, 300), (17, 16, 2100), (33, 100, 31),
            (64, 512, 1024), (100, 333, 200), (129, 127, 130), (256, 256, 512), (300, 1021, 617),
-           (1030, 520, 260), (16, 70, 1100), (3, 40, 6000)]
+           (1030, 520, 260), (16, 70, 1100), (3, 40, 6000), (20, 3100, 130), (40, 3100, 300), (90, 1100, 200)]
 # tiles in LDS: whole, split along K, and of 256
 LARGE_LINEARS = [(1030, 1031, 1033), (70, 2000, 8300), (4000, 3001, 200)]
 
