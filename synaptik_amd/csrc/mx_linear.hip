@@ -504,7 +504,8 @@ __global__ void __launch_bounds__(256) mx_linear_sum(const float* __restrict__ p
 enum Route { ROWS_INLINE, ROWS, TILES };
 struct Plan {
   Route route;
-  int tile, slices, chunk;
+  int large;          // rows of tiles of 256, ahead of those of 128
+  int slices, chunk;  // groups of a slice
 };
 // Which form runs (us on MI355X, e4m3 activations and e2m1 weights, a synchronous run's 13 us
 // included):
@@ -512,25 +513,36 @@ struct Plan {
 //   * ROWS up to 2^30 multiply-adds (500x1021x617 21.8 against 27.2, 300x1024x1024 23.7 against
 //     29.2; 1024^3 33.7 against 30.5), 2^31 of up to 64 rows (64x4096x4096 30.9 against 34.6;
 //     64x8192x8192 70 against 46), and always up to 16;
-//   * tiles of 256 when there are enough of them for three quarters of the CUs (8192x4096x4096 281,
-//     of 128 307; 8192x512x4096, 64 tiles of 256, 73 against 58 for 256 of 128);
+//   * tiles of 256, of 128, or the rows of as many rounds of 256 CUs as tiles of 256 fill and then the
+//     others on tiles of 128, whichever takes the fewest rounds; a tile of 256 takes 3.6 times one of
+//     128, 2.6 times with 4 bits on both sides (8192x4096x4096 290 on 256, 320 on 128; 4096x5120x2048,
+//     320 tiles, 122, 102 and mixed 101; 4100x4100x4000 203, 161 and 160, of 4-bit codes 99, 93 and 87;
+//     4000x2900x2048, 192 tiles, 74 against 71, of 4-bit codes 46.5 against 50.5);
 //   * K split between workgroups when there are fewer than 256 tiles of 128 and 16 groups and more
 //     (128x4096x4096 38 in eight, 51 whole; 300x4096x4096 47 in four, 54 whole; but 1024^3, eight
 //     groups, 34 in two and 30.5 whole).
 constexpr int64_t INLINE_GROUPS = 128;
-Plan plan(int64_t M, int64_t N, int64_t K) {
+Plan plan(int64_t M, int64_t N, int64_t K, bool four) {
   const int64_t G = mx_groups(K);
-  Plan w{TILES, 128, 1, (int)G};
+  Plan w{TILES, 0, 1, (int)G};
   const double work = (double)M * (double)N * (double)K;
-  auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-  if (M <= 16 && M * G <= INLINE_GROUPS) w.route = ROWS_INLINE;
+  auto tiles = [&](int64_t m, int64_t t) { return std::max<int64_t>(0, (m + t - 1) / t) * ((N + t - 1) / t); };
+  if (M <= 16 && M * G <= INLINE_GROUPS) {
+    w.route = ROWS_INLINE;
   // (tiles address a row within 32 bits)
-  else if (M <= 16 || work < (M <= 64 ? 2.0 : 1.0) * (1 << 30) || K > (1 << 22)) w.route = ROWS;
-  else if (tiles(256) >= 192) w.tile = 256;
-  else if (tiles(128) < 256 && G >= 16) {
-    const int64_t s = std::max<int64_t>(1, std::min(384 / tiles(128), G / 4));
+  } else if (M <= 16 || work < (M <= 64 ? 2.0 : 1.0) * (1 << 30) || K > (1 << 22)) {
+    w.route = ROWS;
+  } else if (tiles(M, 128) < 256 && G >= 16) {
+    const int64_t s = std::max<int64_t>(1, std::min(384 / tiles(M, 128), G / 4));
     w.chunk = (int)((G + s - 1) / s);
     w.slices = (int)((G + w.chunk - 1) / w.chunk);
+  } else {
+    const int64_t strips = (M + 255) / 256, whole = tiles(M, 256) / 256 * 256 / tiles(1, 256);
+    double least = 1e300;
+    for (int64_t m : {(int64_t)0, whole, strips}) {  // rounds, in tiles of 128
+      const double t = (four ? 2.6 : 3.6) * (double)((m * tiles(1, 256) + 255) / 256) + (double)((tiles(M - 256 * m, 128) + 255) / 256);
+      if (t < least) least = t, w.large = (int)m;
+    }
   }
   return w;
 }
@@ -577,17 +589,26 @@ hipError_t launch(const LinearParams& p, const Plan& w, char* scratch, hipStream
   t.l.x_codes = k.codes;
   t.xt = k.xt; t.wt = k.wt; t.MP = k.MP; t.NP = k.NP;
   t.chunk = w.chunk;
-  t.tiles_m = (p.M + w.tile - 1) / w.tile;
-  t.tiles_n = (p.N + w.tile - 1) / w.tile;
   if (w.slices > 1)
     t.partial = reinterpret_cast<float*>(k.codes + (int64_t)p.M * G * mx_group_bytes(FX));
-  const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)w.slices);
   constexpr int bytes = mx_group_bytes(FX) + mx_group_bytes(FW);
   constexpr int NS = bytes == 256 ? 2 : bytes == 192 ? 3 : 4;
-  if (w.tile == 256)
-    hipLaunchKernelGGL((mx_linear_tile<FX, FW, 256, 256, 4, 2, NS>), grid, dim3(512), 0, s, t);
-  else
-    hipLaunchKernelGGL((mx_linear_tile<FX, FW, 128, 128, 2, 2, NS>), grid, dim3(256), 0, s, t);
+  auto go = [&](auto tile, int row0, int rows) {
+    constexpr int T = decltype(tile)::value, WM = T == 256 ? 4 : 2;
+    if (rows <= 0) return;
+    TileParams q = t;
+    q.l.M = rows;
+    q.l.x_codes += (int64_t)row0 * G * mx_group_bytes(FX);
+    q.l.Y += row0 * p.ldy;
+    q.xt += row0;
+    q.tiles_m = (rows + T - 1) / T;
+    q.tiles_n = (p.N + T - 1) / T;
+    hipLaunchKernelGGL((mx_linear_tile<FX, FW, T, T, WM, 2, NS>), dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)w.slices),
+                       dim3(128 * WM), 0, s, q);
+  };
+  const int large = std::min(p.M, 256 * w.large);
+  go(std::integral_constant<int, 256>(), 0, large);
+  go(std::integral_constant<int, 128>(), large, p.M - large);
   if (w.slices > 1) {
     const int64_t plane = (int64_t)p.M * p.N;
     hipLaunchKernelGGL(mx_linear_sum, dim3((unsigned)std::min<int64_t>(8192, (plane + 255) / 256)), dim3(256),
@@ -603,7 +624,7 @@ namespace {
 constexpr int64_t MAX_ROWS = 1 << 20;
 
 int64_t piece_scratch_bytes(int64_t M, int64_t N, int64_t K) {
-  const Plan w = plan(M, N, K);
+  const Plan w = plan(M, N, K, false);  // (the tiles' sizes take no scratch)
   if (w.route == ROWS_INLINE) return 0;
   const int64_t G = mx_groups(K);
   if (w.route == ROWS) return pad256(M * G * 128) + M * G * 4;
@@ -613,7 +634,7 @@ int64_t piece_scratch_bytes(int64_t M, int64_t N, int64_t K) {
 
 hipError_t launch_piece(const MxLinearParams& in, void* scratch, hipStream_t s) {
   const int64_t G = mx_groups(in.K);
-  const Plan w = plan(in.M, in.N, in.K);
+  const Plan w = plan(in.M, in.N, in.K, in.x_format == MX_E2M1 && in.w_format == MX_E2M1);
   LinearParams p{};
   p.X = in.X; p.codes = in.codes; p.scales = in.scales; p.bias = in.bias; p.Y = in.Y;
   p.ldx = in.ldx; p.ldy = in.ldy; p.K = in.K;
