@@ -334,7 +334,10 @@ __global__ void __launch_bounds__(256) mx_gemm_sum(const float* __restrict__ par
 // are added in wave order. v_mfma_f32_16x16x32_bf16 takes from lane l the eight values k = 8 (l / 16)
 // .. + 7 of row or column l mod 16: the lane loads them of MB rows of A, splits them, and of four
 // columns of B (4 (l mod 16) + j is column l mod 16 of product j), whose codes lie four to a word, a
-// word for each k.
+// word for each k. The L1's requests bound it, so of the eight k's scales a lane loads one and takes
+// the others from its neighbours, and of a transposed A the two fragments' rows are neighbours, eight
+// bytes a k (1024^3 transposed 28.5 -> 25.0 us a run with both, 64x8192x8192 71 -> 66); addresses are
+// one base a wave and 32-bit offsets.
 template <bool TA>
 __device__ __forceinline__ void load_a8(const float* __restrict__ a, int64_t lda, int64_t m, int64_t k,
                                         int64_t K, float (&v)[8]) {
@@ -359,13 +362,23 @@ struct DirectParams {
   float* C;  // or the partial sums [slices][M][N] of a product split along K
   int64_t lda, ldc, plane, K, G;
   int M, N, chunks, per_slice, row_tiles;
+  int near;  // a chunk's values lie within 2^32 bytes of its first
 };
+// A buffer from p on, which the wave agrees on.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, -1, 0x00020000);
+}
+// The value of lane I of this lane's eight.
+template <int I>
+__device__ __forceinline__ uint32_t of_eight(int v) {
+  return (uint32_t)__builtin_amdgcn_ds_swizzle(v, (I << 5) | 0x18);
+}
 template <int F, bool TA, int MB>
-__global__ void __launch_bounds__(512) mx_direct(DirectParams p) {
+__global__ void __launch_bounds__(512, 4) mx_direct(DirectParams p) {
   extern __shared__ __align__(16) float sums[];  // [waves][MB][4][64][4]
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int64_t n = (int64_t)(blockIdx.x / p.row_tiles) * 64 + 4 * c;
+  const int64_t n0 = (int64_t)(blockIdx.x / p.row_tiles) * 64;
   const int64_t m0 = (int64_t)(blockIdx.x % p.row_tiles) * (16 * MB);
   const int last = min(p.chunks, (int)(blockIdx.y + 1) * p.per_slice);
   floatx4 acc[MB][4];
@@ -373,20 +386,72 @@ __global__ void __launch_bounds__(512) mx_direct(DirectParams p) {
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  // row c of fragment i
+  auto row_of = [&](int i) { return m0 + (TA ? MB * c + i : 16 * i + c); };
+  // byte offsets of this lane's first values of a chunk
+  const uint32_t row_bytes = (uint32_t)p.G * mx_group_bytes(F), row_scales = (uint32_t)p.G * 4, lda4 = (uint32_t)p.lda * 4;
+  const uint32_t code_at = 8 * q * row_bytes + c * (F == MX_E2M1 ? 2 : 4), scale_at = (8 * q + (c & 7)) * row_scales + (c >> 3);
+  uint32_t a_at[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) {
+    const uint32_t m = (uint32_t)(min(row_of(i), (int64_t)p.M - 1) - m0);
+    a_at[i] = TA ? 8 * q * lda4 + 4 * m : m * lda4 + 32 * q;
+  }
+  const uint8_t* codes0 = p.codes + (n0 / 4) * (F == MX_E2M1 ? 2 : 4);
+  const uint8_t* scales0 = p.scales + n0 / MX_BLOCK;
+  const bool pairs = TA && MB == 2 && m0 + 32 <= p.M;  // (of rows, eight bytes)
+  const float* a0 = TA ? p.A + m0 : p.A + m0 * p.lda;
   for (int t = blockIdx.y * p.per_slice + wave; t < last; t += waves) {
-    const int64_t k = (int64_t)t * 32 + 8 * q;
     uint32_t w[8], s[8];
     float a[MB][8];
+    const int64_t k0 = (int64_t)t * 32;
+    if (k0 + 32 <= p.K && p.near) {
+      const auto rw = buffer_at(codes0 + k0 * row_bytes), rs = buffer_at(scales0 + k0 * row_scales);
+      const auto ra = buffer_at(a0 + (TA ? k0 * p.lda : k0));
+      const int scale = __builtin_amdgcn_raw_buffer_load_b8(rs, scale_at, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // (behind K the last row again, against zeros of A)
-      const int64_t row = min(k + i, p.K - 1);
-      w[i] = mx_load4<F>(p.codes, row * p.G * 32 + n / 4);
-      s[i] = p.scales[row * p.G * 4 + n / 32];
+      for (int i = 0; i < 8; ++i)
+        w[i] = F == MX_E2M1 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rw, code_at, i * row_bytes, 0)
+                            : (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rw, code_at, i * row_bytes, 0);
+      if (pairs) {
+        if constexpr (TA && MB == 2) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b64(ra, a_at[0], j * lda4, 0);
+            a[0][j] = __uint_as_float(x[0]);
+            a[1][j] = __uint_as_float(x[1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          if constexpr (TA) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              a[i][j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ra, a_at[i], j * lda4, 0));
+          } else {
+            const uintx4 x = __builtin_amdgcn_raw_buffer_load_b128(ra, a_at[i], 0, 0);
+            const uintx4 y = __builtin_amdgcn_raw_buffer_load_b128(ra, a_at[i], 16, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { a[i][j] = __uint_as_float(x[j]); a[i][4 + j] = __uint_as_float(y[j]); }
+          }
+        }
+      }
+      s[0] = of_eight<0>(scale), s[1] = of_eight<1>(scale), s[2] = of_eight<2>(scale), s[3] = of_eight<3>(scale);
+      s[4] = of_eight<4>(scale), s[5] = of_eight<5>(scale), s[6] = of_eight<6>(scale), s[7] = of_eight<7>(scale);
+    } else {
+      const int64_t k = k0 + 8 * q;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // (behind K the last row again, against zeros of A)
+        const int64_t row = min(k + i, p.K - 1);
+        w[i] = mx_load4<F>(p.codes, row * p.G * 32 + n0 / 4 + c);
+        s[i] = p.scales[row * p.G * 4 + (n0 + 4 * c) / MX_BLOCK];
+      }
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+        load_a8<TA>(p.A, p.lda, min(row_of(i), (int64_t)p.M - 1), k, p.K, a[i]);
     }
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-      load_a8<TA>(p.A, p.lda, min(m0 + 16 * i + c, (int64_t)p.M - 1), k, p.K, a[i]);
     bf16x8 b[4];
     fragments_of4<F>(w, s, b);
 #pragma unroll
@@ -410,11 +475,11 @@ __global__ void __launch_bounds__(512) mx_direct(DirectParams p) {
           floatx4{acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]};
   __syncthreads();
   float* out = p.C + blockIdx.y * p.plane;
-  const int64_t n0 = (int64_t)(blockIdx.x / p.row_tiles) * 64;
   for (int e = threadIdx.x; e < MB * 256; e += blockDim.x) {
     floatx4 v = *reinterpret_cast<const floatx4*>(sums + e * 4);
     for (int x = 1; x < waves; ++x) v += *reinterpret_cast<const floatx4*>(sums + (x * MB * 256 + e) * 4);
-    const int64_t row = m0 + (e >> 8) * 16 + ((e & 63) >> 4) * 4 + ((e >> 6) & 3);
+    const int c = ((e & 63) >> 4) * 4 + ((e >> 6) & 3), i = e >> 8;
+    const int64_t row = m0 + (TA ? MB * c + i : 16 * i + c);
     const int64_t col = n0 + 4 * (e & 15);
     if (row >= p.M) continue;
     float* dst = out + row * p.ldc + col;
@@ -500,6 +565,7 @@ hipError_t launch_piece(const MxGemmParams& p, int64_t G, void* scratch, hipStre
     d.lda = p.lda; d.ldc = ld_sums; d.plane = plane; d.K = p.K; d.G = G;
     d.M = (int)p.M; d.N = (int)p.N; d.chunks = (int)((p.K + 31) / 32); d.per_slice = w.chunk;
     d.row_tiles = (int)((p.M + 16 * w.mb - 1) / (16 * w.mb));
+    d.near = p.lda < (1 << 24) && G < (1 << 20);  // (32 rows)
     const dim3 grid((unsigned)((p.N + 63) / 64 * d.row_tiles), (unsigned)w.slices), block(64 * w.waves);
     mx_with_format(p.format, [&](auto f) {
       constexpr int F = decltype(f)::value;

@@ -286,6 +286,20 @@ def test_product_with_strides_and_a_matrix_of_no_depth(ctx, trans_a):
     assert np.array_equal(got, np.zeros((5, 6), np.float32))
 
 
+def test_product_of_rows_far_apart(ctx):
+    """Rows of A 64 MiB apart: a wave's 32 lie further than a 32-bit offset reaches."""
+    M, N, K, lda = 20, 70, 100, (1 << 24) + 8
+    rng = np.random.default_rng(6)
+    A = rng.standard_normal((M, K)).astype(np.float32)
+    codes, scales, B = mx.stored(rng.standard_normal((K, N)), "e4m3")
+    wide = np.zeros((M - 1) * lda + K, np.float32)
+    for m in range(M):
+        wide[m * lda:m * lda + K] = A[m]
+    got = gpu_mx_gemm(ctx, wide, codes, scales, M, N, K, "e4m3", False, lda=lda)
+    A = A.astype(np.float64)
+    assert (np.abs(got - A @ B) <= 2 * (3 * K + 1) * U * (np.abs(A) @ np.abs(B))).all()
+
+
 @pytest.mark.parametrize("size", [48, 560, 1209])
 def test_product_with_infinities_and_nans(ctx, size):
     """A value that is not finite makes every result that it contributes to not finite, and no
