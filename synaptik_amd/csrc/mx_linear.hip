@@ -184,23 +184,21 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
       }
     }
   }
-  // register r of a lane: column n = 4 (lane / 16) + r, row m = lane mod 16
+  // register r of a lane: column n = 4 (lane / 16) + r, row m = lane mod 16 (its four columns' banks
+  // apart from those of the other columns of the rows that are read together)
+  auto at = [](int quad, int row) { return (quad * 16 + (row ^ (4 * quad))) * 4; };
 #pragma unroll
   for (int i = 0; i < MB; ++i)
-    *reinterpret_cast<floatx4*>(sums + ((wave * MB + i) * 64 + lane) * 4) = acc[i];
+    *reinterpret_cast<floatx4*>(sums + (wave * MB + i) * 256 + at(q, lane & 15)) = acc[i];
   __syncthreads();
-  for (int e = threadIdx.x; e < MB * 64; e += blockDim.x) {
-    floatx4 v = *reinterpret_cast<const floatx4*>(sums + e * 4);
-    for (int k = 1; k < waves; ++k) v += *reinterpret_cast<const floatx4*>(sums + (k * MB * 64 + e) * 4);
-    const int row = blockIdx.y * (16 * MB) + (e >> 6) * 16 + (e & 15);
-    const int col = blockIdx.x * 16 + ((e & 63) >> 4) * 4;
-    if (row >= p.M) continue;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (col + r >= p.N) break;
-      const float z = p.bias != nullptr ? v[r] + p.bias[col + r] : v[r];
-      p.Y[row * p.ldy + col + r] = apply_act(p.act, z);
-    }
+  for (int e = threadIdx.x; e < MB * 256; e += blockDim.x) {
+    const int c = e & 15, r = (e >> 4) & 15, from = (e >> 8) * 256 + at(c >> 2, r) + (c & 3);
+    float v = sums[from];
+    for (int k = 1; k < waves; ++k) v += sums[k * MB * 256 + from];
+    const int row = blockIdx.y * (16 * MB) + (e >> 8) * 16 + r, col = blockIdx.x * 16 + c;
+    if (row >= p.M || col >= p.N) continue;
+    if (p.bias != nullptr) v += p.bias[col];
+    p.Y[row * p.ldy + col] = apply_act(p.act, v);
   }
 }
 
@@ -565,9 +563,10 @@ hipError_t launch(const LinearParams& p, const Plan& w, char* scratch, hipStream
       };
       // as many row fragments as leave three quarters of the CUs a workgroup (48x4096x4096 28.6 us
       // with four, 30.2 with two, 31.4 with one; 128x1024x2048 24.3, 21.5, 22.5; 64x1024x4096 30.6,
-      // 25.1, 22.2)
+      // 25.1, 22.2) and eight waves a CU (362x784x44, one wave each, 20.0 with four, 18.3 with one)
       auto enough = [&](int mb) {
-        return p.M > 8 * mb && (int64_t)((p.N + 15) / 16) * ((p.M + 16 * mb - 1) / (16 * mb)) >= 192;
+        const int64_t n = (int64_t)((p.N + 15) / 16) * ((p.M + 16 * mb - 1) / (16 * mb));
+        return p.M > 8 * mb && n >= 192 && n * waves >= 2048;
       };
       if (enough(4)) go(std::integral_constant<int, 4>());
       else if (enough(2)) go(std::integral_constant<int, 2>());
