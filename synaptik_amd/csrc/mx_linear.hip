@@ -89,14 +89,15 @@ struct LinearParams {
 // instruction contracts does not matter as long as both operands agree. Weights are not staged:
 // each is used once, and the loads of U groups are in flight at once.
 //
-// INLINE: every workgroup encodes the few rows of X itself, four values a thread and round, into
-// LDS as bfloat16 [M][128 G], while its first weights arrive; otherwise X comes encoded.
+// INLINE: every workgroup encodes its rows of X itself, four values a thread and round, into LDS as
+// bfloat16 [rows][128 G] (16-byte pieces of a group in another order for each row, so that rows are
+// read from different banks), while its first weights arrive; otherwise X comes encoded.
 template <int FX>
-__device__ __forceinline__ void encode_rows(const LinearParams& p, char* lds) {
-  const int q = threadIdx.x & 31, total = p.M * p.G;
+__device__ __forceinline__ void encode_rows(const LinearParams& p, char* lds, int row0, int rows) {
+  const int q = threadIdx.x & 31, total = rows * p.G;
   for (int t = threadIdx.x >> 5; t < total; t += blockDim.x >> 5) {
     const int m = t / p.G, k = (t - m * p.G) * MX_GROUP + 4 * q;
-    const float* x = p.X + m * p.ldx + k;
+    const float* x = p.X + (row0 + m) * p.ldx + k;
     float v[4];
     if (k + 4 <= p.K) {
       const float4u f = *reinterpret_cast<const float4u*>(x);
@@ -116,7 +117,7 @@ __device__ __forceinline__ void encode_rows(const LinearParams& p, char* lds) {
     // (a lost block's reciprocal is of no account: its scale makes it NaN)
     const uint32_t c = mx_codes4<FX, false>(v, mx_reciprocal(min(s, 254u)));
     const uint2 out = {mx_values2<FX, 0>(c, mx_scale_operand(s)), mx_values2<FX, 1>(c, mx_scale_operand(s))};
-    reinterpret_cast<uint2*>(lds)[t * 32 + q] = out;
+    reinterpret_cast<uint2*>(lds)[t * 32 + (q ^ (2 * m))] = out;
   }
 }
 
@@ -128,7 +129,8 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
   const int lane = threadIdx.x & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   float* sums = reinterpret_cast<float*>(lds);
-  char* x_rows = lds + waves * 1024;
+  char* x_rows = lds + waves * MB * 1024;
+  const int row0 = blockIdx.y * (16 * MB), rows = min(16 * MB, p.M - row0);
   const int64_t n = min((int)blockIdx.x * 16 + (lane & 15), p.N - 1);
   const uint8_t* w_codes = p.codes + n * p.G * BW + q * (BW / 4);
   const uint8_t* w_scales = p.scales + n * p.G * 4 + q;
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
       }
     }
     if (INLINE && !encoded) {  // (once, every wave)
-      encode_rows<FX>(p, x_rows);
+      encode_rows<FX>(p, x_rows, row0, rows);
       __syncthreads();
       encoded = true;
     }
@@ -169,10 +171,11 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = w[u].eight(i, wf);
       if constexpr (INLINE) {
-        const bf16x8* b = reinterpret_cast<const bf16x8*>(x_rows) + (m[0] * p.G + g0 + u * waves) * 16 + q * 4;
+        const int r = min(lane & 15, rows - 1);
+        const bf16x8* b = reinterpret_cast<const bf16x8*>(x_rows) + (r * p.G + g0 + u * waves) * 16;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], b[j], acc[0], 0, 0, 0);
+          acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], b[(4 * q + j) ^ r], acc[0], 0, 0, 0);
       } else {
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
@@ -502,12 +505,16 @@ __global__ void __launch_bounds__(256) mx_linear_sum(const float* __restrict__ p
 enum Route { ROWS_INLINE, ROWS, TILES };
 struct Plan {
   Route route;
+  int mb, waves;      // few rows: row fragments and waves of a workgroup
   int large;          // rows of tiles of 256, ahead of those of 128
   int slices, chunk;  // groups of a slice
 };
 // Which form runs (us on MI355X, e4m3 activations and e2m1 weights, a synchronous run's 13 us
 // included):
-//   * few rows: INLINE up to 128 groups of X (1x4096x4096 17.0; encoded by a launch of its own 19.6);
+//   * few rows: INLINE up to 128 groups of X a workgroup, with a wave for every four of them
+//     (1x4096x4096 16.6; encoded by a launch of its own 19.6), and for more than 16 rows only while
+//     the groups that all workgroups encode stay few (20x1000x500 15.8 against 18.3, 128x1024x128 14.7
+//     against 17.9, 362x784x44 17.2 against 17.5; but 2400x512x64 24.8 against 20.5);
 //   * ROWS up to 2^30 multiply-adds (500x1021x617 21.8 against 27.2, 300x1024x1024 23.7 against
 //     29.2; 1024^3 33.7 against 30.5), 2^31 of up to 64 rows (64x4096x4096 30.9 against 34.6;
 //     64x8192x8192 70 against 46), and always up to 16;
@@ -519,17 +526,28 @@ struct Plan {
 //   * K split between workgroups when there are fewer than 256 tiles of 128 and 16 groups and more
 //     (128x4096x4096 38 in eight, 51 whole; 300x4096x4096 47 in four, 54 whole; but 1024^3, eight
 //     groups, 34 in two and 30.5 whole).
-constexpr int64_t INLINE_GROUPS = 128;
+constexpr int64_t INLINE_GROUPS = 128, INLINE_WORK = 600000;
 Plan plan(int64_t M, int64_t N, int64_t K, bool four) {
   const int64_t G = mx_groups(K);
-  Plan w{TILES, 0, 1, (int)G};
+  Plan w{TILES, 0, 0, 0, 1, (int)G};
   const double work = (double)M * (double)N * (double)K;
   auto tiles = [&](int64_t m, int64_t t) { return std::max<int64_t>(0, (m + t - 1) / t) * ((N + t - 1) / t); };
-  if (M <= 16 && M * G <= INLINE_GROUPS) {
-    w.route = ROWS_INLINE;
   // (tiles address a row within 32 bits)
-  } else if (M <= 16 || work < (M <= 64 ? 2.0 : 1.0) * (1 << 30) || K > (1 << 22)) {
-    w.route = ROWS;
+  if (M <= 16 || work < (M <= 64 ? 2.0 : 1.0) * (1 << 30) || K > (1 << 22)) {
+    w.waves = (int)std::min<int64_t>(16, G);
+    // as many row fragments as leave three quarters of the CUs a workgroup (48x4096x4096 28.6 us
+    // with four, 30.2 with two, 31.4 with one; 128x1024x2048 24.3, 21.5, 22.5; 64x1024x4096 30.6,
+    // 25.1, 22.2) and eight waves a CU (362x784x44, one wave each, 20.0 with four, 18.3 with one)
+    auto enough = [&](int mb) {
+      const int64_t n = ((N + 15) / 16) * ((M + 16 * mb - 1) / (16 * mb));
+      return M > 8 * mb && n >= 192 && n * w.waves >= 2048;
+    };
+    w.mb = enough(4) ? 4 : enough(2) ? 2 : 1;
+    const int64_t rows = std::min<int64_t>(M, 16 * w.mb);
+    // (with two row fragments and more there is too much to encode)
+    const bool in_line = w.mb == 1 && rows * G <= INLINE_GROUPS && (M <= 16 || M * G * N <= INLINE_WORK);
+    w.route = in_line ? ROWS_INLINE : ROWS;
+    if (in_line) w.waves = (int)std::max<int64_t>(w.waves, std::min<int64_t>(16, rows * G / 4));
   } else if (tiles(M, 128) < 256 && G >= 16) {
     const int64_t s = std::max<int64_t>(1, std::min(384 / tiles(M, 128), G / 4));
     w.chunk = (int)((G + s - 1) / s);
@@ -550,28 +568,17 @@ hipError_t launch(const LinearParams& p, const Plan& w, char* scratch, hipStream
   const int G = p.G;
   const Route r = w.route;
   if (r == ROWS_INLINE || r == ROWS) {
-    const int waves = std::max(1, std::min(16, G));
-    const dim3 block(64 * waves);
-    if (r == ROWS_INLINE)
-      hipLaunchKernelGGL((mx_linear_rows<FX, FW, 1, true, 1>), dim3((p.N + 15) / 16), block,
-                         waves * 1024 + (size_t)p.M * G * 256, s, p);
-    else {
-      auto go = [&](auto mb) {
-        constexpr int MB = decltype(mb)::value;
-        hipLaunchKernelGGL((mx_linear_rows<FX, FW, MB, false, 1>),
-                           dim3((p.N + 15) / 16, (p.M + 16 * MB - 1) / (16 * MB)), block, waves * MB * 1024, s, p);
-      };
-      // as many row fragments as leave three quarters of the CUs a workgroup (48x4096x4096 28.6 us
-      // with four, 30.2 with two, 31.4 with one; 128x1024x2048 24.3, 21.5, 22.5; 64x1024x4096 30.6,
-      // 25.1, 22.2) and eight waves a CU (362x784x44, one wave each, 20.0 with four, 18.3 with one)
-      auto enough = [&](int mb) {
-        const int64_t n = (int64_t)((p.N + 15) / 16) * ((p.M + 16 * mb - 1) / (16 * mb));
-        return p.M > 8 * mb && n >= 192 && n * waves >= 2048;
-      };
-      if (enough(4)) go(std::integral_constant<int, 4>());
-      else if (enough(2)) go(std::integral_constant<int, 2>());
-      else go(std::integral_constant<int, 1>());
-    }
+    auto go = [&](auto mb, auto in_line) {
+      constexpr int MB = decltype(mb)::value;
+      constexpr bool INLINE = decltype(in_line)::value;
+      hipLaunchKernelGGL((mx_linear_rows<FX, FW, MB, INLINE, 1>),
+                         dim3((p.N + 15) / 16, (p.M + 16 * MB - 1) / (16 * MB)), dim3(64 * w.waves),
+                         w.waves * MB * 1024 + (INLINE ? (size_t)std::min(p.M, 16 * MB) * G * 256 : 0), s, p);
+    };
+    if (r == ROWS_INLINE) go(std::integral_constant<int, 1>(), std::true_type());
+    else if (w.mb == 4) go(std::integral_constant<int, 4>(), std::false_type());
+    else if (w.mb == 2) go(std::integral_constant<int, 2>(), std::false_type());
+    else go(std::integral_constant<int, 1>(), std::false_type());
     return hipGetLastError();
   }
   PrepareParams k{};

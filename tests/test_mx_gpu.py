@@ -357,7 +357,8 @@ def linear_room(X, W, bias, act, z):
 LINEARS = [(1, 1, 1), (1, 7, 33), (1, 300, 1000), (1, 1030, 4096), (2, 130, 128), (3, 64, 129),
            (4, 17, 600), (5, 33, 257), (15, 65, 64), (16, 1030, 300), (17, 16, 2100), (33, 100, 31),
            (64, 512, 1024), (100, 333, 200), (129, 127, 130), (256, 256, 512), (300, 1021, 617),
-           (1030, 520, 260), (16, 70, 1100), (3, 40, 6000), (20, 3100, 130), (40, 3100, 300), (90, 1100, 200)]
+           (1030, 520, 260), (16, 70, 1100), (3, 40, 6000), (20, 3100, 130), (40, 3100, 300), (90, 1100, 200), (20, 3100, 1500),
+           (40, 3100, 1500), (700, 30, 130)]
 # tiles in LDS: whole, split along K, of 256, and of 256 ahead of 128
 LARGE_LINEARS = [(1030, 1031, 1033), (70, 2000, 8300), (4000, 3001, 200), (4000, 4050, 70), (4400, 4000, 100)]
 
