@@ -198,7 +198,10 @@ struct WideParams {
 // passing through registers; fragments lie in memory as in LDS, so every copy and every fragment
 // read is linear. A stage is copied NS - 1 stages before it is read; before a stage is read, each
 // wave has waited for its own copies into it, and has finished with the stage whose place the next
-// copies take. A stage's fragments are read while the one before is multiplied.
+// copies take. A stage's fragments are read while the one before is multiplied. The matrix cores
+// bound it: 4096^3 takes 266 us, the three products together 1.55 PFLOP/s (a large bfloat16 product of
+// the library 1.34), the cores busy 77% of the cycles at the 1.92 GHz that power leaves. Two by four or
+// four by two waves and three to five stages are within 3%; four larger waves are 8% slower.
 template <int BM, int BN, int WM, int WN, int NS>
 __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
   constexpr int WAVES = WM * WN, TM = BM / 32 / WM, TN = BN / 32 / WN;
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(256) mx_gemm_sum(const float* __restrict__ par
 // word for each k. The L1's requests bound it, so of the eight k's scales a lane loads one and takes
 // the others from its neighbours, and of a transposed A the two fragments' rows are neighbours, eight
 // bytes a k (1024^3 transposed 28.5 -> 25.0 us a run with both, 64x8192x8192 71 -> 66); addresses are
-// one base a wave and 32-bit offsets.
+// one base a wave and 32-bit offsets. 1024^3 takes 14.4 us, 149 TFLOP/s of binary32 products.
 template <bool TA>
 __device__ __forceinline__ void load_a8(const float* __restrict__ a, int64_t lda, int64_t m, int64_t k,
                                         int64_t K, float (&v)[8]) {

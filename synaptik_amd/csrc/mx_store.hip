@@ -29,7 +29,10 @@ __device__ __forceinline__ void store4(float* p, int rest, const float (&v)[4]) 
   }
 }
 
-// One group of 128 values for 32 lanes, four values a lane, U groups a lane and round.
+// One group of 128 values for 32 lanes, four values a lane, U groups a lane and round: a block is
+// eight lanes, whose largest magnitude goes round by DPP. Memory bounds it: [8192, 4096] to e2m1 takes
+// 26 us, 152 MB at 5.9 TB/s, and the way back 23 us, 6.6 TB/s; [500, 1021]
+// 2.9 us, little more than a launch.
 template <int F, bool KEEP, int U>
 __global__ void __launch_bounds__(256) mx_encode(const float* __restrict__ x, int64_t ldx,
                                                  uint8_t* __restrict__ codes,
@@ -187,7 +190,9 @@ int64_t act_grad_rows(int64_t R, int64_t C) {
 unsigned store_grid(int64_t groups, int u) {
   return (unsigned)std::min<int64_t>((groups + 8 * u - 1) / (8 * u), 1 << 20);
 }
-// Enough groups that every CU has work with four in flight a lane.
+// Enough groups that every CU has work with four in flight a lane (e4m3, us a run with four and with
+// one: encoding [256, 4096] 14.5 and 14.1, [1024, 4096] 16.4 and 16.2, [2048, 4096] 19.4 and 20.5,
+// [8192, 4096] 37.6 and 39.2; restoring the last 37.3 and 37.5).
 constexpr int64_t STORE_MANY = 4 * 8 * 1024;
 
 }  // namespace
