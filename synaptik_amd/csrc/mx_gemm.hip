@@ -499,11 +499,15 @@ __global__ void __launch_bounds__(512, 4) mx_direct(DirectParams p) {
 }
 
 // How a product runs (us on MI355X, e4m3, a synchronous run's 13 us included):
-//   * straight into registers up to 5 * 2^28 multiply-adds (1024^3 30.0, packed 34.5; 500x1021x1531
-//     30.5 against 33.3; but 1500x1500x1000 52 against 46), and whatever the depth for up to 64 rows
-//     or 128 columns, where packing the other operand costs most (64x8192x8192 73 against 93,
-//     4096x128x4096 44 against 76; 128 rows, 128x4096x4096, 47 against 45); two row fragments a
-//     workgroup from 2^28 on (64x4096x4096 35 against 41 with one, but 300x300x1000 22.2 against 21.7);
+//   * straight into registers up to 5 * 2^28 multiply-adds (1024^3 25.2, packed 33.8; 1250x1250x1000
+//     32.6 against 37.3; but 1500x1500x1000 52 against 44), 3 * 2^28 where there are tiles of 128 for
+//     three quarters of the CUs (2048x2048x200 25.5 against 26.2, but 2000x2000x300 34.4 against 28.8,
+//     4000x4000x60 35.5 against 32.1), and whatever the depth for up to 64 rows or 128 columns, where
+//     packing the other operand costs most (64x8192x8192 66 against 93, 4096x128x4096 40 against 76;
+//     128 rows, 128x4096x4096, 47 against 45); two row fragments a workgroup from 2^28 on (64x4096x4096
+//     35 against 41 with one, but 300x300x1000 22.2 against 21.7); eight waves a workgroup, or as few
+//     as make eight a CU and have four chunks each (2048x2048x200 25.2 against 34 with seven of one
+//     chunk, 3000x3000x100 33.9 against 39.5);
 //   * packed on tiles of 256, of 128, or the rows of as many rounds of 256 CUs as tiles of 256 fill and
 //     then the others on tiles of 128, whichever takes the fewest rounds; a tile of 256 takes 3.6 times
 //     one of 128 (4096^3 342 on 256, 368 on 128; 4000x2900x2048, 192 tiles, 155 against 148;
@@ -522,18 +526,18 @@ ProductPlan plan(int64_t M, int64_t N, int64_t K) {
   ProductPlan w{};
   const double work = (double)M * (double)N * (double)K;
   int64_t units, s;
-  if (work <= 5.0 * (1 << 28) || M <= 64 || N <= 128) {
+  auto tiles = [&](int64_t m, int64_t t) { return std::max<int64_t>(0, (m + t - 1) / t) * ((N + t - 1) / t); };
+  if (work <= (tiles(M, 128) < 192 ? 5.0 : 3.0) * (1 << 28) || M <= 64 || N <= 128) {
     w.direct = true;
     w.mb = work >= (double)(1 << 28) ? 2 : 1;
     units = (K + 31) / 32;
-    w.waves = (int)std::min<int64_t>(8, units);
     const int64_t t = ((N + 63) / 64) * ((M + 16 * w.mb - 1) / (16 * w.mb));
+    w.waves = (int)std::min<int64_t>({8, units, std::max<int64_t>((units + 3) / 4, (2048 + t - 1) / t)});
     s = std::min(512 / t, units / (2 * w.waves));
   } else {
     w.KT = units = (K + 15) / 16;
     w.MT = (M + 31) / 32;
     w.NT = (N + 31) / 32;
-    auto tiles = [&](int64_t m, int64_t t) { return std::max<int64_t>(0, (m + t - 1) / t) * ((N + t - 1) / t); };
     const int64_t strips = (M + 255) / 256, whole = tiles(M, 256) / 256 * 256 / tiles(1, 256);
     double least = 1e300;
     for (int64_t m : {(int64_t)0, whole, strips}) {  // rounds, in tiles of 128

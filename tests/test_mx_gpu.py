@@ -204,7 +204,7 @@ def gpu_mx_gemm(ctx, A, codes, scales, M, N, K, format, trans_a, lda=None, ldc=N
 PRODUCTS = [(1, 1, 1), (1, 5, 3), (3, 2, 40), (16, 16, 16), (33, 31, 32), (1, 1000, 700), (10, 300, 129),
             (64, 64, 64), (65, 130, 100), (128, 128, 512), (200, 10, 900), (255, 257, 333),
             (257, 513, 65), (512, 512, 512), (700, 390, 1025), (1024, 1030, 260), (130, 4100, 77),
-            (1025, 1023, 1027)]
+            (1025, 1023, 1027), (2100, 1030, 33), (2000, 1100, 190), (3000, 2900, 95)]
 # small tiles whole and split along K, large tiles, and large tiles ahead of small ones
 LARGE_PRODUCTS = [(4100, 2100, 70), (4000, 2000, 300), (1600, 1500, 600), (4100, 2100, 200), (4000, 4050, 90), (4600, 4000, 90)]
 
