@@ -512,9 +512,9 @@ __global__ void __launch_bounds__(512, 4) mx_direct(DirectParams p) {
 //     then the others on tiles of 128, whichever takes the fewest rounds; a tile of 256 takes 3.6 times
 //     one of 128 (4096^3 342 on 256, 368 on 128; 4000x2900x2048, 192 tiles, 155 against 148;
 //     4096x5120x2048, 320 tiles, 284, 250 and mixed 229; 5000x4000x2000 277, 232 and 224).
-// Either is split along K into as many slices as bring 512 (256 tiles) workgroups, of at least two
-// chunks of 32 k a wave (eight fragments): 16x4096x4096 27 in eight, packed 1024^3 34.5 in four and
-// 40.5 whole.
+// Either is split along K into as many slices as bring 256 workgroups, of at least two chunks of 32 k a
+// wave (eight fragments): 500x1021x1531 22.6 whole and 26.7 in two, 208x384x6272 26.9 in five and 29.3
+// in ten, 16x4096x4096 23.4 in four and 31.1 whole; packed 1024^3 34.5 in four and 40.5 whole.
 struct ProductPlan {
   bool direct;
   int mb, waves;            // direct: row fragments and waves a workgroup
@@ -533,7 +533,7 @@ ProductPlan plan(int64_t M, int64_t N, int64_t K) {
     units = (K + 31) / 32;
     const int64_t t = ((N + 63) / 64) * ((M + 16 * w.mb - 1) / (16 * w.mb));
     w.waves = (int)std::min<int64_t>({8, units, std::max<int64_t>((units + 3) / 4, (2048 + t - 1) / t)});
-    s = std::min(512 / t, units / (2 * w.waves));
+    s = std::min(256 / t, units / (2 * w.waves));
   } else {
     w.KT = units = (K + 15) / 16;
     w.MT = (M + 31) / 32;
