@@ -165,7 +165,8 @@ int32_t shk_hip_program_release(void* program);
 int32_t shk_hip_program_validate(const void* image, uint64_t image_bytes,
                                  uint64_t* out_arena_bytes);
 /* Runs the program once: binds in[i] / out[i] to the image's input / output slots by index,
- * validates sizes and aliasing (INCOMPATIBLE_RESOURCE), enqueues every step, waits, and maps
+ * validates sizes, aliasing and the alignment of microscaled operands (codes 16 bytes, scales
+ * 4; INCOMPATIBLE_RESOURCE), enqueues every step, waits, and maps
  * the device status word (ARITHMETIC, INDEX_OUT_OF_BOUNDS). Replaces
  * synaptik_metal_mpsgraph_executable_run (synaptik_metal_foundation.m:9984-10083).
  * Runs from several threads proceed concurrently on different leases; their kernels are

@@ -292,8 +292,9 @@ class ProgramBuilder:
     # ---- microscaled tensors ----
     # A microscaled [R, C] tensor is a pair of u8 slots (codes, scales): per row, groups of 128
     # values as codes of 8 bits (e4m3, e5m2) or 4 bits (e2m1, the even column in a byte's low
-    # half), and a power of two 2^(s - 127) for each block of 32 values. Codes behind the last
-    # column are zero.
+    # half), and a power of two 2^(s - 127) for each block of 32 values (s = 255: NaN). Codes behind
+    # the last column are zero, and no scale there is 255. Buffers bound to codes lie at a multiple
+    # of 16 bytes, to scales at a multiple of 4.
     def mx_tensor(self, rows: int, cols: int, format: str, kind: str = "internal"):
         """The (codes, scales) slots of a microscaled tensor: "internal", "input", "inout" or
         "output"."""
@@ -327,7 +328,9 @@ class ProgramBuilder:
     def mx_gemm(self, A, B, C, M, N, K, *, format="e4m3", trans_a=False, lda=None, ldc=None) -> Step:
         """C [M, N] = op(A) . B for a binary32 A [M, K] (trans_a: stored [K, M]) and a microscaled
         B = (codes, scales) [K, N]: a weight gradient dW = dZ^T . X from X's checkpoint, or an
-        input gradient dX = dZ . W through microscaled weights. A is not rounded."""
+        input gradient dX = dZ . W through microscaled weights. A is not rounded (a value counts with
+        an error below 2^-126); sums are binary32. A value that is not finite makes the results it
+        contributes to not finite, infinities or NaN."""
         return self._add(OP_MX_GEMM, [A, *B, C],
                          [M, N, K, lda if lda is not None else (M if trans_a else K),
                           ldc if ldc is not None else N, int(trans_a), _mx_format(format)])
