@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(SUMS == WHOLE ? 1024 : 256)
 
 // Whether one workgroup takes all rows of its columns, whose sums then need no second launch (us, a
 // run's 11 included: 500x4096 17.2 against 18.8, 1024x1000 18.5 against 19.5, 1024x4096 22.5 either
-// way, but 2048x1000 28.0 against 22.4).
-bool whole_sums(int64_t R) { return R <= 1024; }
+// way, but 2048x1000 28.0 against 22.4); a launch has fewer than 2^32 threads.
+bool whole_sums(int64_t R, int64_t C) { return R <= 1024 && C <= 1 << 26; }
 
 // Rows a workgroup takes otherwise: 16 (four a wave, all in flight at once) or as many as make 64
 // slabs of rows, whose sums the second launch reads fastest (4096x1000 24.7 us, with 32 / 128 / 256
@@ -238,7 +238,7 @@ hipError_t launch_mx_decode(const uint8_t* codes, const uint8_t* scales, float* 
 }
 
 int64_t mx_act_grad_partial_doubles(int64_t R, int64_t C) {
-  if (R <= 0 || C <= 0 || whole_sums(R)) return 0;
+  if (R <= 0 || C <= 0 || whole_sums(R, C)) return 0;
   const int64_t rows = act_grad_rows(R, C);
   return (R + rows - 1) / rows * C;
 }
@@ -247,7 +247,7 @@ hipError_t launch_mx_act_grad(const float* dy, int64_t ldy, const uint8_t* codes
                               const uint8_t* scales, float* dz, int64_t ldz, float* colsum, int64_t R,
                               int64_t C, int format, int act, double* partial, hipStream_t s) {
   if (C <= 0) return hipSuccess;
-  const bool whole = colsum != nullptr && whole_sums(R);
+  const bool whole = colsum != nullptr && whole_sums(R, C);
   const int64_t G = mx_groups(C), rows = whole ? R : act_grad_rows(R, C);
   const int64_t slabs = whole ? 1 : (R + rows - 1) / rows;
   if (slabs > 0) {

@@ -172,6 +172,21 @@ def test_activation_gradient_in_place_and_with_strides(ctx):
     prog.close()
 
 
+def test_activation_gradient_of_a_very_long_row(ctx):
+    """More columns than one launch of a workgroup for every 32 of them takes."""
+    C = (1 << 27) + 37
+    dy = np.tile(np.arange(-500, 501, dtype=np.float32), C // 1001 + 1)[:C]
+    groups = -(-C // 128)
+    codes = np.tile(np.arange(256, dtype=np.uint8) % 0x78, groups // 2 + 1)[:groups * 128]  # no NaN
+    pb = ProgramBuilder()
+    d, Y = pb.input(C), pb.mx_tensor(1, C, "e4m3", "input")
+    dz, db = pb.output(C), pb.output(C)
+    pb.mx_act_grad(d, Y, dz, 1, C, act="relu", colsum=db)
+    got = run_program(ctx, pb, [dy, codes, np.full(groups * 4, 127, np.uint8)], [dz, db])
+    want = np.where(codes[:C] > 0, dy, np.float32(0))
+    assert np.array_equal(got[0], want) and np.array_equal(got[1], want)
+
+
 def test_column_sums_of_no_rows_are_zero(ctx):
     pb = ProgramBuilder()
     d, Y = pb.input(0), pb.mx_tensor(0, 5, "e4m3", "input")
