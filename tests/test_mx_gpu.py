@@ -528,10 +528,11 @@ def test_weight_gradient_against_differences(ctx):
         assert abs(got[o, i] - diff) <= room
 
 
-def test_repeated_runs_graphs_and_the_static_entry_agree(ctx):
+@pytest.mark.parametrize("shape", [(300, 260, 280), (2100, 1300, 1290)], ids=str)
+def test_repeated_runs_graphs_and_the_static_entry_agree(ctx, shape):
     """The same bits from plain runs, graph replays with other work between them, an asynchronous
     run and the entry that allocates nothing."""
-    R, I, O = 300, 260, 280
+    R, I, O = shape
     rng = np.random.default_rng(8)
     ins = [a.astype(np.float32) for a in (rng.standard_normal((R, I)), rng.standard_normal((O, I)) / 16,
                                           rng.standard_normal(O), rng.standard_normal((R, O)))]
@@ -567,9 +568,10 @@ def test_repeated_runs_graphs_and_the_static_entry_agree(ctx):
     other.close()
 
 
-def test_concurrent_runs_of_one_program(ctx):
+@pytest.mark.parametrize("shape", [(40, 200, 300), (70, 200, 5000), (600, 1100, 1700)], ids=str)
+def test_concurrent_runs_of_one_program(ctx, shape):
     import threading
-    M, N, K = 40, 200, 300
+    M, N, K = shape
     rng = np.random.default_rng(1)
     codes, scales, _ = mx.stored(rng.standard_normal((N, K)), "e2m1")
     pb = ProgramBuilder()
