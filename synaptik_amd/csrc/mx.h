@@ -23,9 +23,9 @@ constexpr int mx_group_bytes(int format) { return format == MX_E2M1 ? 64 : 128; 
 
 // Encoding picks the smallest power of two under which the block's largest finite magnitude lies
 // within the format, so that nothing saturates (but for values that would round to 2^128: they take
-// the largest code below, MxFormat::LARGEST, so that a finite value stays finite), and never one below 2^MX_LEAST_EXPONENT: then
-// every nonzero value a code stands for (at least 2^-16 times its scale) is a normal binary32 and
-// bfloat16 number.
+// the largest code below, MxFormat::LARGEST, so that a finite value stays finite), and never one
+// below 2^MX_LEAST_EXPONENT: then every nonzero value a code stands for (at least 2^-16 times its
+// scale) is a normal binary32 and bfloat16 number.
 constexpr int MX_LEAST_EXPONENT = -110;
 
 template <int F>

@@ -394,8 +394,10 @@ __global__ void __launch_bounds__(512, 4) mx_direct(DirectParams p) {
   // row c of fragment i
   auto row_of = [&](int i) { return m0 + (TA ? MB * c + i : 16 * i + c); };
   // byte offsets of this lane's first values of a chunk
-  const uint32_t row_bytes = (uint32_t)p.G * mx_group_bytes(F), row_scales = (uint32_t)p.G * 4, lda4 = (uint32_t)p.lda * 4;
-  const uint32_t code_at = 8 * q * row_bytes + c * (F == MX_E2M1 ? 2 : 4), scale_at = (8 * q + (c & 7)) * row_scales + (c >> 3);
+  const uint32_t row_bytes = (uint32_t)p.G * mx_group_bytes(F), row_scales = (uint32_t)p.G * 4;
+  const uint32_t lda4 = (uint32_t)p.lda * 4;
+  const uint32_t code_at = 8 * q * row_bytes + c * (F == MX_E2M1 ? 2 : 4);
+  const uint32_t scale_at = (8 * q + (c & 7)) * row_scales + (c >> 3);
   uint32_t a_at[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
@@ -526,8 +528,7 @@ ProductPlan plan(int64_t M, int64_t N, int64_t K) {
   ProductPlan w{};
   const double work = (double)M * (double)N * (double)K;
   int64_t units, s;
-  auto tiles = [&](int64_t m, int64_t t) { return std::max<int64_t>(0, (m + t - 1) / t) * ((N + t - 1) / t); };
-  if (work <= (tiles(M, 128) < 192 ? 5.0 : 3.0) * (1 << 28) || M <= 64 || N <= 128) {
+  if (work <= (mx_tiles(M, N, 128) < 192 ? 5.0 : 3.0) * (1 << 28) || M <= 64 || N <= 128) {
     w.direct = true;
     w.mb = work >= (double)(1 << 28) ? 2 : 1;
     units = (K + 31) / 32;
@@ -538,13 +539,8 @@ ProductPlan plan(int64_t M, int64_t N, int64_t K) {
     w.KT = units = (K + 15) / 16;
     w.MT = (M + 31) / 32;
     w.NT = (N + 31) / 32;
-    const int64_t strips = (M + 255) / 256, whole = tiles(M, 256) / 256 * 256 / tiles(1, 256);
-    double least = 1e300;
-    for (int64_t m : {(int64_t)0, whole, strips}) {  // rounds, in tiles of 128
-      const double t = 3.6 * (double)((m * tiles(1, 256) + 255) / 256) + (double)((tiles(M - 256 * m, 128) + 255) / 256);
-      if (t < least) least = t, w.large = (int)m;
-    }
-    s = w.large ? 1 : std::min(256 / tiles(M, 128), units / 8);
+    w.large = mx_large_rows(M, N, 3.6);
+    s = w.large ? 1 : std::min(256 / mx_tiles(M, N, 128), units / 8);
   }
   s = std::max<int64_t>(1, s);
   w.chunk = (int)((units + s - 1) / s);

@@ -528,7 +528,6 @@ Plan plan(int64_t M, int64_t N, int64_t K, bool four) {
   const int64_t G = mx_groups(K);
   Plan w{TILES, 0, 0, 0, 1, (int)G};
   const double work = (double)M * (double)N * (double)K;
-  auto tiles = [&](int64_t m, int64_t t) { return std::max<int64_t>(0, (m + t - 1) / t) * ((N + t - 1) / t); };
   // (tiles address a row within 32 bits)
   if (M <= 16 || work < (M <= 64 ? 2.0 : 1.0) * (1 << 30) || K > (1 << 22)) {
     w.waves = (int)std::min<int64_t>(16, G);
@@ -545,17 +544,12 @@ Plan plan(int64_t M, int64_t N, int64_t K, bool four) {
     const bool in_line = w.mb == 1 && rows * G <= INLINE_GROUPS && (M <= 16 || M * G * N <= INLINE_WORK);
     w.route = in_line ? ROWS_INLINE : ROWS;
     if (in_line) w.waves = (int)std::max<int64_t>(w.waves, std::min<int64_t>(16, rows * G / 4));
-  } else if (tiles(M, 128) < 256 && G >= 16) {
-    const int64_t s = std::max<int64_t>(1, std::min(384 / tiles(M, 128), G / 4));
+  } else if (mx_tiles(M, N, 128) < 256 && G >= 16) {
+    const int64_t s = std::max<int64_t>(1, std::min(384 / mx_tiles(M, N, 128), G / 4));
     w.chunk = (int)((G + s - 1) / s);
     w.slices = (int)((G + w.chunk - 1) / w.chunk);
   } else {
-    const int64_t strips = (M + 255) / 256, whole = tiles(M, 256) / 256 * 256 / tiles(1, 256);
-    double least = 1e300;
-    for (int64_t m : {(int64_t)0, whole, strips}) {  // rounds, in tiles of 128
-      const double t = (four ? 2.6 : 3.6) * (double)((m * tiles(1, 256) + 255) / 256) + (double)((tiles(M - 256 * m, 128) + 255) / 256);
-      if (t < least) least = t, w.large = (int)m;
-    }
+    w.large = mx_large_rows(M, N, four ? 2.6 : 3.6);
   }
   return w;
 }
@@ -606,8 +600,8 @@ hipError_t launch(const LinearParams& p, const Plan& w, char* scratch, hipStream
     q.xt += row0;
     q.tiles_m = (rows + T - 1) / T;
     q.tiles_n = (p.N + T - 1) / T;
-    hipLaunchKernelGGL((mx_linear_tile<FX, FW, T, T, WM, 2, NS>), dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)w.slices),
-                       dim3(128 * WM), 0, s, q);
+    hipLaunchKernelGGL((mx_linear_tile<FX, FW, T, T, WM, 2, NS>),
+                       dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)w.slices), dim3(128 * WM), 0, s, q);
   };
   const int large = std::min(p.M, 256 * w.large);
   go(std::integral_constant<int, 256>(), 0, large);

@@ -257,9 +257,9 @@ hipError_t launch_mx_act_grad(const float* dy, int64_t ldy, const uint8_t* codes
         constexpr int ACT = decltype(a)::value;
         auto with = [&](auto sums, void* to) {
           constexpr int SUMS = decltype(sums)::value, COLS = SUMS == WHOLE ? 32 : 256;
-          hipLaunchKernelGGL((mx_act_grad<F, ACT, SUMS>), dim3((unsigned)((C + COLS - 1) / COLS), (unsigned)slabs),
-                             dim3(SUMS == WHOLE ? 1024 : 256), 0, s, dy, ldy, codes, scales, dz, ldz, to, R,
-                             (int)C, G, rows);
+          const dim3 grid((unsigned)((C + COLS - 1) / COLS), (unsigned)slabs);
+          hipLaunchKernelGGL((mx_act_grad<F, ACT, SUMS>), grid, dim3(SUMS == WHOLE ? 1024 : 256), 0, s, dy,
+                             ldy, codes, scales, dz, ldz, to, R, (int)C, G, rows);
         };
         if (colsum == nullptr) with(std::integral_constant<int, NO_SUMS>(), nullptr);
         else if (whole) with(std::integral_constant<int, WHOLE>(), colsum);

@@ -38,5 +38,23 @@ __device__ __forceinline__ void mx_tile_of(int id, int tiles_m, int tiles_n, int
   tn = in_band / rows;
 }
 
+// A product's tiles: how many of its rows of tiles of 256, the first ones, are taken (none, as many
+// as fill whole rounds of the 256 CUs, or all); the rows behind them go to tiles of 128. The fewest
+// rounds win, a tile of 256 counting `ratio` of 128.
+inline int64_t mx_tiles(int64_t M, int64_t N, int64_t edge) {
+  return M <= 0 ? 0 : ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
+}
+inline int mx_large_rows(int64_t M, int64_t N, double ratio) {
+  const int64_t all = (M + 255) / 256, row = mx_tiles(1, N, 256), filled = all * row / 256 * 256 / row;
+  int64_t best = 0;
+  double least = 1e300;
+  for (int64_t m : {(int64_t)0, filled, all}) {
+    const int64_t large = (m * row + 255) / 256, small = (mx_tiles(M - 256 * m, N, 128) + 255) / 256;
+    const double t = ratio * (double)large + (double)small;
+    if (t < least) least = t, best = m;
+  }
+  return (int)best;
+}
+
 }  // namespace
 }  // namespace shk
