@@ -13,6 +13,7 @@
 // it, and so is all that the part leads. (B's values are normal: scales start at 2^-110.)
 #include <algorithm>
 
+#include "launch_limits.h"
 #include "mx_tiles.h"
 
 namespace shk {
@@ -159,26 +160,29 @@ __device__ __forceinline__ void pack_b(const uint8_t* __restrict__ codes,
   for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8*>(at + 8 * 16 * j) = out[j];
 }
 
-// Both operands in one launch: workgroup (bk, block) packs 32 k of 64 rows of A, then of 256 columns
-// of B, the blocks of one bk in a row: they read and write neighbouring memory (a transposed 4096^2 A
-// and B 36.8 us, 208 MB at 5.7 TB/s; 43.1 with the k of one block in a row).
+// Both operands in one launch: unit (bk, block) is 32 k of 64 rows of A, then of 256 columns of B, the
+// blocks of one bk in a row: they read and write neighbouring memory (a transposed 4096^2 A and B 36.8
+// us, 208 MB at 5.7 TB/s; 43.1 with the k of one block in a row). A workgroup takes one, or several
+// where there are more than a launch has workgroups (launch_limits.h).
 struct PackParams {
   const float* A;
   const uint8_t* codes;
   const uint8_t* scales;
   char* pa;
   char* pb;
-  int64_t lda, M, N, K, G, MT, NT;
+  int64_t lda, M, N, K, G, MT, NT, units;
   int a_blocks, blocks;
 };
 template <int F, bool TA>
-__global__ void __launch_bounds__(256) mx_pack(PackParams p) {
-  const int64_t bk = blockIdx.x / p.blocks, block = blockIdx.x % p.blocks;
-  if (block < p.a_blocks) {
-    if (TA) pack_a_t(p.A, p.lda, p.pa, p.M, p.K, p.MT, bk, block);
-    else pack_a_n(p.A, p.lda, p.pa, p.M, p.K, p.MT, bk, block);
-  } else {
-    pack_b<F>(p.codes, p.scales, p.pb, p.N, p.K, p.G, p.NT, bk, block - p.a_blocks);
+__global__ void __launch_bounds__(PACK_THREADS) mx_pack(PackParams p) {
+  for (int64_t unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+    const int64_t bk = unit / p.blocks, block = unit - bk * p.blocks;
+    if (block < p.a_blocks) {
+      if (TA) pack_a_t(p.A, p.lda, p.pa, p.M, p.K, p.MT, bk, block);
+      else pack_a_n(p.A, p.lda, p.pa, p.M, p.K, p.MT, bk, block);
+    } else {
+      pack_b<F>(p.codes, p.scales, p.pb, p.N, p.K, p.G, p.NT, bk, block - p.a_blocks);
+    }
   }
 }
 
@@ -586,13 +590,13 @@ hipError_t launch_piece(const MxGemmParams& p, int64_t G, void* scratch, hipStre
       else by_rows(std::false_type());
     });
   } else {
-    PackParams k{p.A, p.codes, p.scales, pa, pb, p.lda, p.M, p.N, p.K, G, w.MT, w.NT, (int)((p.M + 63) / 64)};
-    k.blocks = (int)(k.a_blocks + (p.N + 255) / 256);
-    const dim3 packs((unsigned)((w.KT + 1) / 2 * k.blocks));
+    PackParams k{p.A, p.codes, p.scales, pa, pb, p.lda, p.M, p.N, p.K, G, w.MT, w.NT,
+                 mx_pack_units(p.M, p.N, p.K), (int)((p.M + 63) / 64), (int)mx_pack_blocks(p.M, p.N)};
+    const dim3 packs((unsigned)mx_pack_groups(k.units));
     mx_with_format(p.format, [&](auto f) {
       constexpr int F = decltype(f)::value;
-      if (p.transA) hipLaunchKernelGGL((mx_pack<F, true>), packs, dim3(256), 0, s, k);
-      else hipLaunchKernelGGL((mx_pack<F, false>), packs, dim3(256), 0, s, k);
+      if (p.transA) hipLaunchKernelGGL((mx_pack<F, true>), packs, dim3(PACK_THREADS), 0, s, k);
+      else hipLaunchKernelGGL((mx_pack<F, false>), packs, dim3(PACK_THREADS), 0, s, k);
     });
     WideParams q{};
     q.pb = pb;
