@@ -15,6 +15,7 @@
 // Java Math.max (NaN wins, +0.0 beats -0.0).
 #include "common.h"
 #include "kernels.h"
+#include "launch_limits.h"
 #include "pw_divide.h"
 #include "rowvec.h"
 #include <algorithm>
@@ -295,7 +296,7 @@ __global__ void copy_kernel(const float* __restrict__ s, float* __restrict__ d, 
 // Column sums, pass 1: block (cx, ry) sums a 64-column x `rows`-row panel; each of the 4 waves
 // walks a quarter of the panel's rows with lanes on consecutive columns (coalesced 256 B rows).
 // The panel height is chosen per call so that a launch has ~1024 blocks even for short inputs.
-constexpr int CS_COLS = 64;
+constexpr int CS_COLS = COLSUM_WIDTH;
 constexpr int64_t CS_TARGET_BLOCKS = 1024;
 int64_t colsum_rows_per_panel(int64_t R, int64_t N) {
   const int64_t colblocks = (N + CS_COLS - 1) / CS_COLS;
@@ -453,6 +454,14 @@ __global__ void __launch_bounds__(256) colsum_pass2(const double* part, float* o
     float v = (float)(s / divisor);
     if (accumulate) v = out[col] + v;
     out[col] = v;
+  }
+}
+void launch_colsum_pass2(const double* part, float* out, int64_t P, int64_t N, int64_t step, double divisor,
+                         int accumulate, hipStream_t s) {
+  for (int64_t n = 0; n < N; n += COLSUM_COLS) {
+    const int64_t cols = std::min(COLSUM_COLS, N - n);
+    hipLaunchKernelGGL(colsum_pass2, dim3((unsigned)colsum_groups(cols)), dim3(COLSUM_THREADS), 0, s, part + n,
+                       out + n, P, cols, step, divisor, accumulate);
   }
 }
 
@@ -874,6 +883,14 @@ int64_t colsum_partial_doubles(int64_t R, int64_t N) {
 hipError_t launch_colsum(const float* x, float* out, int64_t R, int64_t N, int64_t ldx,
                          double divisor, int accumulate, double* partial, hipStream_t s) {
   if (N <= 0) return hipSuccess;
+  if (N > 2 * COLSUM_COLS - 4 * CS_COLS) {
+    for (int64_t n = 0; n < N; n += COLSUM_COLS) {
+      const hipError_t e = launch_colsum(x + n, out + n, R, std::min(COLSUM_COLS, N - n), ldx, divisor,
+                                         accumulate, partial, s);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   if (N <= CS_SMALL_MAX_N && R <= CS_SMALL_MAX_R) {
     hipLaunchKernelGGL(colsum_small, dim3((unsigned)((N + CS_COLS - 1) / CS_COLS)), dim3(1024), 0,
                        s, x, out, R, N, ldx, divisor, accumulate);
@@ -886,8 +903,7 @@ hipError_t launch_colsum(const float* x, float* out, int64_t R, int64_t N, int64
     // (64 columns fill colsum_pass1's lanes: [1000000, 33] 120 us, 144 in fours)
     if (N > CS_COLS && (aligned || R > CS_FEW_UNALIGNED || (R > 4 && N > CS_FEW_COLS))) {
       dim3 g1((unsigned)((N + 4 * CS_COLS - 1) / (4 * CS_COLS)), (unsigned)P);
-      // (sixteen waves of 2^30 and more columns are more threads than a grid dimension holds)
-      if (R <= CS_FEW_ROWS || N >= (1ll << 30) - 4 * CS_COLS)
+      if (R <= CS_FEW_ROWS)
         hipLaunchKernelGGL(colsum_pass1_v4<4>, g1, dim3(256), 0, s, x, partial, R, N, ldx, rows);
       else
         hipLaunchKernelGGL(colsum_pass1_v4<16>, g1, dim3(1024), 0, s, x, partial, R, N, ldx, rows);
@@ -896,8 +912,7 @@ hipError_t launch_colsum(const float* x, float* out, int64_t R, int64_t N, int64
       hipLaunchKernelGGL(colsum_pass1, g1, dim3(256), 0, s, x, partial, R, N, ldx, rows);
     }
   }
-  hipLaunchKernelGGL(colsum_pass2, dim3((unsigned)((N + CS_COLS - 1) / CS_COLS)), dim3(256), 0, s,
-                     partial, out, P, N, N, divisor, accumulate);
+  launch_colsum_pass2(partial, out, P, N, N, divisor, accumulate, s);
   return hipGetLastError();
 }
 
@@ -913,8 +928,7 @@ hipError_t launch_colsum_finish(double* partial, float* out, int64_t P, int64_t 
     P = chunks;
     step = CS_FOLD_CHUNK * N;
   }
-  hipLaunchKernelGGL(colsum_pass2, dim3(x), dim3(256), 0, s, (const double*)partial, out, P, N, step,
-                     1.0, 0);
+  launch_colsum_pass2(partial, out, P, N, step, 1.0, 0, s);
   return hipGetLastError();
 }
 

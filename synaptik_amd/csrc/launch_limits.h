@@ -18,4 +18,9 @@ inline int64_t mx_pack_units(int64_t M, int64_t N, int64_t K) {
 }
 inline int64_t mx_pack_groups(int64_t units) { return units < PACK_GROUPS ? units : PACK_GROUPS; }
 
+// Column sums have a workgroup of COLSUM_THREADS for every COLSUM_WIDTH columns at the least, which 2^30
+// columns would take beyond a launch: wider ones go COLSUM_COLS at a time.
+constexpr int64_t COLSUM_WIDTH = 64, COLSUM_THREADS = 256, COLSUM_COLS = 1ll << 29;
+inline int64_t colsum_groups(int64_t cols) { return (cols + COLSUM_WIDTH - 1) / COLSUM_WIDTH; }
+
 }  // namespace shk

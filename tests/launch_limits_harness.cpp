@@ -23,6 +23,18 @@ static int check_pack(int64_t M, int64_t N, int64_t K) {
   return 0;
 }
 
+// pieces of COLSUM_COLS columns, COLSUM_THREADS for every COLSUM_WIDTH of a piece
+static int check_colsum(int64_t N) {
+  int64_t reached = 0;
+  for (int64_t n = 0; n < N; n += COLSUM_COLS) {
+    const int64_t cols = N - n < COLSUM_COLS ? N - n : COLSUM_COLS;
+    if (colsum_groups(cols) * COLSUM_THREADS > LAUNCH_THREADS) return fail("column sums' threads", N, n, cols);
+    if (colsum_groups(cols) * COLSUM_WIDTH < cols) return fail("column sums' width", N, n, cols);
+    reached += cols;
+  }
+  return reached == N ? 0 : fail("column sums' pieces", N, reached, 0);
+}
+
 int main() {
   if (LAUNCH_THREADS != 0xffffffffll) return fail("threads", LAUNCH_THREADS, 0, 0);
   const int64_t depths[] = {1, 15, 16, 31, 32, 33, 4096, 700000, 179000000, 1ll << 30, (1ll << 31) - 1};
@@ -31,6 +43,10 @@ int main() {
     for (int64_t M : extents)
       for (int64_t N : extents)
         if (check_pack(M, N, K)) return 1;
+  for (int64_t N : {(int64_t)1, (int64_t)65, (1ll << 29) + 1, (1ll << 30) - 64, (1ll << 30) - 63, (1ll << 31) - 257, 1ll << 34})
+    if (check_colsum(N)) return 1;
+  // from here on one launch does not do
+  if (colsum_groups((1ll << 30) - 63) * COLSUM_THREADS <= LAUNCH_THREADS) return fail("wide", 1ll << 30, 0, 0);
   // the shape whose units alone fill more than a launch: 2^32 threads, one unit each
   if (mx_pack_units(65, 129, 179000000) * PACK_THREADS <= LAUNCH_THREADS) return fail("deep", 65, 129, 179000000);
   // one that a device test runs takes more than one unit a workgroup

@@ -3,6 +3,7 @@ round more than once (synaptik_amd/csrc/launch_limits.h)."""
 import numpy as np
 import pytest
 
+from synaptik_amd.native import HipProgram
 from synaptik_amd.program import ProgramBuilder
 from tests.gpu_helpers import run_program
 
@@ -28,3 +29,49 @@ def test_product_deeper_than_one_round_of_packing(ctx, trans_a):
     (got,) = run_program(ctx, pb, [A.T if trans_a else A, codes, scales], [c])
     want = A @ value[nibble[:, :N]]
     assert np.array_equal(got.reshape(M, N), want)
+
+
+def sums_of_a_row(ctx, C, add):
+    """The column sums, at places, of one row of C floats: 1.5 but for a hundred numbers from each
+    place on. add(pb, row slot) adds the step and gives (its other inputs, the slot of the sums, the
+    other outputs)."""
+    places = [0, (1 << 29) - 50, (1 << 30) - 100, C - 100]
+    pb = ProgramBuilder()
+    row = pb.output(C)
+    pb.fill(row, C, 1.5)
+    prog = HipProgram(ctx, pb.image())
+    buf = ctx.buffer(4 * C)
+    prog.run([], [buf])
+    prog.close()
+    for i, at in enumerate(places):
+        buf.upload(np.arange(100, dtype=np.float32) + 100 * i, 4 * at)
+    pb = ProgramBuilder()
+    ins, sums, outs = add(pb, pb.input(C))
+    prog = HipProgram(ctx, pb.image())
+    made = {id(s): ctx.buffer(s.nbytes) for s in ins + outs + [sums]}
+    made[id(sums)].upload(np.full(200, -7.0, np.float32), 4 * (C - 200))
+    prog.run([buf] + [made[id(s)] for s in ins], [made[id(s)] for s in outs + [sums]])
+    prog.close()
+    for i, at in enumerate(places):
+        got = made[id(sums)].download(count=100, offset=4 * at)
+        assert np.array_equal(got, np.arange(100, dtype=np.float32) + 100 * i), at
+    got = made[id(sums)].download(count=100, offset=4 * (C - 200))
+    assert np.array_equal(got, np.full(100, 1.5, np.float32))
+
+
+def test_column_sums_of_more_columns_than_a_launch_finishes(ctx):
+    """2^30 columns and more: 256 threads for every 64 of them are more than a launch has."""
+    C = (1 << 30) + 300
+
+    def act_grad(pb, row):
+        Y, dz, db = pb.mx_tensor(1, C, "e2m1", "input"), pb.output(C), pb.output(C)
+        pb.mx_act_grad(row, Y, dz, 1, C, act=None, format="e2m1", colsum=db)
+        return list(Y), db, [dz]
+
+    def colsum(pb, row):
+        db = pb.output(C)
+        pb.colsum(row, db, 1, C)
+        return [], db, []
+
+    sums_of_a_row(ctx, C, act_grad)
+    sums_of_a_row(ctx, C, colsum)
