@@ -11,6 +11,11 @@
 //   e4m3 (0): 1 sign, 4 exponent, 3 mantissa bits, largest 448, no infinities, NaN 0x7f / 0xff
 //   e5m2 (1): 1, 5, 2, largest 57344, infinities 0x7c / 0xfc, NaN above
 //   e2m1 (2): 1, 2, 1, values 0, 0.5, 1, 1.5, 2, 3, 4, 6; neither infinities nor NaN
+// Restoring and gradients take every scale as it is. The products take values that are zero or from
+// 2^-126 to below 2^128 in magnitude exactly, which is all that encoding gives, and all that scales of
+// 17 to 239 give in any format. Through bfloat16 a smaller one counts with an error below 2^-126 (the
+// matrix cores read subnormal values as zeros) and a larger one as an infinity; the scaled 4-bit
+// instructions take both as they are.
 #pragma once
 #include "common.h"
 

@@ -10,7 +10,8 @@
 // instead of the binary32 ones', 5.3 times as fast (2.5 / 3 against 0.157 PFLOP/s).
 // The matrix cores read subnormal bfloat16 values as zeros, so a value of A counts with an error
 // below 2^-126, the smallest normal binary32 value: the first part that is read as zero is below
-// it, and so is all that the part leads. (B's values are normal: scales start at 2^-110.)
+// it, and so is all that the part leads. A value of B below 2^-126 counts with such an error too;
+// those that encoding gives are zero or normal (its scales start at 2^-110).
 #include <algorithm>
 
 #include "launch_limits.h"

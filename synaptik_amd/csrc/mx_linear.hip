@@ -1,7 +1,7 @@
 // Y = act(X . W^T + b) of microscaled weights W [N, K] (mx.h) and binary32 activations X [M, K],
-// encoded here. The products of stored values are exact in bfloat16's matrix instructions, and of
-// e2m1 on both sides in the scaled ones, which run up to four times as fast (10 against 2.5
-// PFLOP/s); sums are binary32.
+// encoded here. The products of stored values (zero or in the normal range, mx.h) are exact in
+// bfloat16's matrix instructions, and of e2m1 on both sides in the scaled ones, which run up to four
+// times as fast (10 against 2.5 PFLOP/s); sums are binary32.
 #include <algorithm>
 
 #include "mx_tiles.h"

@@ -294,7 +294,11 @@ class ProgramBuilder:
     # values as codes of 8 bits (e4m3, e5m2) or 4 bits (e2m1, the even column in a byte's low
     # half), and a power of two 2^(s - 127) for each block of 32 values (s = 255: NaN). Codes behind
     # the last column are zero, and no scale there is 255. Buffers bound to codes lie at a multiple
-    # of 16 bytes, to scales at a multiple of 4.
+    # of 16 bytes, to scales at a multiple of 4. The products (mx_gemm, mx_linear) take values that are
+    # zero or from 2^-126 to below 2^128 in magnitude exactly: all that mx_encode gives, and all that
+    # scales of 17 to 239 give in any format. Of codes under other scales a value below 2^-126 counts
+    # in a product with an error below 2^-126 (it may count as zero), and one of 2^128 or more is
+    # infinite, or counts as it is where both operands are e2m1.
     def mx_tensor(self, rows: int, cols: int, format: str, kind: str = "internal"):
         """The (codes, scales) slots of a microscaled tensor: "internal", "input", "inout" or
         "output"."""
@@ -329,7 +333,7 @@ class ProgramBuilder:
         """C [M, N] = op(A) . B for a binary32 A [M, K] (trans_a: stored [K, M]) and a microscaled
         B = (codes, scales) [K, N]: a weight gradient dW = dZ^T . X from X's checkpoint, or an
         input gradient dX = dZ . W through microscaled weights. A is not rounded (a value counts with
-        an error below 2^-126); sums are binary32. A value that is not finite makes the results it
+        an error below 2^-126, and so does one of B below 2^-126); sums are binary32. A value that is not finite makes the results it
         contributes to not finite, infinities or NaN."""
         return self._add(OP_MX_GEMM, [A, *B, C],
                          [M, N, K, lda if lda is not None else (M if trans_a else K),
