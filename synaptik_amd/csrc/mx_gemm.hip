@@ -11,7 +11,8 @@
 // The matrix cores read subnormal bfloat16 values as zeros, so a value of A counts with an error
 // below 2^-126, the smallest normal binary32 value: the first part that is read as zero is below
 // it, and so is all that the part leads. A value of B below 2^-126 counts with such an error too;
-// those that encoding gives are zero or normal (its scales start at 2^-110).
+// those that encoding gives are zero or normal (its scales start at 2^-110). An infinite code of B
+// gives NaN, since it meets parts of A that are zero.
 #include <algorithm>
 
 #include "launch_limits.h"

@@ -334,7 +334,8 @@ class ProgramBuilder:
         B = (codes, scales) [K, N]: a weight gradient dW = dZ^T . X from X's checkpoint, or an
         input gradient dX = dZ . W through microscaled weights. A is not rounded (a value counts with
         an error below 2^-126, and so does one of B below 2^-126); sums are binary32. A value that is not finite makes the results it
-        contributes to not finite, infinities or NaN."""
+        contributes to not finite: an infinity of A gives infinities or NaN, an infinite code of B
+        NaN, where a binary32 product may give an infinity."""
         return self._add(OP_MX_GEMM, [A, *B, C],
                          [M, N, K, lda if lda is not None else (M if trans_a else K),
                           ldc if ldc is not None else N, int(trans_a), _mx_format(format)])

@@ -69,3 +69,44 @@ def test_linear_layers_under_every_scale(ctx, shape, x_format, w_format):
     assert (np.abs(got - want) <= x * LEAST)[small].all()
     assert (np.abs(got)[np.abs(want) < LEAST] <= LEAST).all()
     assert np.isinf(got[np.abs(want) >= 2.0 ** 128]).all()
+
+
+@pytest.mark.parametrize("trans_a", [False, True])
+@pytest.mark.parametrize("shape", GEMM_SHAPES, ids=str)
+def test_an_infinite_code_reaches_its_column_alone(ctx, shape, trans_a):
+    """e5m2 has infinities. The wide operand goes to the products in three parts, of which those that
+    are zero make NaN of an infinite code, so a result is NaN where a binary32 product would be
+    infinite: not finite in its whole column, and nowhere else. The last row of B is one that the
+    kernels may read again behind the depth."""
+    M, N, K = shape
+    rng = np.random.default_rng(K)
+    # small whole numbers: sums below 2^24, exact in binary32
+    A = rng.integers(-3, 4, (M, K)).astype(np.float32)
+    B = rng.integers(-3, 4, (K, N)).astype(np.float64)
+    columns = [1, N // 2, N - 1]
+    B[K // 2, 1], B[K - 1, N // 2], B[0, N - 1] = np.inf, -np.inf, np.inf
+    codes, scales, back = mx.stored(B, "e5m2")
+    assert np.array_equal(back, B)
+    got = gpu_mx_gemm(ctx, A.T if trans_a else A, codes, scales, M, N, K, "e5m2", trans_a)
+    assert not np.isfinite(got[:, columns]).any()
+    ok = np.setdiff1d(np.arange(N), columns)
+    assert np.array_equal(got[:, ok], A.astype(np.float64) @ B[:, ok])
+
+
+@pytest.mark.parametrize("x_format", mx.FORMATS)
+@pytest.mark.parametrize("shape", LINEAR_SHAPES, ids=str)
+def test_an_infinite_weight_is_an_infinity(ctx, shape, x_format):
+    """In a linear layer each product is one exact term: an infinite code against values that are not
+    zero gives an infinity of the right sign in its column, and touches no other."""
+    M, N, K = shape
+    rng = np.random.default_rng(M)
+    X = (rng.integers(1, 4, (M, K)) * rng.choice([-1, 1], (M, K))).astype(np.float32)
+    W = rng.integers(-3, 4, (N, K)).astype(np.float64)
+    W[3, K - 1], W[N - 1, 0] = np.inf, -np.inf
+    codes, scales, back = mx.stored(W, "e5m2")
+    assert np.array_equal(back, W) and np.array_equal(mx.stored(X, x_format)[2], X)
+    got = gpu_mx_linear(ctx, X, (codes, scales), None, M, N, K, x_format, "e5m2", None)
+    assert np.array_equal(got[:, 3], np.sign(X[:, K - 1]) * np.inf)
+    assert np.array_equal(got[:, N - 1], np.sign(X[:, 0]) * -np.inf)
+    ok = np.setdiff1d(np.arange(N), [3, N - 1])
+    assert np.array_equal(got[:, ok], X.astype(np.float64) @ W[ok].T)
