@@ -234,7 +234,11 @@ def lower_training_step(spec: MlpSpec, batch: int, optimizer, *, label_dtype: st
     pass as microscaled 8-bit values (ProgramBuilder.mx_encode with keep_nonzero, so that ReLU's
     masks are exact) instead of binary32: 1.03 bytes a value instead of 4, and the forward and
     backward passes then share two binary32 buffers each. The forward pass and the objective are
-    those of the uncompressed step; the gradients are those of the kept values.
+    those of the uncompressed step; the gradients are those of the kept values. ReLU's slopes are exact;
+    those of tanh (1 - y^2) and sigmoid (y (1 - y)) come from outputs that are kept to 1/16 (e4m3) or
+    1/8 (e5m2) below one: they are zero for every |y| of at least 31/32 (e4m3) or 15/16 (e5m2), and
+    coarse below (0.234 instead of 0.19 at y = 0.9 of tanh). Layers that rely on nearly saturated
+    units should train without checkpoints.
     """
     if checkpoint not in CHECKPOINTS:
         raise ValueError(f"unsupported checkpoint format {checkpoint!r}")
