@@ -522,8 +522,9 @@ int32_t validate_mx_step(Validator& v, size_t idx, const Step& st, uint64_t* scr
     }
     default: {  // OP_MX_LINEAR
       const int64_t M = a[0], N = a[1], K = a[2], ldx = a[3], ldy = a[4], act = a[7];
-      if (M < 0 || N < 0 || K < 0 || M > INT32_MAX / 2 || N > INT32_MAX / 2 || !ld_ok(M, N, ldy) ||
-          (N > 0 && !ld_ok(M, K, ldx)) || !format_ok(a[5]) || !format_ok(a[6]) || act < 0 || act > 3)
+      if (M < 0 || N < 0 || K < 0 || M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX - 256 ||
+          !ld_ok(M, N, ldy) || (N > 0 && !ld_ok(M, K, ldx)) || !format_ok(a[5]) || !format_ok(a[6]) ||
+          act < 0 || act > 3)
         return bad_shape("microscaled linear layer");
       if (prod(M, (K + 127) / 128) > INT32_MAX) return bad_shape("microscaled linear layer");
       if (!v.slot_ok(s[0], false, "X") || !v.holds(s[0], span(M, K, ldx), DT_F32, "X") ||
