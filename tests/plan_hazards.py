@@ -7,7 +7,8 @@ synaptik_amd/csrc/*.hip), not from runtime.cpp's step_access:
 
 - slots read and written (operands, outputs, optimizer tensors, the step counter);
 - the reduction scratch of the stream the step runs on (GEMM split-K partials and column-sum
-  partials, COLSUM, REDUCE_ALL, MSE and CE_INDEX partials): read and written;
+  partials, COLSUM, REDUCE_ALL, MSE and CE_INDEX partials, the packed and encoded operands of
+  microscaled products): read and written;
 - the device status word: OR-ed by atomics (commuting with each other), or read by steps that
   act only on a clear word (the optimizer's apply phase, the accumulator commit and clear, the
   step commit), and read and cleared by the run's publication kernel.
@@ -31,6 +32,7 @@ _HDR = struct.Struct("<IIII")
 _SLOT = struct.Struct("<QIIII")
 _STEP = struct.Struct("<II8i16q8f")
 _OPT = struct.Struct("<iiiiiiiiq")
+_PRODUCTS = (P.OP_GEMM, P.OP_MX_GEMM, P.OP_MX_LINEAR)
 
 @dataclass
 class DecodedStep:
@@ -174,6 +176,24 @@ def effects(st: DecodedStep, stream: int | None, status_reads: bool = True) -> E
     elif op in (P.OP_COPY, P.OP_TRANSPOSE):
         R(s[0])
         W(s[1])
+    elif op == P.OP_MX_ENCODE:
+        R(s[0])
+        W(s[1], s[2])
+    elif op == P.OP_MX_DECODE:
+        R(s[0], s[1])
+        W(s[2])
+    elif op == P.OP_MX_ACT_GRAD:  # (partial column sums in the scratch)
+        R(s[0], s[1], s[2])
+        W(s[3], s[4])
+        _scratch(e, scratch)
+    elif op == P.OP_MX_GEMM:  # (fragments and partial sums)
+        R(s[0], s[1], s[2])
+        W(s[3])
+        _scratch(e, scratch)
+    elif op == P.OP_MX_LINEAR:  # (X encoded, scales in the tiles' order, partial sums)
+        R(s[0], s[1], s[2], s[3])
+        W(s[4])
+        _scratch(e, scratch)
     else:
         raise ValueError(f"step {st.index}: opcode {op} has no effects model")
     return e
@@ -288,7 +308,7 @@ def critical_path_plan(steps: list[DecodedStep]):
 
     def cost(st):
         a = st.iargs
-        if st.opcode == P.OP_GEMM:
+        if st.opcode in _PRODUCTS:
             return max(1, a[0] * a[1] * a[2])
         return max(1, a[0] * max(1, a[1]))
 
@@ -328,7 +348,7 @@ def greedy_plan(steps: list[DecodedStep], status_reads: bool = True):
     for j in range(n):
         deps = [i for i in range(j) if conflict(eff[i], eff[j], read_read=True)]
         a = steps[j].iargs
-        large = steps[j].opcode == P.OP_GEMM and min(a[0], a[1], a[2]) > 0 and \
+        large = steps[j].opcode in _PRODUCTS and min(a[0], a[1], a[2]) > 0 and \
             a[0] * a[1] * a[2] >= 1 << 28
         on_tail = tail0 < 0 or tail0 in deps
         stream_of[j] = 0 if (on_tail or large) else 1
