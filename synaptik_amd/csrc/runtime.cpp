@@ -1106,15 +1106,12 @@ bool concurrency_enabled() {
   }();
   return on;
 }
-// Two-stream list schedule: step j goes beside the main chain (stream 1) when it does not
-// depend on the step currently at the tail of stream 0; a step waits (event) for every earlier
-// step on the other stream it depends on. Steps on one stream keep program order.
-// (iarg 0, 1, 2 of the matrix products are their extents M, N, K)
+// Matrix products, whose iarg 0, 1, 2 are their extents M, N, K.
 bool is_product(const Step& st) {
   const uint32_t op = st.rec.opcode;
   return op == OP_GEMM || op == OP_MX_GEMM || op == OP_MX_LINEAR;
 }
-// A GEMM with at least 2^28 multiply-adds: enough tiles to occupy every CU on its own.
+// One with at least 2^28 multiply-adds: enough tiles to occupy every CU on its own.
 bool large_gemm(const Step& st) {
   if (!is_product(st)) return false;
   const int64_t* a = st.rec.iarg;
@@ -1181,6 +1178,9 @@ void plan_fold(Program* pr) {
   });
 }
 
+// Two-stream list schedule: step j goes beside the main chain (stream 1) when it does not
+// depend on the step currently at the tail of stream 0; a step waits (event) for every earlier
+// step on the other stream it depends on. Steps on one stream keep program order.
 void plan_streams(Program* pr) {
   const size_t n = pr->steps.size();
   pr->stream_of.assign(n, 0);

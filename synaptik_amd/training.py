@@ -197,7 +197,9 @@ class TrainingLayout:
     x: Slot | None = None
     y: Slot | None = None
     loss: Slot | None = None
-    grads: list[Slot] = field(default_factory=list)
+    # gradients of weights, then of biases; a checkpointed step that updates at once has none for the
+    # first layer's weights (None) and one slot that the other layers' share
+    grads: list[Slot | None] = field(default_factory=list)
 
 
 def _optimizer_kind(opt) -> str:
