@@ -163,8 +163,8 @@ __device__ __forceinline__ void pack_b(const uint8_t* __restrict__ codes,
 }
 
 // Both operands in one launch: unit (bk, block) is 32 k of 64 rows of A, then of 256 columns of B, the
-// blocks of one bk in a row: they read and write neighbouring memory (a transposed 4096^2 A and B 36.8
-// us, 208 MB at 5.7 TB/s; 43.1 with the k of one block in a row). A workgroup takes one, or several
+// blocks of one bk in a row: they read and write neighbouring memory (a transposed 4096^2 A and B 34.5
+// us, 219 MB at 6.3 TB/s; a sixth more with the k of one block in a row). A workgroup takes one, or several
 // where there are more than a launch has workgroups (launch_limits.h).
 struct PackParams {
   const float* A;
@@ -205,9 +205,10 @@ struct WideParams {
 // read is linear. A stage is copied NS - 1 stages before it is read; before a stage is read, each
 // wave has waited for its own copies into it, and has finished with the stage whose place the next
 // copies take. A stage's fragments are read while the one before is multiplied. The matrix cores
-// bound it: 4096^3 takes 266 us, the three products together 1.55 PFLOP/s (a large bfloat16 product of
-// the library 1.34), the cores busy 77% of the cycles at the 1.92 GHz that power leaves. Two by four or
-// four by two waves and three to five stages are within 3%; four larger waves are 8% slower.
+// bound it: 4096^3 takes 244 us under steady load, the three products together 1.69 PFLOP/s (a large
+// bfloat16 product of the library 1.34), and 266 in the first passes after a pause, when power leaves
+// 1.92 GHz and the cores are busy 77% of the cycles. Two by four or four by two waves and three to five
+// stages are within 3%; four larger waves are 8% slower.
 template <int BM, int BN, int WM, int WN, int NS>
 __global__ void __launch_bounds__(64 * WM * WN) mx_wide(WideParams p) {
   constexpr int WAVES = WM * WN, TM = BM / 32 / WM, TN = BN / 32 / WN;
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(256) mx_gemm_sum(const float* __restrict__ par
 // word for each k. The L1's requests bound it, so of the eight k's scales a lane loads one and takes
 // the others from its neighbours, and of a transposed A the two fragments' rows are neighbours, eight
 // bytes a k (1024^3 transposed 28.5 -> 25.0 us a run with both, 64x8192x8192 71 -> 66); addresses are
-// one base a wave and 32-bit offsets. 1024^3 takes 14.4 us, 149 TFLOP/s of binary32 products.
+// one base a wave and 32-bit offsets. 1024^3 takes 12.2 us, 176 TFLOP/s of binary32 products.
 template <bool TA>
 __device__ __forceinline__ void load_a8(const float* __restrict__ a, int64_t lda, int64_t m, int64_t k,
                                         int64_t K, float (&v)[8]) {
@@ -506,7 +507,8 @@ __global__ void __launch_bounds__(512, 4) mx_direct(DirectParams p) {
   }
 }
 
-// How a product runs (us on MI355X, e4m3, a synchronous run's 13 us included):
+// How a product runs (us on MI355X, e4m3, a synchronous run's 13 us included, both sides in turn in
+// short runs; under steady load large products take up to a tenth less):
 //   * straight into registers up to 5 * 2^28 multiply-adds (1024^3 25.2, packed 33.8; 1250x1250x1000
 //     32.6 against 37.3; but 1500x1500x1000 52 against 44), 3 * 2^28 where there are tiles of 128 for
 //     three quarters of the CUs (2048x2048x200 25.5 against 26.2, but 2000x2000x300 34.4 against 28.8,

@@ -213,9 +213,10 @@ __global__ void __launch_bounds__(1024) mx_linear_rows(LinearParams p) {
 //     width than it has.
 // The 16-byte chunks of a row are permuted by the row's ordinal so that the 16 lanes that read
 // together meet every bank once. Scales come as [group][row] words of four from the launch that
-// encodes X. 8192x4096x4096 of e4m3 by e2m1 takes 233 us, 1.18 PFLOP/s: the matrix cores are busy 55% of
-// the cycles at 2.04 GHz, the vector ALUs' conversions (four an instruction of theirs) most of the
-// others. With 4 bits on both sides it takes 95 us, 2.9 PFLOP/s, a quarter of it the results' store.
+// encodes X. 8192x4096x4096 of e4m3 by e2m1 takes 217 us under steady load, 1.27 PFLOP/s, and 233 in the first
+// passes after a pause: the matrix cores are busy 55% of the cycles then, at 2.04 GHz, the vector ALUs'
+// conversions (four an instruction of theirs) most of the others. With 8 bits on both sides it takes 230
+// us, with 4 bits 106, 2.6 PFLOP/s, a quarter of it the results' store.
 template <int F>
 struct TileRows {
   static constexpr int BYTES = mx_group_bytes(F), CHUNKS = BYTES / 16, PER_COPY = 64 / CHUNKS;
@@ -507,7 +508,7 @@ struct Plan {
   int slices, chunk;  // groups of a slice
 };
 // Which form runs (us on MI355X, e4m3 activations and e2m1 weights, a synchronous run's 13 us
-// included):
+// included, both sides in turn in short runs; under steady load large layers take up to a tenth less):
 //   * few rows: INLINE up to 128 groups of X a workgroup, with a wave for every four of them
 //     (1x4096x4096 16.6; encoded by a launch of its own 19.6), and for more than 16 rows only while
 //     the groups that all workgroups encode stay few (20x1000x500 15.8 against 18.3, 128x1024x128 14.7

@@ -31,7 +31,7 @@ __device__ __forceinline__ void store4(float* p, int rest, const float (&v)[4]) 
 
 // One group of 128 values for 32 lanes, four values a lane, U groups a lane and round: a block is
 // eight lanes, whose largest magnitude goes round by DPP. Memory bounds it: [8192, 4096] to e2m1 takes
-// 26 us, 152 MB at 5.9 TB/s, and the way back 23 us, 6.6 TB/s; [500, 1021]
+// 25 us, 152 MB at 6.1 TB/s, and the way back 23 us, 6.6 TB/s; [500, 1021]
 // 2.9 us, little more than a launch.
 template <int F, bool KEEP, int U>
 __global__ void __launch_bounds__(256) mx_encode(const float* __restrict__ x, int64_t ldx,
@@ -177,7 +177,8 @@ bool whole_sums(int64_t R, int64_t C) { return R <= 1024 && C <= 1 << 26; }
 
 // Rows a workgroup takes otherwise: 16 (four a wave, all in flight at once) or as many as make 64
 // slabs of rows, whose sums the second launch reads fastest (4096x1000 24.7 us, with 32 / 128 / 256
-// slabs 27.2 / 25.8 / 30.7; 4096x4096 41.5: 26 us for 145 MB are 5.6 TB/s), or 1024 workgroups where
+// slabs 27.2 / 25.8 / 30.7; 4096x4096 41.5, of which the first launch is 26 us for 151 MB, 5.8 TB/s, and
+// 32 us, 4.7 TB/s, in a backward pass between other kernels), or 1024 workgroups where
 // there are few columns and the slabs so many that their sums are folded in two launches (8192x200
 // 20.5 against 26.0).
 int64_t act_grad_rows(int64_t R, int64_t C) {
