@@ -43,7 +43,8 @@ int main() {
     for (int64_t M : extents)
       for (int64_t N : extents)
         if (check_pack(M, N, K)) return 1;
-  for (int64_t N : {(int64_t)1, (int64_t)65, (1ll << 29) + 1, (1ll << 30) - 64, (1ll << 30) - 63, (1ll << 31) - 257, 1ll << 34})
+  const int64_t widths[] = {1, 65, (1ll << 29) + 1, (1ll << 30) - 64, (1ll << 30) - 63, (1ll << 31) - 257, 1ll << 34};
+  for (int64_t N : widths)
     if (check_colsum(N)) return 1;
   // from here on one launch does not do
   if (colsum_groups((1ll << 30) - 63) * COLSUM_THREADS <= LAUNCH_THREADS) return fail("wide", 1ll << 30, 0, 0);
