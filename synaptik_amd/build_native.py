@@ -22,7 +22,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # the per-layout GEMM units are the slowest to compile and go first
 SOURCES = ["gemm_nn.hip", "gemm_nt.hip", "gemm_tn.hip", "gemm_tt.hip", "gemm.hip", "gemm_skinny.hip",
            "elementwise.hip", "softmax_loss.hip", "index_ce.hip", "ce_head.hip", "optim.hip", "publish.hip",
-           "mx_store.hip", "mx_gemm.hip", "mx_linear.hip", "runtime.cpp", "lxm.cpp"]
+           "mx_store.hip", "mx_gemm.hip", "mx_linear.hip", "embed.hip", "layer_norm.hip",
+           "gated_scan.hip", "distill.hip", "runtime.cpp", "lxm.cpp"]
 
 COMMON_FLAGS = [
     "--offload-arch=gfx950",

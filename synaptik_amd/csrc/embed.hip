@@ -1,0 +1,572 @@
+// Rows of a table by token, and the table's gradient.
+//
+//   Y[n, :]  = scale * W[t_n, :]                         (zero where t_n is the padding token)
+//   dW[v, :] = scale * sum over n with t_n = v of dY[n, :]
+//
+// A token outside the table flags DEV_INDEX_OUT_OF_BOUNDS; its row of Y is zero and it adds nothing
+// to dW. Bound: both move each row once.
+//
+// The gradient's order of summation is fixed: the rows' ordinals are sorted by token (stable, by
+// digits of EG_BITS bits), the sorted list is cut every EG_TILE rows wherever a token's rows begin
+// or end, a wave sums a piece's rows in ascending order in binary64, and a token whose rows lie
+// in several pieces gets its parts added in ascending order. So a frequent token costs no more than
+// as many rows of different ones, nothing is added by atomics, and results do not depend on what
+// runs when.
+#include <algorithm>
+
+#include "common.h"
+#include "kernels.h"
+#include "row4.h"
+
+namespace shk {
+namespace {
+
+// The token of row n as a table row, or V where there is none (padding, out of bounds).
+struct Tokens {
+  const void* t;
+  int64_t N, V, pad;
+  int is64, has_pad;
+  uint32_t* status;
+  __device__ __forceinline__ uint32_t key(int64_t n, bool flag) const {
+    const int64_t v = is64 ? static_cast<const int64_t*>(t)[n] : (int64_t) static_cast<const int32_t*>(t)[n];
+    if (has_pad && v == pad) return (uint32_t)V;
+    if (v >= 0 && v < V) return (uint32_t)v;
+    if (flag) atomicOr(status, (uint32_t)DEV_INDEX_OUT_OF_BOUNDS);
+    return (uint32_t)V;
+  }
+};
+
+// ---- lookup: L lanes a row, each four columns of every 4 L, U rows at once ----
+template <int L, int U>
+__global__ void __launch_bounds__(256) embed_rows(Tokens t, const float* __restrict__ w, float* __restrict__ y,
+                                                  int64_t D, int64_t ldy, float scale) {
+  constexpr int TEAMS = 256 / L;
+  const int lane = threadIdx.x % L;
+  const int64_t first = ((int64_t)blockIdx.y * L + lane) * 4, step = (int64_t)gridDim.y * L * 4;
+  for (int64_t base = (int64_t)blockIdx.x * (TEAMS * U) + threadIdx.x / L; base < t.N;
+       base += (int64_t)gridDim.x * (TEAMS * U)) {
+    uint32_t key[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t n = base + u * TEAMS;
+      key[u] = n < t.N ? t.key(n, first == 0) : (uint32_t)t.V;
+    }
+    for (int64_t c = first; c < D; c += step) {
+      float4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        v[u] = key[u] < (uint32_t)t.V ? ld4(w + key[u] * D + c, D - c) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t n = base + u * TEAMS;
+        if (n < t.N)
+          st4<true>(y + n * ldy + c, D - c,
+                    make_float4(v[u].x * scale, v[u].y * scale, v[u].z * scale, v[u].w * scale));
+      }
+    }
+  }
+}
+
+template <int L, int U>
+void launch_rows(const Tokens& t, const float* w, float* y, int64_t D, int64_t ldy, float scale, hipStream_t s) {
+  const int64_t rows = 256 / L * U;
+  const unsigned gx = (unsigned)std::min<int64_t>((t.N + rows - 1) / rows, 1 << 18);
+  const unsigned gy = (unsigned)std::min<int64_t>((D + 4 * L - 1) / (4 * L), 1 << 6);
+  hipLaunchKernelGGL((embed_rows<L, U>), dim3(gx, gy), dim3(256), 0, s, t, w, y, D, ldy, scale);
+}
+
+// ---- sorting ----
+constexpr int EG_BITS = 9, EG_BINS = 1 << EG_BITS;
+constexpr int EG_KEYS = 16;                    // keys a thread
+constexpr int EG_SORT = 256 * EG_KEYS;         // keys a workgroup
+constexpr int64_t EG_SCAN_TILES = 64;          // up to here a workgroup adds the others' counts itself
+constexpr int EG_SMALL_KEYS = 4, EG_SMALL = 1024 * EG_SMALL_KEYS;  // keys that one workgroup sorts
+constexpr int EG_TILE = 32;                    // sorted rows a wave sums
+
+// Among the wave's active lanes: those whose digit is this lane's.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool active) {
+  uint64_t mask = __ballot(active);
+#pragma unroll
+  for (int b = 0; b < EG_BITS; ++b) {
+    const uint64_t set = __ballot((digit >> b) & 1);
+    mask &= ((digit >> b) & 1) ? set : ~set;
+  }
+  return mask;
+}
+
+// Rank of each of a wave's keys among its wave's keys of the same digit, K rounds of 64 keys in
+// order; count: the wave's EG_BINS counters in LDS, zero before, the digits' counts after.
+template <int K>
+__device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[K], const bool (&active)[K],
+                                           uint32_t* count, uint32_t (&rank)[K]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const uint64_t same = same_digit(digit[i], active[i]);
+    const int before = __popcll(same & ((1ull << lane) - 1));
+    uint32_t old = 0;
+    if (active[i] && before == 0) old = atomicAdd(&count[digit[i]], (uint32_t)__popcll(same));
+    rank[i] = __shfl(old, active[i] ? __ffsll((unsigned long long)same) - 1 : lane, 64) + before;
+  }
+}
+
+// Exclusive prefix sums of EG_BINS values in LDS, by NT >= EG_BINS / 2 threads.
+template <int NT>
+__device__ __forceinline__ void scan_bins(uint32_t* v, uint32_t* wave_sum_lds) {
+  constexpr int T = EG_BINS / 2;  // threads that take part: two bins each
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  uint32_t a = 0, b = 0, x = 0;
+  if (threadIdx.x < T) {
+    a = v[2 * threadIdx.x];
+    b = v[2 * threadIdx.x + 1];
+    x = a + b;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t up = __shfl_up(x, o, 64);
+      if (lane >= o) x += up;
+    }
+    if (lane == 63) wave_sum_lds[w] = x;
+  }
+  __syncthreads();
+  if (threadIdx.x < T) {
+    uint32_t base = x - a - b;
+    for (int i = 0; i < w; ++i) base += wave_sum_lds[i];
+    v[2 * threadIdx.x] = base;
+    v[2 * threadIdx.x + 1] = base + a;
+  }
+  __syncthreads();
+}
+
+// Sorted keys and row ordinals of up to EG_SMALL rows in one launch.
+__global__ void __launch_bounds__(1024) eg_sort_small(Tokens t, int passes, uint32_t* __restrict__ keys,
+                                                      uint32_t* __restrict__ rows) {
+  constexpr int K = EG_SMALL_KEYS, NW = 16;
+  __shared__ uint32_t count[NW][EG_BINS];
+  __shared__ uint32_t base[EG_BINS];
+  __shared__ uint32_t sums[EG_BINS / 128];
+  __shared__ uint32_t lk[EG_SMALL];
+  __shared__ uint16_t lr[EG_SMALL];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int N = (int)t.N;
+  uint32_t key[K];
+  uint16_t row[K];
+  bool active[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int n = w * 64 * K + i * 64 + lane;
+    active[i] = n < N;
+    key[i] = active[i] ? t.key(n, true) : 0u;
+    row[i] = (uint16_t)n;
+  }
+  for (int p = 0; p < passes; ++p) {
+    uint32_t digit[K], rank[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) digit[i] = (key[i] >> (p * EG_BITS)) & (EG_BINS - 1);
+    for (int i = threadIdx.x; i < NW * EG_BINS; i += 1024) (&count[0][0])[i] = 0;
+    __syncthreads();
+    wave_ranks<K>(digit, active, count[w], rank);
+    __syncthreads();
+    if (threadIdx.x < EG_BINS) {
+      uint32_t sum = 0;
+      for (int i = 0; i < NW; ++i) {
+        const uint32_t c = count[i][threadIdx.x];
+        count[i][threadIdx.x] = sum;
+        sum += c;
+      }
+      base[threadIdx.x] = sum;
+    }
+    __syncthreads();
+    scan_bins<1024>(base, sums);
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      if (active[i]) {
+        const uint32_t to = base[digit[i]] + count[w][digit[i]] + rank[i];
+        lk[to] = key[i];
+        lr[to] = row[i];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int n = w * 64 * K + i * 64 + lane;
+      if (active[i]) {
+        key[i] = lk[n];
+        row[i] = lr[n];
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int n = w * 64 * K + i * 64 + lane;
+    if (active[i]) {
+      keys[n] = key[i];
+      rows[n] = row[i];
+    }
+  }
+}
+
+// Digit counts of each EG_SORT keys: count[tile][bin]. The first pass reads the tokens.
+__global__ void __launch_bounds__(256) eg_count(Tokens t, const uint32_t* __restrict__ keys, int shift,
+                                                uint32_t* __restrict__ count) {
+  __shared__ uint32_t h[4][EG_BINS];
+  for (int i = threadIdx.x; i < 4 * EG_BINS; i += 256) (&h[0][0])[i] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * EG_SORT;
+#pragma unroll 4
+  for (int i = 0; i < EG_KEYS; ++i) {
+    const int64_t n = first + i * 256 + threadIdx.x;
+    if (n < t.N) {
+      const uint32_t key = keys != nullptr ? keys[n] : t.key(n, true);
+      atomicAdd(&h[threadIdx.x >> 6][(key >> shift) & (EG_BINS - 1)], 1u);
+    }
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < EG_BINS; b += 256)
+    count[(int64_t)blockIdx.x * EG_BINS + b] = (h[0][b] + h[1][b]) + (h[2][b] + h[3][b]);
+}
+
+// count[tile][bin] becomes the sum of the bin's counts in the tiles before; row `tiles` the bin's
+// whole count. One workgroup for 64 bins, four parts of the tiles.
+__global__ void __launch_bounds__(256) eg_scan(uint32_t* __restrict__ count, int64_t tiles) {
+  __shared__ uint32_t sum[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t part = (tiles + 3) / 4, lo = min(tiles, w * part), hi = min(tiles, lo + part);
+  uint32_t* c = count + blockIdx.x * 64 + lane;
+  uint32_t s = 0;
+  for (int64_t i = lo; i < hi; ++i) s += c[i * EG_BINS];
+  sum[w][lane] = s;
+  __syncthreads();
+  uint32_t run = 0;
+  for (int i = 0; i < w; ++i) run += sum[i][lane];
+  for (int64_t i = lo; i < hi; ++i) {
+    const uint32_t v = c[i * EG_BINS];
+    c[i * EG_BINS] = run;
+    run += v;
+  }
+  if (w == 3) c[tiles * EG_BINS] = run;
+}
+
+// Moves each key and its row to its place by one digit.
+__global__ void __launch_bounds__(256) eg_scatter(Tokens t, const uint32_t* __restrict__ keys,
+                                                  const uint32_t* __restrict__ rows, int shift,
+                                                  const uint32_t* __restrict__ count, int64_t tiles,
+                                                  uint32_t* __restrict__ keys_out, uint32_t* __restrict__ rows_out) {
+  constexpr int K = EG_KEYS;
+  __shared__ uint32_t h[4][EG_BINS];
+  __shared__ uint32_t base[EG_BINS], before[EG_BINS];
+  __shared__ uint32_t sums[EG_BINS / 128];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t first = (int64_t)blockIdx.x * EG_SORT + w * 64 * K + lane;
+  uint32_t key[K], digit[K], rank[K];
+  bool active[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int64_t n = first + i * 64;
+    active[i] = n < t.N;
+    key[i] = !active[i] ? 0u : keys != nullptr ? keys[n] : t.key(n, false);
+    digit[i] = (key[i] >> shift) & (EG_BINS - 1);
+  }
+  for (int i = threadIdx.x; i < 4 * EG_BINS; i += 256) (&h[0][0])[i] = 0;
+  if (tiles <= EG_SCAN_TILES) {
+    uint32_t all[2] = {0, 0}, mine[2] = {0, 0};
+#pragma unroll 8
+    for (int64_t i = 0; i < tiles; ++i) {
+      const uint32_t* c = count + i * EG_BINS + threadIdx.x;
+      const uint32_t a = c[0], b = c[256];
+      all[0] += a;
+      all[1] += b;
+      mine[0] += i < blockIdx.x ? a : 0u;
+      mine[1] += i < blockIdx.x ? b : 0u;
+    }
+    for (int j = 0; j < 2; ++j) {
+      base[threadIdx.x + 256 * j] = all[j];
+      before[threadIdx.x + 256 * j] = mine[j];
+    }
+  } else {
+    for (int b = threadIdx.x; b < EG_BINS; b += 256) {
+      base[b] = count[tiles * EG_BINS + b];
+      before[b] = count[(int64_t)blockIdx.x * EG_BINS + b];
+    }
+  }
+  __syncthreads();
+  scan_bins<256>(base, sums);
+  wave_ranks<K>(digit, active, h[w], rank);
+  __syncthreads();
+  for (int b = threadIdx.x; b < EG_BINS; b += 256) {
+    uint32_t run = base[b] + before[b];
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = h[i][b];
+      h[i][b] = run;
+      run += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    if (active[i]) {
+      const uint32_t to = h[w][digit[i]] + rank[i];
+      keys_out[to] = key[i];
+      rows_out[to] = rows != nullptr ? rows[first + i * 64] : (uint32_t)(first + i * 64);
+    }
+  }
+}
+
+// ---- sums ----
+struct SumArgs {
+  const float* dy;
+  const uint32_t* keys;  // sorted
+  const uint32_t* rows;  // the row of dY of each
+  float* dw;
+  double* part;          // [tiles][2][D]: a piece that begins before its tile, one that ends behind it
+  int64_t N, V, D, ldy, tiles, segments;  // segments of 256 columns
+  double scale;
+  int accumulate;
+};
+
+__device__ __forceinline__ void eg_result(const SumArgs& a, uint32_t key, int64_t c, const double (&acc)[4]) {
+  float* p = a.dw + key * a.D + c;
+  float4 o = make_float4((float)(acc[0] * a.scale), (float)(acc[1] * a.scale), (float)(acc[2] * a.scale),
+                         (float)(acc[3] * a.scale));
+  if (a.accumulate) {
+    const float4 old = ld4(p, a.D - c);
+    o = make_float4(old.x + o.x, old.y + o.y, old.z + o.z, old.w + o.w);
+  }
+  st4<true>(p, a.D - c, o);
+}
+
+// A wave's part: rows [first, last) of the sorted list, 256 columns from c0 on.
+__device__ __forceinline__ void eg_sum_tile(const SumArgs& a, int64_t tile, int64_t segment) {
+  const int lane = threadIdx.x & 63;
+  const int64_t first = tile * EG_TILE, count = min((int64_t)EG_TILE, a.N - first);
+  const int64_t c = segment * 256 + 4 * lane;
+  // the keys from the one before the tile to the one behind it, one a lane
+  const int64_t at = first - 1 + lane;
+  const uint32_t none = (uint32_t)a.V;
+  const uint32_t key_l = lane < EG_TILE + 2 && at >= 0 && at < a.N ? a.keys[at] : none;
+  const uint32_t row_l = lane < EG_TILE && first + lane < a.N ? a.rows[first + lane] : 0u;
+  auto key_of = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)key_l, i + 1); };
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  bool open = first > 0 && key_of(0) == key_of(-1);  // the piece began before this tile
+  constexpr int U = 8;
+  for (int i0 = 0; i0 < (int)count; i0 += U) {
+    float4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u, (int)count - 1);
+      const uint32_t row = (uint32_t)__builtin_amdgcn_readlane((int)row_l, i);
+      v[u] = key_of(i) < none ? ld4<true>(a.dy + row * a.ldy + c, a.D - c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      if (i >= (int)count) break;
+      const uint32_t key = key_of(i);
+      if (key >= none) return;  // (sorted last)
+      acc[0] += (double)v[u].x;
+      acc[1] += (double)v[u].y;
+      acc[2] += (double)v[u].z;
+      acc[3] += (double)v[u].w;
+      const bool ends = i + 1 < (int)count && key_of(i + 1) != key;
+      if (!ends && i + 1 < (int)count) continue;
+      // the piece's end: a token's last row, or the tile's
+      const bool goes_on = !ends && first + count < a.N && key_of((int)count) == key;
+      if (!open && !goes_on) {
+        eg_result(a, key, c, acc);
+      } else {
+        double* p = a.part + ((2 * tile + (open ? 0 : 1)) * a.D + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < a.D) p[j] = acc[j];
+      }
+      open = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = 0.0;
+    }
+  }
+}
+
+// Zeros in the rows of `EG_FILL` table rows from v0 on that no token names.
+constexpr int EG_FILL = 16;
+__device__ __forceinline__ void eg_fill_rows(const SumArgs& a, int64_t v0) {
+  const int lane = threadIdx.x & 63;
+  const int64_t v = v0 + (lane % EG_FILL);
+  // the first of the sorted keys that is not below v
+  int64_t lo = 0, hi = a.N;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (a.keys[mid] < v) lo = mid + 1;
+    else hi = mid;
+  }
+  const bool absent = v < a.V && !(lo < a.N && a.keys[lo] == v);
+  uint32_t todo = (uint32_t)__ballot(absent) & ((1u << EG_FILL) - 1);
+  while (todo != 0) {
+    const int j = __ffs(todo) - 1;
+    todo &= todo - 1;
+    float* row = a.dw + (v0 + j) * a.D;
+    for (int64_t c = 4 * lane; c < a.D; c += 256) st4<true>(row + c, a.D - c, make_float4(0.f, 0.f, 0.f, 0.f));
+  }
+}
+
+__global__ void __launch_bounds__(256) eg_sum(SumArgs a, int64_t sum_groups) {
+  const int w = threadIdx.x >> 6;
+  if (blockIdx.x < sum_groups) {
+    const int64_t units = a.tiles * a.segments;
+    for (int64_t u = (int64_t)blockIdx.x * 4 + w; u < units; u += sum_groups * 4)
+      eg_sum_tile(a, u / a.segments, u % a.segments);
+    return;
+  }
+  const int64_t waves = ((int64_t)gridDim.x - sum_groups) * 4;
+  for (int64_t v = (((int64_t)blockIdx.x - sum_groups) * 4 + w) * EG_FILL; v < a.V; v += waves * EG_FILL)
+    eg_fill_rows(a, v);
+}
+
+// Adds up the parts of a token whose rows lie in several tiles. One workgroup for the tile in which
+// the token's rows begin and 256 columns; its four waves take consecutive quarters of the tiles
+// behind, whose parts are the first pieces there.
+__global__ void __launch_bounds__(256) eg_join(SumArgs a) {
+  __shared__ double part[4][256];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t units = (a.tiles - 1) * a.segments;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t tile = u / a.segments, c = (u % a.segments) * 256 + 4 * lane;
+    const int64_t end = (tile + 1) * EG_TILE;  // (a tile that another one follows is full)
+    const uint32_t key = a.keys[end - 1];
+    if (key >= a.V || a.keys[end] != key) continue;
+    const int64_t first = tile * EG_TILE;
+    if (first > 0 && a.keys[first - 1] == key) continue;  // began in an earlier tile
+    // tiles whose last key is this token's, which sorted keys have in a row
+    int64_t lo = tile + 1, hi = a.tiles;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (a.keys[min(a.N, (mid + 1) * EG_TILE) - 1] == key) lo = mid + 1;
+      else hi = mid;
+    }
+    // the last tile with a part: lo itself if its first row is the token's
+    const int64_t stop = lo < a.tiles && a.keys[lo * EG_TILE] == key ? lo + 1 : lo;
+    const int64_t n = stop - (tile + 1), quarter = (n + 3) / 4;
+    const int64_t from = tile + 1 + min(n, w * quarter), to = tile + 1 + min(n, (w + 1) * quarter);
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    if (w == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < a.D) acc[j] = a.part[(2 * tile + 1) * a.D + c + j];
+    }
+    for (int64_t i = from; i < to; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < a.D) acc[j] += a.part[2 * i * a.D + c + j];
+    }
+    __syncthreads();  // (the last round's sums have been read)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[w][4 * lane + j] = acc[j];
+    __syncthreads();
+    if (w == 0 && c < a.D) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc[j] = ((part[0][4 * lane + j] + part[1][4 * lane + j]) + part[2][4 * lane + j]) + part[3][4 * lane + j];
+      eg_result(a, key, c, acc);
+    }
+  }
+}
+
+int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// What embed_grad keeps: two lists of keys and rows, digit counts, parts of sums.
+struct Layout {
+  int64_t keys[2], rows[2], count, part, bytes;
+};
+Layout layout(int64_t N, int64_t D) {
+  const int64_t sort = (N + EG_SORT - 1) / EG_SORT, tiles = (N + EG_TILE - 1) / EG_TILE;
+  Layout l{};
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = off;
+    off += round16(bytes);
+    return at;
+  };
+  for (int i = 0; i < 2; ++i) {
+    l.keys[i] = take(4 * N);
+    l.rows[i] = take(4 * N);
+  }
+  l.count = take(4 * (sort + 1) * EG_BINS);
+  l.part = take(tiles > 1 ? 16 * tiles * D : 0);
+  l.bytes = off;
+  return l;
+}
+
+Tokens tokens_of(const EmbedParams& p, uint32_t* status) {
+  return Tokens{p.tokens, p.N, p.V, p.pad, p.is64, p.has_pad, status};
+}
+
+}  // namespace
+
+hipError_t launch_embed(const EmbedParams& p, uint32_t* status, hipStream_t s) {
+  if (p.N <= 0 || p.D <= 0) return hipSuccess;
+  const Tokens t = tokens_of(p, status);
+  // lanes for a row's groups of four; four rows at once where there are enough for every CU
+  const bool many = (double)p.N * (double)p.D >= (double)(1 << 20);
+  auto go = [&](auto lanes) {
+    constexpr int L = decltype(lanes)::value;
+    if (many) launch_rows<L, 4>(t, p.w, p.y, p.D, p.ldy, p.scale, s);
+    else launch_rows<L, 1>(t, p.w, p.y, p.D, p.ldy, p.scale, s);
+  };
+  if (p.D <= 16) go(std::integral_constant<int, 4>());
+  else if (p.D <= 64) go(std::integral_constant<int, 16>());
+  else go(std::integral_constant<int, 64>());
+  return hipGetLastError();
+}
+
+int64_t embed_grad_scratch_bytes(int64_t N, int64_t D) { return layout(N, D).bytes; }
+
+hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* status, hipStream_t s) {
+  if (p.V <= 0 || p.D <= 0 || (p.N <= 0 && p.accumulate)) return hipSuccess;
+  const Tokens t = tokens_of(p, status);
+  const Layout l = layout(p.N, p.D);
+  char* base = static_cast<char*>(scratch);
+  uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(base + l.keys[0]), reinterpret_cast<uint32_t*>(base + l.keys[1])};
+  uint32_t* rows[2] = {reinterpret_cast<uint32_t*>(base + l.rows[0]), reinterpret_cast<uint32_t*>(base + l.rows[1])};
+  uint32_t* count = reinterpret_cast<uint32_t*>(base + l.count);
+  int passes = 1;  // digits of the keys 0 .. V
+  while (passes * EG_BITS < 32 && (p.V >> (passes * EG_BITS)) != 0) ++passes;
+  int at = 0;
+  if (p.N > 0 && p.N <= EG_SMALL) {
+    hipLaunchKernelGGL(eg_sort_small, dim3(1), dim3(1024), 0, s, t, passes, keys[0], rows[0]);
+  } else if (p.N > 0) {
+    const int64_t tiles = (p.N + EG_SORT - 1) / EG_SORT;
+    for (int i = 0; i < passes; ++i) {
+      const uint32_t* ki = i == 0 ? nullptr : keys[at];
+      const uint32_t* ri = i == 0 ? nullptr : rows[at];
+      const int to = i == 0 ? 0 : 1 - at;
+      hipLaunchKernelGGL(eg_count, dim3((unsigned)tiles), dim3(256), 0, s, t, ki, i * EG_BITS, count);
+      if (tiles > EG_SCAN_TILES)
+        hipLaunchKernelGGL(eg_scan, dim3(EG_BINS / 64), dim3(256), 0, s, count, tiles);
+      hipLaunchKernelGGL(eg_scatter, dim3((unsigned)tiles), dim3(256), 0, s, t, ki, ri, i * EG_BITS,
+                         (const uint32_t*)count, tiles, keys[to], rows[to]);
+      at = to;
+    }
+  }
+  SumArgs a{};
+  a.dy = p.w;
+  a.keys = keys[at];
+  a.rows = rows[at];
+  a.dw = p.y;
+  a.part = reinterpret_cast<double*>(base + l.part);
+  a.N = p.N;
+  a.V = p.V;
+  a.D = p.D;
+  a.ldy = p.ldy;
+  a.tiles = (p.N + EG_TILE - 1) / EG_TILE;
+  a.segments = (p.D + 255) / 256;
+  a.scale = (double)p.scale;
+  a.accumulate = p.accumulate;
+  constexpr int64_t MOST = 1 << 20;  // workgroups of either half
+  const int64_t sums = std::min<int64_t>((a.tiles * a.segments + 3) / 4, MOST);
+  const int64_t fills = p.accumulate ? 0 : std::min<int64_t>((p.V + 4 * EG_FILL - 1) / (4 * EG_FILL), MOST);
+  hipLaunchKernelGGL(eg_sum, dim3((unsigned)(sums + fills)), dim3(256), 0, s, a, sums);
+  if (a.tiles > 1)
+    hipLaunchKernelGGL(eg_join, dim3((unsigned)std::min<int64_t>((a.tiles - 1) * a.segments, MOST)), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace shk

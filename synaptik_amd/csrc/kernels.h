@@ -278,6 +278,94 @@ struct MxLinearParams {
 hipError_t launch_mx_linear(const MxLinearParams& p, void* scratch, hipStream_t s);
 int64_t mx_linear_scratch_bytes(int64_t M, int64_t N, int64_t K);
 
+// Rows of a table [V, D] by token (embed.hip): y [N, D] (row stride ldy) = scale * w[token], zero at the
+// padding token. The gradient reads dy in w's place, with row stride ldy, and writes the table's
+// gradient [V, D] to y, or adds to it.
+struct EmbedParams {
+  const float* w;
+  const void* tokens;
+  float* y;
+  int64_t N, V, D, ldy, pad;
+  int is64, has_pad, accumulate;
+  float scale;
+};
+hipError_t launch_embed(const EmbedParams& p, uint32_t* status, hipStream_t s);
+hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* status, hipStream_t s);
+int64_t embed_grad_scratch_bytes(int64_t N, int64_t D);
+
+// Layer norm over the last axis (layer_norm.hip): y [R, C] from x [R, C]; gamma, beta [C] may be null.
+// y may be x with the same row stride.
+struct LayerNormParams {
+  const float* x;
+  const float* gamma;
+  const float* beta;
+  float* y;
+  int64_t R, C, ldx, ldy;
+  float eps;
+};
+hipError_t launch_layer_norm(const LayerNormParams& p, hipStream_t s);
+// dx, and the sums dgamma, dbeta [C] where not null; dx may be dy with the same row stride.
+struct LayerNormGradParams {
+  const float* dy;
+  const float* x;
+  const float* gamma;
+  float* dx;
+  float* dgamma;
+  float* dbeta;
+  int64_t R, C, lddy, ldx, lddx;
+  float eps;
+};
+hipError_t launch_layer_norm_grad(const LayerNormGradParams& p, double* scratch, hipStream_t s);
+int64_t layer_norm_grad_scratch_bytes(int64_t R, int64_t C);
+
+// Gated linear recurrence of sequences [B, T, D] (gated_scan.hip): h from the gates' inputs z, the
+// inputs u and the first states h0 [B, D] (null: zero); last [B, D] (null: not wanted) may be h0.
+struct GatedScanParams {
+  const float* z;
+  const float* u;
+  const float* h0;
+  const void* lengths;  // [B]; null: all T
+  float* h;
+  float* last;
+  int64_t B, T, D;
+  int len64;
+};
+hipError_t launch_gated_scan(const GatedScanParams& p, float* scratch, uint32_t* status, hipStream_t s);
+// Gradients of z, u and h0 from those of h and of the last state (dlast; null: zero); dh0 (null: not
+// wanted) may be dlast.
+struct GatedScanGradParams {
+  const float* dh;
+  const float* z;
+  const float* u;
+  const float* h;
+  const float* h0;
+  const float* dlast;
+  const void* lengths;
+  float* dz;
+  float* du;
+  float* dh0;
+  int64_t B, T, D;
+  int len64;
+};
+hipError_t launch_gated_scan_grad(const GatedScanGradParams& p, float* scratch, uint32_t* status, hipStream_t s);
+int64_t gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D);
+
+// Divergence from a teacher's K largest logits of each row (distill.hip), and its gradient (null: not
+// wanted).
+constexpr int64_t DISTILL_MOST = 1024;  // K
+struct DistillParams {
+  const float* logits;
+  const void* index;
+  const float* teacher;
+  float* loss;
+  float* grad;
+  int64_t R, C, K;
+  int is64;
+  float T, g;
+};
+hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* status, hipStream_t s);
+int64_t distill_scratch_bytes(int64_t R);
+
 // Y[C,R] = X[R,C]^T
 hipError_t launch_transpose(const float* x, float* y, int64_t R, int64_t C, hipStream_t s);
 

@@ -1,0 +1,457 @@
+// Layer norm over the last axis of X [R, C] and its backward pass.
+//
+//   mean = sum x / C, var = sum (x - mean)^2 / C, rstd = 1 / sqrt(var + eps)
+//   y  = (x - mean) rstd gamma + beta                              (gamma, beta optional)
+//   g  = dy gamma,  xh = (x - mean) rstd
+//   dx = rstd (g - sum g / C - xh sum (g xh) / C)
+//   dgamma = sum over rows of dy xh,  dbeta = sum over rows of dy
+//
+// Bound: memory. A row is read once and held in registers through its statistics, and the backward
+// pass forms them again from the x that it reads anyway, so that nothing but x is kept between the
+// two and a mean far from zero is not rounded to binary32 on the way. The mean and the sum of
+// squares about it are binary64, as are all sums. dgamma and dbeta are summed beside dx: each
+// workgroup takes every G-th group of rows, keeps its columns' sums in registers and writes one
+// row of partial sums, which a second launch adds in a fixed order.
+#include <algorithm>
+
+#include "common.h"
+#include "kernels.h"
+#include "row4.h"
+
+namespace shk {
+namespace {
+
+// Sums over the L lanes (a power of two) that hold one row.
+template <int L>
+__device__ __forceinline__ double team_sum(double v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// Sums over a workgroup of NT threads of K values; `lds` is free again after the next barrier.
+template <int NT, int K>
+__device__ __forceinline__ void group_sum(double (&v)[K], double* lds) {
+  constexpr int NW = NT / 64;
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+  if (NW == 1) return;
+  const int w = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) lds[w * K + k] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    double s = lds[k];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) s += lds[i * K + k];
+    v[k] = s;
+  }
+}
+
+// A row in the registers of T threads, V groups of four floats each, T groups apart.
+template <int T, int V>
+struct Row {
+  float4 v[V];
+  __device__ __forceinline__ void load(const float* p, int t, int64_t C) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t c = 4 * (t + (int64_t)i * T);
+      v[i] = ld4<true>(p + c, C - c);
+    }
+  }
+};
+#define LN_EACH(i, j, c, C)                                      \
+  _Pragma("unroll") for (int i = 0; i < V; ++i)                  \
+    _Pragma("unroll") for (int j = 0; j < 4; ++j)                \
+      if (const int64_t c = 4 * (t + (int64_t)i * T) + j; c < (C))
+
+__device__ __forceinline__ float& at(float4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
+__device__ __forceinline__ float at(const float4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
+
+struct FwdArgs {
+  const float* x;
+  const float* gamma;
+  const float* beta;
+  float* y;
+  int64_t R, C, ldx, ldy;
+  double eps;
+};
+
+// T threads a row: a part of a wave (SUM: team_sum), or the whole workgroup.
+template <int NT, int T, int V>
+__global__ void __launch_bounds__(NT) ln_fwd(FwdArgs a) {
+  __shared__ double lds[2][NT / 64];
+  const int t = threadIdx.x % T;
+  Row<T, V> gm, bt;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int64_t c = 4 * (t + (int64_t)i * T);
+    gm.v[i] = a.gamma != nullptr ? ld4(a.gamma + c, a.C - c) : make_float4(1.f, 1.f, 1.f, 1.f);
+    bt.v[i] = a.beta != nullptr ? ld4(a.beta + c, a.C - c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int64_t r = (int64_t)blockIdx.x * (NT / T) + threadIdx.x / T; r < a.R; r += (int64_t)gridDim.x * (NT / T)) {
+    Row<T, V> x;
+    x.load(a.x + r * a.ldx, t, a.C);
+    double s[1] = {0.0};
+    LN_EACH(i, j, c, a.C) s[0] += (double)at(x.v[i], j);
+    if constexpr (T < NT) s[0] = team_sum<T>(s[0]);
+    else group_sum<NT, 1>(s, lds[0]);
+    const double mean = s[0] / (double)a.C;
+    double q[1] = {0.0};
+    LN_EACH(i, j, c, a.C) {
+      const double d = (double)at(x.v[i], j) - mean;
+      q[0] = fma(d, d, q[0]);
+    }
+    if constexpr (T < NT) q[0] = team_sum<T>(q[0]);
+    else group_sum<NT, 1>(q, lds[1]);
+    const double rstd = 1.0 / sqrt(q[0] / (double)a.C + a.eps);
+    float* y = a.y + r * a.ldy;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        at(o, j) = fmaf((float)(((double)at(x.v[i], j) - mean) * rstd), at(gm.v[i], j), at(bt.v[i], j));
+      const int64_t c = 4 * (t + (int64_t)i * T);
+      st4<true>(y + c, a.C - c, o);
+    }
+  }
+}
+
+// Rows too wide for registers: three readings by one workgroup.
+constexpr int LN_WIDE = 1024;
+__device__ __forceinline__ void wide_stats(const float* x, int64_t C, double eps, double (*lds)[LN_WIDE / 64],
+                                           double& mean, double& rstd) {
+  double s[1] = {0.0}, q[1] = {0.0};
+  for (int64_t c = 4 * threadIdx.x; c < C; c += 4 * LN_WIDE) {
+    const float4 v = ld4(x + c, C - c);
+    s[0] += ((double)v.x + (double)v.y) + ((double)v.z + (double)v.w);
+  }
+  group_sum<LN_WIDE, 1>(s, lds[0]);
+  mean = s[0] / (double)C;
+  for (int64_t c = 4 * threadIdx.x; c < C; c += 4 * LN_WIDE) {
+    const float4 v = ld4(x + c, C - c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double d = c + j < C ? (double)at(v, j) - mean : 0.0;
+      q[0] = fma(d, d, q[0]);
+    }
+  }
+  group_sum<LN_WIDE, 1>(q, lds[1]);
+  rstd = 1.0 / sqrt(q[0] / (double)C + eps);
+}
+__global__ void __launch_bounds__(LN_WIDE) ln_fwd_wide(FwdArgs a) {
+  __shared__ double lds[2][LN_WIDE / 64];
+  for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
+    const float* x = a.x + r * a.ldx;
+    double mean, rstd;
+    wide_stats(x, a.C, a.eps, lds, mean, rstd);
+    float* y = a.y + r * a.ldy;
+    for (int64_t c = 4 * threadIdx.x; c < a.C; c += 4 * LN_WIDE) {
+      const float4 v = ld4(x + c, a.C - c);
+      const float4 gm = a.gamma != nullptr ? ld4(a.gamma + c, a.C - c) : make_float4(1.f, 1.f, 1.f, 1.f);
+      const float4 bt = a.beta != nullptr ? ld4(a.beta + c, a.C - c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        at(o, j) = fmaf((float)(((double)at(v, j) - mean) * rstd), at(gm, j), at(bt, j));
+      st4<true>(y + c, a.C - c, o);
+    }
+  }
+}
+
+struct BwdArgs {
+  const float* dy;
+  const float* x;
+  const float* gamma;
+  float* dx;
+  double* part;   // [gridDim.x][2][C]: partial sums of dgamma and dbeta; null: neither is wanted
+  double* stats;  // [R][2]: mean and rstd (wide rows)
+  int64_t R, C, lddy, ldx, lddx;
+  double eps;
+};
+
+// dy and dx may be the same memory: a thread writes the elements that it read.
+template <int NT, int T, int V>
+__global__ void __launch_bounds__(NT) ln_bwd(BwdArgs a) {
+  __shared__ double lds[4][NT / 64];
+  const int t = threadIdx.x % T;
+  Row<T, V> gm;
+  double dg[V][4], db[V][4];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int64_t c = 4 * (t + (int64_t)i * T);
+    gm.v[i] = a.gamma != nullptr ? ld4(a.gamma + c, a.C - c) : make_float4(1.f, 1.f, 1.f, 1.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dg[i][j] = db[i][j] = 0.0;
+  }
+  const int64_t step = (int64_t)gridDim.x * (NT / T);
+  int64_t r = (int64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
+  Row<T, V> x, dy, nx, ndy;
+  if (r < a.R) {
+    nx.load(a.x + r * a.ldx, t, a.C);
+    ndy.load(a.dy + r * a.lddy, t, a.C);
+  }
+  for (; r < a.R; r += step) {
+    x = nx;
+    dy = ndy;
+    if (r + step < a.R) {  // the next row is on its way while this one is summed
+      nx.load(a.x + (r + step) * a.ldx, t, a.C);
+      ndy.load(a.dy + (r + step) * a.lddy, t, a.C);
+    }
+    double s[1] = {0.0};
+    LN_EACH(i, j, c, a.C) s[0] += (double)at(x.v[i], j);
+    if constexpr (T < NT) s[0] = team_sum<T>(s[0]);
+    else group_sum<NT, 1>(s, lds[0]);
+    const double mean = s[0] / (double)a.C;
+    double q[3] = {0.0, 0.0, 0.0};  // sums of d^2, g, g d with d = x - mean
+    LN_EACH(i, j, c, a.C) {
+      const double d = (double)at(x.v[i], j) - mean;
+      const double g = (double)at(dy.v[i], j) * (double)at(gm.v[i], j);
+      q[0] = fma(d, d, q[0]);
+      q[1] += g;
+      q[2] = fma(g, d, q[2]);
+    }
+    if constexpr (T < NT) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) q[k] = team_sum<T>(q[k]);
+    } else {
+      group_sum<NT, 3>(q, lds[1]);
+    }
+    const double rstd = 1.0 / sqrt(q[0] / (double)a.C + a.eps);
+    const double c1 = q[1] / (double)a.C, c2 = rstd * rstd * (q[2] / (double)a.C);
+    float* dx = a.dx + r * a.lddx;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double d = (double)at(x.v[i], j) - mean, v = (double)at(dy.v[i], j);
+        const double g = v * (double)at(gm.v[i], j);
+        at(o, j) = (float)(rstd * (fma(-d, c2, g) - c1));
+        dg[i][j] = fma(v, d * rstd, dg[i][j]);
+        db[i][j] += v;
+      }
+      const int64_t c = 4 * (t + (int64_t)i * T);
+      st4<true>(dx + c, a.C - c, o);
+    }
+  }
+  if (a.part == nullptr) return;
+  double* out = a.part + (int64_t)blockIdx.x * 2 * a.C;
+  if constexpr (T == NT) {
+    LN_EACH(i, j, c, a.C) {
+      out[c] = dg[i][j];
+      out[a.C + c] = db[i][j];
+    }
+  } else {
+    // the rows that a wave holds beside each other, then the four waves one after the other
+    __shared__ double cols[2][4 * T * V];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int o = 32; o >= T; o >>= 1) {
+          dg[i][j] += __shfl_xor(dg[i][j], o, 64);
+          db[i][j] += __shfl_xor(db[i][j], o, 64);
+        }
+    for (int w = 0; w < NT / 64; ++w) {
+      if ((int)(threadIdx.x >> 6) == w && (threadIdx.x & 63) < T) {
+        LN_EACH(i, j, c, a.C) {
+          cols[0][c] = w == 0 ? dg[i][j] : cols[0][c] + dg[i][j];
+          cols[1][c] = w == 0 ? db[i][j] : cols[1][c] + db[i][j];
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < (int)a.C; c += NT) {
+      out[c] = cols[0][c];
+      out[a.C + c] = cols[1][c];
+    }
+  }
+}
+
+__global__ void __launch_bounds__(LN_WIDE) ln_bwd_wide(BwdArgs a) {
+  __shared__ double lds[5][LN_WIDE / 64];
+  for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
+    const float* x = a.x + r * a.ldx;
+    const float* dy = a.dy + r * a.lddy;
+    double mean, rstd;
+    wide_stats(x, a.C, a.eps, lds, mean, rstd);
+    double q[2] = {0.0, 0.0};
+    for (int64_t c = 4 * threadIdx.x; c < a.C; c += 4 * LN_WIDE) {
+      const float4 xv = ld4(x + c, a.C - c), v = ld4(dy + c, a.C - c);
+      const float4 gm = a.gamma != nullptr ? ld4(a.gamma + c, a.C - c) : make_float4(1.f, 1.f, 1.f, 1.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (c + j >= a.C) break;
+        const double g = (double)at(v, j) * (double)at(gm, j);
+        q[0] += g;
+        q[1] = fma(g, (double)at(xv, j) - mean, q[1]);
+      }
+    }
+    group_sum<LN_WIDE, 2>(q, lds[2]);
+    const double c1 = q[0] / (double)a.C, c2 = rstd * rstd * (q[1] / (double)a.C);
+    float* dx = a.dx + r * a.lddx;
+    for (int64_t c = 4 * threadIdx.x; c < a.C; c += 4 * LN_WIDE) {
+      const float4 xv = ld4(x + c, a.C - c), v = ld4(dy + c, a.C - c);
+      const float4 gm = a.gamma != nullptr ? ld4(a.gamma + c, a.C - c) : make_float4(1.f, 1.f, 1.f, 1.f);
+      float4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double g = (double)at(v, j) * (double)at(gm, j);
+        at(o, j) = (float)(rstd * (fma(-((double)at(xv, j) - mean), c2, g) - c1));
+      }
+      st4<true>(dx + c, a.C - c, o);
+    }
+  }
+}
+
+// Mean and rstd of every row.
+__global__ void __launch_bounds__(LN_WIDE) ln_stats_wide(BwdArgs a) {
+  __shared__ double lds[2][LN_WIDE / 64];
+  for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
+    double mean, rstd;
+    wide_stats(a.x + r * a.ldx, a.C, a.eps, lds, mean, rstd);
+    if (threadIdx.x == 0) {
+      a.stats[2 * r] = mean;
+      a.stats[2 * r + 1] = rstd;
+    }
+  }
+}
+// Partial column sums of wide rows from their statistics: 256 columns, every gridDim.y-th row.
+__global__ void __launch_bounds__(256) ln_cols_wide(BwdArgs a) {
+  for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < a.C; c += (int64_t)gridDim.x * 256) {
+    double dg = 0.0, db = 0.0;
+    for (int64_t r = blockIdx.y; r < a.R; r += gridDim.y) {
+      const double v = (double)a.dy[r * a.lddy + c];
+      dg = fma(v, ((double)a.x[r * a.ldx + c] - a.stats[2 * r]) * a.stats[2 * r + 1], dg);
+      db += v;
+    }
+    double* out = a.part + (int64_t)blockIdx.y * 2 * a.C;
+    out[c] = dg;
+    out[a.C + c] = db;
+  }
+}
+
+// Adds P rows of partial sums: 32 columns by 16 parts of the rows.
+__global__ void __launch_bounds__(512) ln_finish(const double* __restrict__ part, int64_t P, int64_t C,
+                                                 float* dgamma, float* dbeta) {
+  __shared__ double sum[16][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  for (int64_t base = (int64_t)blockIdx.x * 32; base < 2 * C; base += (int64_t)gridDim.x * 32) {
+    const int64_t c = base + x;
+    double s = 0.0;
+    if (c < 2 * C) {
+#pragma unroll 4
+      for (int64_t p = y; p < P; p += 16) s += part[p * 2 * C + c];
+    }
+    sum[y][x] = s;
+    __syncthreads();
+    if (y == 0 && c < 2 * C) {
+      double all = sum[0][x];
+      for (int i = 1; i < 16; ++i) all += sum[i][x];
+      float* out = c < C ? dgamma : dbeta;
+      if (out != nullptr) out[c < C ? c : c - C] = (float)all;
+    }
+    __syncthreads();
+  }
+}
+
+constexpr int64_t LN_REGS = 16384;  // columns up to which a row is held in registers
+
+// Rows that a workgroup of the backward pass takes at once, and the workgroups.
+struct BwdShape {
+  int64_t rows, groups;
+};
+BwdShape bwd_shape(int64_t R, int64_t C) {
+  BwdShape b{};
+  if (C > LN_REGS) {
+    b.rows = 1;
+    b.groups = std::min<int64_t>(R, 64);
+  } else if (C > 1024) {
+    b.rows = 1;
+    b.groups = std::min<int64_t>(R, 512);
+  } else {
+    int64_t lanes = 2;
+    while (lanes < 64 && 4 * lanes < C) lanes *= 2;
+    b.rows = 256 / lanes;
+    b.groups = std::min<int64_t>((R + b.rows - 1) / b.rows, 1024);
+  }
+  return b;
+}
+
+template <int NT, int T, int V>
+void launch_fwd(const FwdArgs& a, hipStream_t s) {
+  const int64_t rows = NT / T;
+  const unsigned g = (unsigned)std::min<int64_t>((a.R + rows - 1) / rows, 1 << 16);
+  hipLaunchKernelGGL((ln_fwd<NT, T, V>), dim3(g), dim3(NT), 0, s, a);
+}
+
+}  // namespace
+
+hipError_t launch_layer_norm(const LayerNormParams& p, hipStream_t s) {
+  if (p.R <= 0 || p.C <= 0) return hipSuccess;
+  const FwdArgs a{p.x, p.gamma, p.beta, p.y, p.R, p.C, p.ldx, p.ldy, (double)p.eps};
+  if (p.C <= 8) launch_fwd<256, 2, 1>(a, s);
+  else if (p.C <= 16) launch_fwd<256, 4, 1>(a, s);
+  else if (p.C <= 32) launch_fwd<256, 8, 1>(a, s);
+  else if (p.C <= 64) launch_fwd<256, 16, 1>(a, s);
+  else if (p.C <= 128) launch_fwd<256, 32, 1>(a, s);
+  else if (p.C <= 256) launch_fwd<256, 64, 1>(a, s);
+  else if (p.C <= 512) launch_fwd<256, 64, 2>(a, s);
+  else if (p.C <= 1024) launch_fwd<256, 64, 4>(a, s);
+  else if (p.C <= 2048) launch_fwd<256, 256, 2>(a, s);
+  else if (p.C <= 4096) launch_fwd<256, 256, 4>(a, s);
+  else if (p.C <= 8192) launch_fwd<512, 512, 4>(a, s);
+  else if (p.C <= LN_REGS) launch_fwd<1024, 1024, 4>(a, s);
+  else
+    hipLaunchKernelGGL(ln_fwd_wide, dim3((unsigned)std::min<int64_t>(p.R, 1 << 16)), dim3(LN_WIDE), 0, s, a);
+  return hipGetLastError();
+}
+
+int64_t layer_norm_grad_scratch_bytes(int64_t R, int64_t C) {
+  if (R <= 0 || C <= 0) return 0;
+  return bwd_shape(R, C).groups * 16 * C + (C > LN_REGS ? 16 * R : 0);
+}
+
+hipError_t launch_layer_norm_grad(const LayerNormGradParams& p, double* scratch, hipStream_t s) {
+  if (p.C <= 0) return hipSuccess;
+  const bool sums = p.dgamma != nullptr || p.dbeta != nullptr;
+  const BwdShape b = bwd_shape(p.R, p.C);
+  BwdArgs a{p.dy, p.x, p.gamma, p.dx, sums ? scratch : nullptr, scratch + b.groups * 2 * p.C, p.R, p.C,
+            p.lddy, p.ldx, p.lddx, (double)p.eps};
+  if (p.R > 0) {
+    const dim3 g((unsigned)b.groups);
+    if (p.C <= 8) hipLaunchKernelGGL((ln_bwd<256, 2, 1>), g, dim3(256), 0, s, a);
+    else if (p.C <= 16) hipLaunchKernelGGL((ln_bwd<256, 4, 1>), g, dim3(256), 0, s, a);
+    else if (p.C <= 32) hipLaunchKernelGGL((ln_bwd<256, 8, 1>), g, dim3(256), 0, s, a);
+    else if (p.C <= 64) hipLaunchKernelGGL((ln_bwd<256, 16, 1>), g, dim3(256), 0, s, a);
+    else if (p.C <= 128) hipLaunchKernelGGL((ln_bwd<256, 32, 1>), g, dim3(256), 0, s, a);
+    else if (p.C <= 256) hipLaunchKernelGGL((ln_bwd<256, 64, 1>), g, dim3(256), 0, s, a);
+    else if (p.C <= 512) hipLaunchKernelGGL((ln_bwd<256, 64, 2>), g, dim3(256), 0, s, a);
+    else if (p.C <= 1024) hipLaunchKernelGGL((ln_bwd<256, 64, 4>), g, dim3(256), 0, s, a);
+    else if (p.C <= 2048) hipLaunchKernelGGL((ln_bwd<256, 256, 2>), g, dim3(256), 0, s, a);
+    else if (p.C <= 4096) hipLaunchKernelGGL((ln_bwd<512, 512, 2>), g, dim3(512), 0, s, a);
+    else if (p.C <= 8192) hipLaunchKernelGGL((ln_bwd<1024, 1024, 2>), g, dim3(1024), 0, s, a);
+    else if (p.C <= LN_REGS) hipLaunchKernelGGL((ln_bwd<1024, 1024, 4>), g, dim3(1024), 0, s, a);
+    else {
+      const dim3 rows((unsigned)std::min<int64_t>(p.R, 1 << 16));
+      if (sums) {
+        // (before dx, which may take dy's place)
+        hipLaunchKernelGGL(ln_stats_wide, rows, dim3(LN_WIDE), 0, s, a);
+        hipLaunchKernelGGL(ln_cols_wide, dim3((unsigned)std::min<int64_t>((p.C + 255) / 256, 1 << 16), (unsigned)b.groups),
+                           dim3(256), 0, s, a);
+      }
+      hipLaunchKernelGGL(ln_bwd_wide, rows, dim3(LN_WIDE), 0, s, a);
+    }
+  }
+  if (sums)
+    hipLaunchKernelGGL(ln_finish, dim3((unsigned)std::min<int64_t>((2 * p.C + 31) / 32, 1 << 20)), dim3(512), 0, s,
+                       (const double*)scratch, p.R > 0 ? b.groups : 0, p.C, p.dgamma, p.dbeta);
+  return hipGetLastError();
+}
+
+}  // namespace shk

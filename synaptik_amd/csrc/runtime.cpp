@@ -15,10 +15,12 @@
 #include <atomic>
 #include <cstdlib>
 #include <map>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <condition_variable>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <string>
@@ -189,6 +191,13 @@ enum Opcode : uint32_t {
   OP_MX_ACT_GRAD = 19,
   OP_MX_GEMM = 20,
   OP_MX_LINEAR = 21,
+  OP_EMBED = 22,
+  OP_EMBED_GRAD = 23,
+  OP_LAYER_NORM = 24,
+  OP_LAYER_NORM_GRAD = 25,
+  OP_GATED_SCAN = 26,
+  OP_GATED_SCAN_GRAD = 27,
+  OP_DISTILL = 28,
 };
 
 #pragma pack(push, 1)
@@ -209,6 +218,10 @@ struct OptEntry {
   int32_t p, g, m, v;
   int32_t pn, mn, vn, pad;
   int64_t n;
+};
+// Slots of a gated recurrence's backward step beyond the step's eight (payload).
+struct ScanEntry {
+  int32_t dh0, lengths;
 };
 #pragma pack(pop)
 static_assert(sizeof(SlotRecord) == 24, "slot record layout");
@@ -540,6 +553,154 @@ int32_t validate_mx_step(Validator& v, size_t idx, const Step& st, uint64_t* scr
   }
 }
 
+// Embeddings, layer norm, gated recurrences and distillation.
+int32_t validate_token_step(Validator& v, size_t idx, const Step& st, uint64_t* scratch_doubles) {
+  const StepRecord& r = st.rec;
+  const int32_t* s = r.slot;
+  const int64_t* a = r.iarg;
+  auto need = [&](int64_t bytes) {
+    *scratch_doubles = std::max<uint64_t>(*scratch_doubles, (uint64_t)(bytes + 7) / 8);
+  };
+  auto bad_shape = [&](const char* what) {
+    return fail(SHK_HIP_STATUS_UNSUPPORTED_SHAPE, "step %zu: invalid %s", idx, what);
+  };
+  auto aliases = [&](const char* what) {
+    return fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED, "step %zu: %s aliases another operand", idx, what);
+  };
+  auto flag_ok = [](int64_t f) { return f == 0 || f == 1; };
+  auto extent_ok = [](int64_t n) { return n >= 0 && n <= INT32_MAX; };
+  auto ld_ok = [](int64_t R, int64_t C, int64_t ld) { return R <= 0 || C <= 0 || ld >= C; };
+  // slot `w` is none of `others`, absent ones aside
+  auto apart = [](int32_t w, std::initializer_list<int32_t> others) {
+    for (int32_t o : others)
+      if (w >= 0 && w == o) return false;
+    return true;
+  };
+  if (r.opcode != OP_GATED_SCAN_GRAD && !st.payload.empty())
+    return fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED, "step %zu: takes no payload", idx);
+  switch (r.opcode) {
+    case OP_EMBED: case OP_EMBED_GRAD: {
+      const bool grad = r.opcode == OP_EMBED_GRAD;
+      const int64_t N = a[0], V = a[1], D = a[2], ldy = a[3], is64 = a[4];
+      if (!extent_ok(N) || !extent_ok(V) || !extent_ok(D) || !ld_ok(N, D, ldy) || !flag_ok(is64) || !flag_ok(a[5]) ||
+          (grad && !flag_ok(a[7])))
+        return bad_shape("embedding");
+      const char* row = grad ? "dY" : "Y";
+      const char* table = grad ? "dW" : "W";
+      const int32_t rows = grad ? s[0] : s[2], tab = grad ? s[2] : s[0];
+      if (!v.slot_ok(s[0], false, grad ? row : table) || !v.slot_ok(s[1], false, "tokens") ||
+          !v.slot_ok(s[2], false, grad ? table : row) || !v.holds(rows, span(N, D, ldy), DT_F32, row) ||
+          !v.holds(s[1], N, is64 ? DT_I64 : DT_I32, "tokens") || !v.holds(tab, prod(V, D), DT_F32, table) ||
+          !v.writable(s[2], grad ? table : row))
+        return v.err;
+      if (!apart(s[2], {s[0], s[1]})) return aliases(grad ? table : row);
+      if (grad) {
+        // (16 bytes for each column of every 32nd row at most, far below 2^63 with N rows of D held above)
+        need(shk::embed_grad_scratch_bytes(N, D));
+      }
+      return SHK_HIP_STATUS_OK;
+    }
+    case OP_LAYER_NORM: {
+      const int64_t R = a[0], C = a[1], ldx = a[2], ldy = a[3];
+      if (!extent_ok(R) || !extent_ok(C) || !ld_ok(R, C, ldx) || !ld_ok(R, C, ldy) || !(r.farg[0] >= 0.0f) ||
+          !std::isfinite(r.farg[0]))
+        return bad_shape("layer norm");
+      if (!v.slot_ok(s[0], false, "X") || !v.slot_ok(s[1], true, "gamma") || !v.slot_ok(s[2], true, "beta") ||
+          !v.slot_ok(s[3], false, "Y") || !v.holds(s[0], span(R, C, ldx), DT_F32, "X") ||
+          !v.holds(s[1], C, DT_F32, "gamma") || !v.holds(s[2], C, DT_F32, "beta") ||
+          !v.holds(s[3], span(R, C, ldy), DT_F32, "Y") || !v.writable(s[3], "Y"))
+        return v.err;
+      // Y may replace X row by row
+      if (!apart(s[3], {s[1], s[2]}) || (s[3] == s[0] && ldx != ldy)) return aliases("Y");
+      return SHK_HIP_STATUS_OK;
+    }
+    case OP_LAYER_NORM_GRAD: {
+      const int64_t R = a[0], C = a[1], lddy = a[2], ldx = a[3], lddx = a[4];
+      if (!extent_ok(R) || !extent_ok(C) || !ld_ok(R, C, lddy) || !ld_ok(R, C, ldx) || !ld_ok(R, C, lddx) ||
+          !(r.farg[0] >= 0.0f) || !std::isfinite(r.farg[0]))
+        return bad_shape("layer norm gradient");
+      if (!v.slot_ok(s[0], false, "dY") || !v.slot_ok(s[1], false, "X") || !v.slot_ok(s[2], true, "gamma") ||
+          !v.slot_ok(s[3], false, "dX") || !v.slot_ok(s[4], true, "dgamma") || !v.slot_ok(s[5], true, "dbeta") ||
+          !v.holds(s[0], span(R, C, lddy), DT_F32, "dY") || !v.holds(s[1], span(R, C, ldx), DT_F32, "X") ||
+          !v.holds(s[2], C, DT_F32, "gamma") || !v.holds(s[3], span(R, C, lddx), DT_F32, "dX") ||
+          !v.holds(s[4], C, DT_F32, "dgamma") || !v.holds(s[5], C, DT_F32, "dbeta") || !v.writable(s[3], "dX") ||
+          !v.writable(s[4], "dgamma") || !v.writable(s[5], "dbeta"))
+        return v.err;
+      // dX may replace dY row by row
+      if (!apart(s[3], {s[1], s[2], s[4], s[5]}) || (s[3] == s[0] && lddy != lddx)) return aliases("dX");
+      if (!apart(s[4], {s[0], s[1], s[2], s[5]})) return aliases("dgamma");
+      if (!apart(s[5], {s[0], s[1], s[2]})) return aliases("dbeta");
+      need(shk::layer_norm_grad_scratch_bytes(R, C));
+      return SHK_HIP_STATUS_OK;
+    }
+    case OP_GATED_SCAN: case OP_GATED_SCAN_GRAD: {
+      const bool grad = r.opcode == OP_GATED_SCAN_GRAD;
+      const int64_t B = a[0], T = a[1], D = a[2], is64 = a[3];
+      const int64_t states = prod(B, D), all = prod(states, T);
+      if (!extent_ok(B) || !extent_ok(T) || !extent_ok(D) || !flag_ok(is64) || states > INT32_MAX || states < 0 ||
+          all < 0 || all > INT64_MAX / 64)
+        return bad_shape("gated recurrence");
+      const uint32_t lt = is64 ? DT_I64 : DT_I32;
+      if (!grad) {
+        // Z, U, h0, lengths, H, last
+        if (!v.slot_ok(s[0], false, "Z") || !v.slot_ok(s[1], false, "U") || !v.slot_ok(s[2], true, "h0") ||
+            !v.slot_ok(s[3], true, "lengths") || !v.slot_ok(s[4], false, "H") || !v.slot_ok(s[5], true, "last") ||
+            !v.holds(s[0], all, DT_F32, "Z") || !v.holds(s[1], all, DT_F32, "U") ||
+            !v.holds(s[2], states, DT_F32, "h0") || !v.holds(s[3], B, lt, "lengths") ||
+            !v.holds(s[4], all, DT_F32, "H") || !v.holds(s[5], states, DT_F32, "last") || !v.writable(s[4], "H") ||
+            !v.writable(s[5], "last"))
+          return v.err;
+        // the last state may replace the first
+        if (!apart(s[4], {s[0], s[1], s[2], s[3], s[5]})) return aliases("H");
+        if (!apart(s[5], {s[0], s[1], s[3]})) return aliases("last");
+      } else {
+        if (st.payload.size() != sizeof(ScanEntry))
+          return fail(SHK_HIP_STATUS_GRAPH_COMPILATION_FAILED, "step %zu: a recurrence's gradient needs its slot entry",
+                      idx);
+        const ScanEntry& e = *reinterpret_cast<const ScanEntry*>(st.payload.data());
+        // dH, Z, U, H, h0, dlast, dZ, dU; dh0, lengths
+        if (!v.slot_ok(s[0], false, "dH") || !v.slot_ok(s[1], false, "Z") || !v.slot_ok(s[2], false, "U") ||
+            !v.slot_ok(s[3], false, "H") || !v.slot_ok(s[4], true, "h0") || !v.slot_ok(s[5], true, "dlast") ||
+            !v.slot_ok(s[6], false, "dZ") || !v.slot_ok(s[7], false, "dU") || !v.slot_ok(e.dh0, true, "dh0") ||
+            !v.slot_ok(e.lengths, true, "lengths") || !v.holds(s[0], all, DT_F32, "dH") ||
+            !v.holds(s[1], all, DT_F32, "Z") || !v.holds(s[2], all, DT_F32, "U") || !v.holds(s[3], all, DT_F32, "H") ||
+            !v.holds(s[4], states, DT_F32, "h0") || !v.holds(s[5], states, DT_F32, "dlast") ||
+            !v.holds(s[6], all, DT_F32, "dZ") || !v.holds(s[7], all, DT_F32, "dU") ||
+            !v.holds(e.dh0, states, DT_F32, "dh0") || !v.holds(e.lengths, B, lt, "lengths") ||
+            !v.writable(s[6], "dZ") || !v.writable(s[7], "dU") || !v.writable(e.dh0, "dh0"))
+          return v.err;
+        // the first state's gradient may replace the last one's
+        if (!apart(s[6], {s[0], s[1], s[2], s[3], s[4], s[5], s[7], e.dh0, e.lengths})) return aliases("dZ");
+        if (!apart(s[7], {s[0], s[1], s[2], s[3], s[4], s[5], e.dh0, e.lengths})) return aliases("dU");
+        if (!apart(e.dh0, {s[0], s[1], s[2], s[3], s[4], e.lengths})) return aliases("dh0");
+      }
+      need(shk::gated_scan_scratch_bytes(B, T, D));
+      return SHK_HIP_STATUS_OK;
+    }
+    default: {  // OP_DISTILL
+      const int64_t R = a[0], C = a[1], K = a[2], is64 = a[3];
+      const float T = r.farg[0];
+      if (!extent_ok(R) || C <= 0 || C > INT32_MAX - 1024 || K <= 0 || !flag_ok(is64) || !(T > 0.0f) ||
+          !std::isfinite(T) || !std::isfinite(1.0f / T))
+        return bad_shape("distillation");
+      if (K > shk::DISTILL_MOST)
+        return fail(SHK_HIP_STATUS_UNSUPPORTED_SHAPE, "step %zu: more than %lld teacher entries a row", idx,
+                    (long long)shk::DISTILL_MOST);
+      if (!v.slot_ok(s[0], false, "logits") || !v.slot_ok(s[1], false, "indices") ||
+          !v.slot_ok(s[2], false, "teacher logits") || !v.slot_ok(s[3], false, "loss") ||
+          !v.slot_ok(s[4], true, "grad") || !v.holds(s[0], prod(R, C), DT_F32, "logits") ||
+          !v.holds(s[1], prod(R, K), is64 ? DT_I64 : DT_I32, "indices") ||
+          !v.holds(s[2], prod(R, K), DT_F32, "teacher logits") || !v.holds(s[3], 1, DT_F32, "loss") ||
+          !v.holds(s[4], prod(R, C), DT_F32, "grad") || !v.writable(s[3], "loss") || !v.writable(s[4], "grad"))
+        return v.err;
+      if (!apart(s[3], {s[0], s[1], s[2], s[4]})) return aliases("loss");
+      if (!apart(s[4], {s[0], s[1], s[2]})) return aliases("grad");
+      need(shk::distill_scratch_bytes(R));
+      return SHK_HIP_STATUS_OK;
+    }
+  }
+}
+
 int32_t validate_step(const std::vector<SlotRecord>& slots, size_t idx, const Step& st,
                       uint64_t* scratch_doubles) {
   Validator v{slots, idx};
@@ -828,6 +989,9 @@ int32_t validate_step(const std::vector<SlotRecord>& slots, size_t idx, const St
       return SHK_HIP_STATUS_OK;
     case OP_MX_ENCODE: case OP_MX_DECODE: case OP_MX_ACT_GRAD: case OP_MX_GEMM: case OP_MX_LINEAR:
       return validate_mx_step(v, idx, st, scratch_doubles);
+    case OP_EMBED: case OP_EMBED_GRAD: case OP_LAYER_NORM: case OP_LAYER_NORM_GRAD: case OP_GATED_SCAN:
+    case OP_GATED_SCAN_GRAD: case OP_DISTILL:
+      return validate_token_step(v, idx, st, scratch_doubles);
     default:
       return fail(SHK_HIP_STATUS_UNSUPPORTED_OPERATION, "step %zu: unknown opcode %u", idx, r.opcode);
   }
@@ -1000,6 +1164,77 @@ hipError_t enqueue_step(const Step& st, const Bound& b, hipStream_t stream, doub
       p.x_format = (int)a[5]; p.w_format = (int)a[6]; p.act = (int)a[7];
       return shk::launch_mx_linear(p, scratch, stream);
     }
+    case OP_EMBED: case OP_EMBED_GRAD: {
+      shk::EmbedParams p{};
+      p.w = b.get<const float>(s[0]);
+      p.tokens = b.get<const void>(s[1]);
+      p.y = b.get<float>(s[2]);
+      p.N = a[0]; p.V = a[1]; p.D = a[2]; p.ldy = a[3];
+      p.is64 = (int)a[4]; p.has_pad = (int)a[5]; p.pad = a[6]; p.accumulate = (int)a[7];
+      p.scale = r.farg[0];
+      return r.opcode == OP_EMBED ? shk::launch_embed(p, status, stream)
+                                  : shk::launch_embed_grad(p, scratch, status, stream);
+    }
+    case OP_LAYER_NORM: {
+      shk::LayerNormParams p{};
+      p.x = b.get<const float>(s[0]);
+      p.gamma = b.get<const float>(s[1]);
+      p.beta = b.get<const float>(s[2]);
+      p.y = b.get<float>(s[3]);
+      p.R = a[0]; p.C = a[1]; p.ldx = a[2]; p.ldy = a[3];
+      p.eps = r.farg[0];
+      return shk::launch_layer_norm(p, stream);
+    }
+    case OP_LAYER_NORM_GRAD: {
+      shk::LayerNormGradParams p{};
+      p.dy = b.get<const float>(s[0]);
+      p.x = b.get<const float>(s[1]);
+      p.gamma = b.get<const float>(s[2]);
+      p.dx = b.get<float>(s[3]);
+      p.dgamma = b.get<float>(s[4]);
+      p.dbeta = b.get<float>(s[5]);
+      p.R = a[0]; p.C = a[1]; p.lddy = a[2]; p.ldx = a[3]; p.lddx = a[4];
+      p.eps = r.farg[0];
+      return shk::launch_layer_norm_grad(p, scratch, stream);
+    }
+    case OP_GATED_SCAN: {
+      shk::GatedScanParams p{};
+      p.z = b.get<const float>(s[0]);
+      p.u = b.get<const float>(s[1]);
+      p.h0 = b.get<const float>(s[2]);
+      p.lengths = b.get<const void>(s[3]);
+      p.h = b.get<float>(s[4]);
+      p.last = b.get<float>(s[5]);
+      p.B = a[0]; p.T = a[1]; p.D = a[2]; p.len64 = (int)a[3];
+      return shk::launch_gated_scan(p, reinterpret_cast<float*>(scratch), status, stream);
+    }
+    case OP_GATED_SCAN_GRAD: {
+      const ScanEntry& e = *reinterpret_cast<const ScanEntry*>(st.payload.data());
+      shk::GatedScanGradParams p{};
+      p.dh = b.get<const float>(s[0]);
+      p.z = b.get<const float>(s[1]);
+      p.u = b.get<const float>(s[2]);
+      p.h = b.get<const float>(s[3]);
+      p.h0 = b.get<const float>(s[4]);
+      p.dlast = b.get<const float>(s[5]);
+      p.dz = b.get<float>(s[6]);
+      p.du = b.get<float>(s[7]);
+      p.dh0 = b.get<float>(e.dh0);
+      p.lengths = b.get<const void>(e.lengths);
+      p.B = a[0]; p.T = a[1]; p.D = a[2]; p.len64 = (int)a[3];
+      return shk::launch_gated_scan_grad(p, reinterpret_cast<float*>(scratch), status, stream);
+    }
+    case OP_DISTILL: {
+      shk::DistillParams p{};
+      p.logits = b.get<const float>(s[0]);
+      p.index = b.get<const void>(s[1]);
+      p.teacher = b.get<const float>(s[2]);
+      p.loss = b.get<float>(s[3]);
+      p.grad = b.get<float>(s[4]);
+      p.R = a[0]; p.C = a[1]; p.K = a[2]; p.is64 = (int)a[3];
+      p.T = r.farg[0]; p.g = r.farg[1];
+      return shk::launch_distill(p, scratch, status, stream);
+    }
     default:
       return hipErrorInvalidValue;
   }
@@ -1068,6 +1303,27 @@ Access step_access(const Step& st) {
     case OP_MX_ACT_GRAD: R(sl[0]); R(sl[1]); R(sl[2]); W(sl[3]); W(sl[4]); break;
     case OP_MX_GEMM: R(sl[0]); R(sl[1]); R(sl[2]); W(sl[3]); break;
     case OP_MX_LINEAR: R(sl[0]); R(sl[1]); R(sl[2]); R(sl[3]); W(sl[4]); break;
+    // (a token, length or index out of bounds flags the word)
+    case OP_EMBED: R(sl[0]); R(sl[1]); W(sl[2]); x.status_or = true; break;
+    case OP_EMBED_GRAD:
+      R(sl[0]); R(sl[1]); W(sl[2]);
+      if (a[7]) R(sl[2]);  // accumulate
+      x.status_or = true;
+      break;
+    case OP_LAYER_NORM: R(sl[0]); R(sl[1]); R(sl[2]); W(sl[3]); break;
+    case OP_LAYER_NORM_GRAD: R(sl[0]); R(sl[1]); R(sl[2]); W(sl[3]); W(sl[4]); W(sl[5]); break;
+    case OP_GATED_SCAN:
+      R(sl[0]); R(sl[1]); R(sl[2]); R(sl[3]); W(sl[4]); W(sl[5]);
+      x.status_or = sl[3] >= 0;
+      break;
+    case OP_GATED_SCAN_GRAD: {
+      const ScanEntry& e = *reinterpret_cast<const ScanEntry*>(st.payload.data());
+      for (int k = 0; k < 6; ++k) R(sl[k]);
+      R(e.lengths); W(sl[6]); W(sl[7]); W(e.dh0);
+      x.status_or = e.lengths >= 0;
+      break;
+    }
+    case OP_DISTILL: R(sl[0]); R(sl[1]); R(sl[2]); W(sl[3]); W(sl[4]); x.status_or = true; break;
     default:  // unknown: conflicts with everything
       x.status_read = true;
       W(-2);
@@ -1083,6 +1339,9 @@ bool step_launches(const StepRecord& r) {
     case OP_MX_ENCODE: case OP_MX_DECODE: case OP_MX_GEMM: case OP_MX_LINEAR:
       return a[0] > 0 && a[1] > 0;
     case OP_MX_ACT_GRAD: return a[1] > 0 && (a[0] > 0 || r.slot[4] >= 0);
+    case OP_LAYER_NORM: return a[0] > 0 && a[1] > 0;
+    case OP_LAYER_NORM_GRAD: return a[1] > 0 && (a[0] > 0 || r.slot[4] >= 0 || r.slot[5] >= 0);
+    case OP_GATED_SCAN: case OP_GATED_SCAN_GRAD: return a[0] > 0 && a[2] > 0;
     case OP_COLSUM: return a[1] > 0;
     case OP_ROW_REDUCE: case OP_SOFTMAX: case OP_CE_HEAD: case OP_FILL: case OP_COPY:
       return a[0] > 0;

@@ -48,6 +48,13 @@ OP_MX_DECODE = 18
 OP_MX_ACT_GRAD = 19
 OP_MX_GEMM = 20
 OP_MX_LINEAR = 21
+OP_EMBED = 22
+OP_EMBED_GRAD = 23
+OP_LAYER_NORM = 24
+OP_LAYER_NORM_GRAD = 25
+OP_GATED_SCAN = 26
+OP_GATED_SCAN_GRAD = 27
+OP_DISTILL = 28
 
 ACT = {None: 0, "none": 0, "relu": 1, "tanh": 2, "sigmoid": 3}
 REDUCE_KIND = {"sum": 0, "mean": 1, "max": 2, "lse": 3}
@@ -348,6 +355,79 @@ class ProgramBuilder:
         return self._add(OP_MX_LINEAR, [X, *W, bias, Y],
                          [M, N, K, ldx if ldx is not None else K, ldy if ldy is not None else N,
                           _mx_format(x_format), _mx_format(w_format), ACT[act]])
+
+    # ---- models of tokens ----
+    def embed(self, W, tokens, Y, N, V, D, *, scale=1.0, pad=None, ldy=None) -> Step:
+        """Y [N, D] = scale * W[tokens] of a table W [V, D] and N tokens (i32 or i64), a zero row where
+        the token is `pad`. Any other token outside [0, V) fails the run (INDEX_OUT_OF_BOUNDS); its
+        row is zero."""
+        return self._add(OP_EMBED, [W, tokens, Y],
+                         [N, V, D, ldy if ldy is not None else D, self._is64(tokens), int(pad is not None),
+                          pad if pad is not None else 0], [scale])
+
+    def embed_grad(self, dY, tokens, dW, N, V, D, *, scale=1.0, pad=None, ldy=None,
+                   accumulate=False) -> Step:
+        """dW [V, D]: row v is scale times the sum of the rows of dY [N, D] whose token is v (in
+        binary64, in a fixed order), zero where there are none. With `accumulate` the sums are added
+        to dW (a table that is the output layer's weight too) and other rows are left as they are.
+        Tokens as for embed; one out of bounds adds nothing."""
+        return self._add(OP_EMBED_GRAD, [dY, tokens, dW],
+                         [N, V, D, ldy if ldy is not None else D, self._is64(tokens), int(pad is not None),
+                          pad if pad is not None else 0, int(accumulate)], [scale])
+
+    def layer_norm(self, X, Y, R, C, *, gamma=None, beta=None, eps=1e-5, ldx=None, ldy=None) -> Step:
+        """Y [R, C] = (X - mean) / sqrt(var + eps) * gamma + beta over each row of X; mean and var are
+        binary64. Y may be X (with ldy = ldx). A row with a value that is not finite is NaN."""
+        return self._add(OP_LAYER_NORM, [X, gamma, beta, Y],
+                         [R, C, ldx if ldx is not None else C, ldy if ldy is not None else C], [eps])
+
+    def layer_norm_grad(self, dY, X, dX, R, C, *, gamma=None, dgamma=None, dbeta=None, eps=1e-5,
+                        lddy=None, ldx=None, lddx=None) -> Step:
+        """The gradients of layer_norm's input, dX [R, C], and where given of gamma and beta, [C], from
+        dY [R, C] and the input X. dX may be dY (with lddx = lddy). Sums are binary64, in a fixed
+        order."""
+        return self._add(OP_LAYER_NORM_GRAD, [dY, X, gamma, dX, dgamma, dbeta],
+                         [R, C, lddy if lddy is not None else C, ldx if ldx is not None else C,
+                          lddx if lddx is not None else C], [eps])
+
+    def gated_scan(self, Z, U, H, B, T, D, *, h0=None, last=None, lengths=None) -> Step:
+        """The recurrence h_t = f_t h_(t-1) + (1 - f_t) u_t with f = sigmoid(z) over B sequences of T
+        positions, Z, U and H [B, T, D]; from the states h0 [B, D] (zero without), the states behind
+        the sequences into `last` [B, D], which may be h0: with T = 1 that moves a server's requests
+        on by a token. (Sequences stored position by position, [T, B, D], are one of width B D.)
+
+        lengths [B] (i32 or i64) are the positions that each sequence has: those behind are not
+        read, H is zero there, and `last` is the state at the end, h0 for a length of zero. A length
+        outside [0, T] fails the run (INDEX_OUT_OF_BOUNDS). A state that is not finite stays not
+        finite (an infinity may become NaN)."""
+        return self._add(OP_GATED_SCAN, [Z, U, h0, lengths, H, last], [B, T, D, self._is64(lengths)])
+
+    def gated_scan_grad(self, dH, Z, U, H, dZ, dU, B, T, D, *, h0=None, dlast=None, dh0=None,
+                        lengths=None) -> Step:
+        """The gradients of gated_scan's Z, U and, where dh0 is given, h0, from those of H and of the
+        last states (dlast, zero without), with the forward step's H, h0 and lengths. dZ and dU are
+        zero behind a sequence's end, where dH is not read. dh0 may be dlast."""
+        payload = struct.pack("<ii", _sid(dh0), _sid(lengths))
+        return self._add(OP_GATED_SCAN_GRAD, [dH, Z, U, H, h0, dlast, dZ, dU],
+                         [B, T, D, self._is64(lengths)], payload=payload)
+
+    def distill(self, logits, indices, teacher, loss, R, C, K, *, grad=None, temperature=1.0,
+                g=1.0) -> Step:
+        """loss[0] = T^2 / n sum_r sum_j p_rj (log p_rj - log q_r,i_rj): the divergence of the
+        distributions q = softmax(logits / T) over C classes from p = softmax(teacher / T) over a
+        row's K entries (at most 1024), the teacher's logits [R, K] of the classes `indices` [R, K]
+        (i32 or i64); T is the temperature and n the number of rows that have an entry. `grad`
+        receives g times the logits' gradient, g T / n (q - p).
+
+        An entry of index -1 or logit -inf is absent; a row without entries has a zero gradient
+        (none has one: the loss is NaN). Any other index outside [0, C) fails the run
+        (INDEX_OUT_OF_BOUNDS). Entries of one class add up. T is positive, and 1 / T finite."""
+        return self._add(OP_DISTILL, [logits, indices, teacher, loss, grad],
+                         [R, C, K, self._is64(indices)], [temperature, g])
+
+    @staticmethod
+    def _is64(slot) -> int:
+        return 1 if isinstance(slot, Slot) and slot.dtype == "i64" else 0
 
     # ---- encoding ----
     def image(self) -> bytes:
