@@ -5,7 +5,7 @@
 //   du_t = (1 - f_t) G_t,  dz_t = G_t (h_{t-1} - u_t) f_t (1 - f_t),  dh0 = f_0 G_0
 //
 // Each of the B D channels is a chain of steps s -> f s + b (forward b = (1 - f) u; backward, from
-// the last position on, b = f dh and s = f_t G_t), and a run of steps is again such a step: its
+// the last position on, s -> f (s + dh) with s = f_t G_t), and a run of steps is again such a step: its
 // product of f and its result from s = 0. So a workgroup takes 64 channels, one a lane, its NW waves
 // take TS consecutive positions each, form their runs' steps, read each other's from LDS, and
 // carry on from their own first state: one pass over the data, whose positions' gates stay in
@@ -28,8 +28,11 @@ namespace {
 // f = sigmoid(z) and k = 1 - f, each rounded once (fexp64.h).
 __device__ __forceinline__ void gates(float z, float& f, float& k) {
   const ExpParts p = exp_parts(-(double)fminf(fabsf(z), 110.0f));
-  const double e = fma(p.p, p.scale, p.scale);
-  const float a = (float)quotient_12(1.0, 1.0 + e), b = (float)quotient_12(e, 1.0 + e);
+  const double e = fma(p.p, p.scale, p.scale), d = 1.0 + e;
+  double y = __builtin_amdgcn_rcp(d);  // (quotient_12 of 1 and of e, with one reciprocal)
+  y = fma(fma(-d, y, 1.0), y, y);
+  const double q = e * y;
+  const float a = (float)fma(fma(-d, y, 1.0), y, y), b = (float)fma(fma(-d, q, e), y, q);
   f = z != z ? z : z >= 0.0f ? a : b;
   k = z != z ? z : z >= 0.0f ? b : a;
 }
@@ -51,6 +54,8 @@ struct ScanArgs {
   float* step_b;
   float* state;
   int64_t B, T, D, chunk, chunks;  // chunk: positions of one; chunks > 1: split
+  int64_t waves, parts;  // groups of up to 64 channels: of all sequences, of one
+  int pack, lanes;       // sequences a wave takes, lanes of each
   int len64;
 };
 
@@ -65,46 +70,62 @@ __device__ __forceinline__ int64_t scan_length(const ScanArgs& a, int64_t b, boo
   return n;
 }
 
-// What a position reads: forward z, u; backward z, dh, u, h_{t-1} (a chunk's step: z and dh).
-template <bool BACK>
-struct Position {
-  float z, u;
-  float dh, hp;
-};
-
 template <bool BACK, int MODE, int NW, int CW, int TS>
 __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
+  constexpr int READS = !BACK || MODE == STEPS ? 2 : 4;  // z and u; z and dh; z, dh, u and h_{t-1}
   __shared__ float2 steps[2][NW * CW][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tw = NW > 1 ? w : 0;
-  const int64_t channels = a.B * a.D;
-  const int64_t groups = (channels + 64 * CW - 1) / (64 * CW);
-  for (int64_t unit = blockIdx.x; unit < groups * a.chunks; unit += gridDim.x) {
-    const int64_t piece = unit / groups;  // in the order of the steps
-    const int64_t n0 = (unit % groups) * (64 * CW) + (CW > 1 ? w * 64 : 0) + lane;
-    const bool live = n0 < channels;
-    const int64_t n = live ? n0 : channels - 1;
-    const int64_t seq = n / a.D, base = seq * a.T * a.D + (n - seq * a.D);
-    const int64_t len = scan_length(a, seq, live && piece == 0);
-    // steps [lo, hi) of this piece; step p is position p forward, T - 1 - p backward
-    const int64_t lo = piece * a.chunk, hi = min(a.T, lo + a.chunk);
-    auto position = [&](int64_t p) { return BACK ? a.T - 1 - p : p; };
-
-    auto load = [&](Position<BACK> (&q)[TS], int64_t p0) {
+  const int64_t width = a.T * a.D;  // floats of a sequence
+  const int64_t blocks = (a.waves + CW - 1) / CW;
+  for (int64_t unit = blockIdx.x; unit < blocks * a.chunks; unit += gridDim.x) {
+    const int64_t piece = unit / blocks, wave = (unit % blocks) * CW + (CW > 1 ? w : 0);
+    // this wave's channels: 64 of one sequence, or those of `pack` short ones
+    const int64_t first_seq = wave / a.parts * a.pack, part = wave % a.parts;
+    const int sub = a.pack > 1 ? lane / a.lanes : 0, c = (int)part * 64 + (a.pack > 1 ? lane % a.lanes : lane);
+    const bool live = wave < a.waves && sub < a.pack && c < a.D && first_seq + sub < a.B;
+    const int64_t seq = live ? first_seq + sub : 0, n = seq * a.D + (live ? c : 0);
+    const int64_t base = first_seq * width + part * 64;
+    const uint32_t at = 4u * (uint32_t)(sub * width + (c - (int)part * 64));  // bytes from there
+    const int len = (int)scan_length(a, seq, live && piece == 0);
+    // steps [lo, hi) of this piece; step p is position p forward, T - 1 - p backward; this lane's
+    // sequence has those of [from, to)
+    const int T = (int)a.T, lo = (int)(piece * a.chunk), hi = (int)min(a.T, piece * a.chunk + a.chunk);
+    const int from = BACK ? T - len : 0, to = BACK ? T : len;
+    const int64_t dir = BACK ? -a.D : a.D;
+    auto row = [&](const float* x, int p) { return x + base + (int64_t)(BACK ? T - 1 - p : p) * a.D; };
+    auto get = [&](const float* x) {
+      return __builtin_nontemporal_load(reinterpret_cast<const float*>(reinterpret_cast<const char*>(x) + at));
+    };
+    auto put = [&](float* x, float v) {
+      __builtin_nontemporal_store(v, reinterpret_cast<float*>(reinterpret_cast<char*>(x) + at));
+    };
+    const float* const src[4] = {a.z, BACK ? a.dh : a.u, a.u, a.h};
+    float next[READS][TS];
+    auto load = [&](int p0) {
+      // (behind step p0 + TS - 1 lies the position whose state is read with the last)
+      const bool whole = p0 + TS <= (BACK ? min(hi, T - 1) : hi) && __all(!live || (from <= p0 && p0 + TS <= to));
+      if (whole) {
+        if (live) {
+#pragma unroll
+          for (int r = 0; r < READS; ++r) {
+            const float* x = row(src[r], p0) - (r == 3 ? a.D : 0);
+#pragma unroll
+            for (int i = 0; i < TS; ++i, x += dir) next[r][i] = get(x);
+          }
+        }
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
-        const int64_t p = p0 + i, t = position(p);
-        const bool in = p < hi && t < len && live;
-        const int64_t at = base + t * a.D;
-        q[i].z = in ? __builtin_nontemporal_load(a.z + at) : 0.0f;
-        if (!BACK) {
-          q[i].u = in ? __builtin_nontemporal_load(a.u + at) : 0.0f;
-        } else {
-          q[i].dh = in ? __builtin_nontemporal_load(a.dh + at) : 0.0f;
-          if (MODE != STEPS) {
-            q[i].u = in ? __builtin_nontemporal_load(a.u + at) : 0.0f;
-            q[i].hp = !in ? 0.0f : t > 0 ? __builtin_nontemporal_load(a.h + at - a.D)
-                                 : a.h0 != nullptr ? a.h0[n] : 0.0f;
+        const int p = p0 + i;
+        const bool in = live && p < hi && p >= from && p < to;
+#pragma unroll
+        for (int r = 0; r < READS; ++r) {
+          next[r][i] = 0.0f;
+          if (in) {
+            if (r < 3 || p < T - 1) next[r][i] = get(row(src[r], p) - (r == 3 ? a.D : 0));
+            else next[r][i] = a.h0 != nullptr ? a.h0[n] : 0.0f;
           }
         }
       }
@@ -112,37 +133,34 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
 
     float state = 0.0f, all = 1.0f;
     if (MODE == WHOLE) state = a.first != nullptr ? a.first[n] : 0.0f;
-    if (MODE == CHUNK) state = a.state[piece * channels + n];
-    Position<BACK> next[TS];
-    load(next, lo + tw * TS);
+    if (MODE == CHUNK) state = a.state[piece * a.B * a.D + n];
+    load(lo + tw * TS);
     int turn = 0;
-    for (int64_t p0 = lo; p0 < hi; p0 += NW * TS, turn ^= 1) {
-      float f[TS], k[TS], b[TS], v[TS], w2[TS];
+    for (int p0 = lo; p0 < hi; p0 += NW * TS, turn ^= 1) {
+      const int q0 = p0 + tw * TS;
+      float f[TS], b[TS], k[TS], v[TS], m[TS];
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
-        const int64_t p = p0 + tw * TS + i, t = position(p);
-        if (p < hi) {
-          gates(next[i].z, f[i], k[i]);
-          if (!(t < len)) f[i] = 1.0f;
-          if (BACK) {
-            v[i] = next[i].dh;
-            b[i] = f[i] * v[i];
-            if (MODE != STEPS) w2[i] = (next[i].hp - next[i].u) * (f[i] * k[i]);
-          } else {
-            b[i] = t < len ? k[i] * next[i].u : 0.0f;
-          }
+        gates(next[0][i], f[i], k[i]);
+        const bool in = q0 + i < hi && q0 + i >= from && q0 + i < to;
+        if (BACK) {
+          v[i] = next[1][i];
+          if (MODE != STEPS) m[i] = in ? (next[3][i] - next[2][i]) * (f[i] * k[i]) : 0.0f;
+          k[i] = in ? k[i] : 0.0f;
+          v[i] = in ? v[i] : 0.0f;
         } else {
-          f[i] = 1.0f;
-          b[i] = k[i] = v[i] = w2[i] = 0.0f;
+          b[i] = in ? k[i] * next[1][i] : 0.0f;
         }
+        f[i] = in ? f[i] : 1.0f;
+        __builtin_amdgcn_sched_barrier(0);  // one gate's binary64 values at a time
       }
-      if (p0 + NW * TS < hi) load(next, p0 + (NW + tw) * TS);
+      if (p0 + NW * TS < hi) load(q0 + NW * TS);
       float s = state;
       if (NW > 1 || MODE == STEPS) {
         float run_f = 1.0f, run_b = 0.0f;
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          run_b = fmaf(f[i], run_b, b[i]);
+          run_b = BACK ? f[i] * (run_b + v[i]) : fmaf(f[i], run_b, b[i]);
           run_f *= f[i];
         }
         if (NW > 1) {
@@ -160,32 +178,29 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
           all *= run_f;
         }
       }
-      if (MODE != STEPS) {
+      if (MODE != STEPS && live) {
+        float* x[2] = {const_cast<float*>(row(a.out[0], q0)), BACK ? const_cast<float*>(row(a.out[1], q0)) : nullptr};
 #pragma unroll
-        for (int i = 0; i < TS; ++i) {
-          const int64_t p = p0 + tw * TS + i, t = position(p);
-          const bool in = p < hi && live, real = t < len;
-          const int64_t at = base + t * a.D;
+        for (int i = 0; i < TS; ++i, x[0] += dir, x[1] += BACK ? dir : 0) {
+          if (q0 + i >= hi) break;
           if (BACK) {
             const float g = v[i] + s;
-            if (in) {
-              __builtin_nontemporal_store(real ? g * w2[i] : 0.0f, a.out[0] + at);
-              __builtin_nontemporal_store(real ? g * k[i] : 0.0f, a.out[1] + at);
-            }
-            s = fmaf(f[i], s, b[i]);
+            put(x[0], g * m[i]);
+            put(x[1], g * k[i]);
+            s = f[i] * g;
           } else {
             s = fmaf(f[i], s, b[i]);
-            if (in) __builtin_nontemporal_store(real ? s : 0.0f, a.out[0] + at);
+            put(x[0], q0 + i < to ? s : 0.0f);
           }
         }
-        if (NW == 1) state = s;
       }
+      if (NW == 1 && MODE != STEPS) state = s;
     }
     if (tw == 0 && live) {
       if (MODE == WHOLE && a.last != nullptr) a.last[n] = state;
       if (MODE == STEPS) {
-        a.step_f[piece * channels + n] = all;
-        a.step_b[piece * channels + n] = state;
+        a.step_f[piece * a.B * a.D + n] = all;
+        a.step_b[piece * a.B * a.D + n] = state;
       }
     }
     if (NW > 1) __syncthreads();  // the steps in LDS have been read
@@ -206,10 +221,21 @@ __global__ void __launch_bounds__(64) scan_carry(ScanArgs a) {
   }
 }
 
+// Lanes of a wave for one sequence of D channels: all 64, or the next power of two where several
+// sequences' offsets stay within 32 bits.
+int scan_lanes(int64_t B, int64_t T, int64_t D) {
+  int lanes = 64;
+  while (lanes > 1 && lanes / 2 >= D) lanes /= 2;
+  return B > 1 && lanes < 64 && T * D <= (1 << 29) / (64 / lanes) ? lanes : 64;
+}
+int64_t scan_waves(int64_t B, int64_t T, int64_t D) {
+  const int64_t pack = 64 / scan_lanes(B, T, D);
+  return (B + pack - 1) / pack * ((D + 63) / 64);
+}
 // Positions of a chunk: all of them where the channels fill the CUs or there is little to split.
 constexpr int64_t SCAN_GROUPS = 512, SCAN_LEAST = 512;
 int64_t scan_chunk(int64_t B, int64_t T, int64_t D) {
-  const int64_t groups = (B * D + 63) / 64;
+  const int64_t groups = scan_waves(B, T, D);
   if (groups >= SCAN_GROUPS / 2 || T < 2 * SCAN_LEAST) return T;
   const int64_t chunks = std::min(T / SCAN_LEAST, (SCAN_GROUPS + groups - 1) / groups);
   return chunks <= 1 ? T : ((T + chunks - 1) / chunks + 255) / 256 * 256;
@@ -218,25 +244,29 @@ int64_t scan_chunk(int64_t B, int64_t T, int64_t D) {
 template <bool BACK>
 hipError_t launch_scan(ScanArgs a, float* scratch, hipStream_t s) {
   const int64_t channels = a.B * a.D;
-  auto blocks = [&](int64_t wide) {
-    return dim3((unsigned)std::min<int64_t>((channels + wide - 1) / wide * a.chunks, 1 << 20));
+  a.lanes = scan_lanes(a.B, a.T, a.D);
+  a.pack = 64 / a.lanes;
+  a.parts = (a.D + 63) / 64;
+  a.waves = scan_waves(a.B, a.T, a.D);
+  auto blocks = [&](int64_t waves) {
+    return dim3((unsigned)std::min<int64_t>((a.waves + waves - 1) / waves * a.chunks, 1 << 20));
   };
-  constexpr int TS = BACK ? 8 : 16;
+  constexpr int TS = 8;
   a.chunk = std::max<int64_t>(1, scan_chunk(a.B, a.T, a.D));
   a.chunks = std::max<int64_t>(1, (a.T + a.chunk - 1) / a.chunk);
   if (a.chunks > 1) {
     a.step_f = scratch;
     a.step_b = scratch + a.chunks * channels;
     a.state = scratch + 2 * a.chunks * channels;
-    hipLaunchKernelGGL((scan_kernel<BACK, STEPS, 16, 1, TS>), blocks(64), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((scan_kernel<BACK, STEPS, 16, 1, TS>), blocks(1), dim3(1024), 0, s, a);
     hipLaunchKernelGGL(scan_carry, dim3((unsigned)((channels + 63) / 64)), dim3(64), 0, s, a);
-    hipLaunchKernelGGL((scan_kernel<BACK, CHUNK, 16, 1, TS>), blocks(64), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((scan_kernel<BACK, CHUNK, 16, 1, TS>), blocks(1), dim3(1024), 0, s, a);
   } else if (a.T <= 8) {
-    hipLaunchKernelGGL((scan_kernel<BACK, WHOLE, 1, 4, 4>), blocks(256), dim3(256), 0, s, a);
-  } else if (a.T <= 4 * TS) {
-    hipLaunchKernelGGL((scan_kernel<BACK, WHOLE, 4, 1, TS>), blocks(64), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((scan_kernel<BACK, WHOLE, 1, 4, 4>), blocks(4), dim3(256), 0, s, a);
+  } else if (a.T <= 8 * TS) {
+    hipLaunchKernelGGL((scan_kernel<BACK, WHOLE, 4, 1, TS>), blocks(1), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((scan_kernel<BACK, WHOLE, 16, 1, TS>), blocks(64), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((scan_kernel<BACK, WHOLE, 16, 1, TS>), blocks(1), dim3(1024), 0, s, a);
   }
   return hipGetLastError();
 }

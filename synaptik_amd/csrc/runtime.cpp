@@ -637,7 +637,8 @@ int32_t validate_token_step(Validator& v, size_t idx, const Step& st, uint64_t* 
       const bool grad = r.opcode == OP_GATED_SCAN_GRAD;
       const int64_t B = a[0], T = a[1], D = a[2], is64 = a[3];
       const int64_t states = prod(B, D), all = prod(states, T);
-      if (!extent_ok(B) || !extent_ok(T) || !extent_ok(D) || !flag_ok(is64) || states > INT32_MAX || states < 0 ||
+      // (the kernel counts positions in an int, some tiles ahead)
+      if (!extent_ok(B) || !extent_ok(T) || T > INT32_MAX - 4096 || !extent_ok(D) || !flag_ok(is64) || states > INT32_MAX || states < 0 ||
           all < 0 || all > INT64_MAX / 64)
         return bad_shape("gated recurrence");
       const uint32_t lt = is64 ? DT_I64 : DT_I32;
