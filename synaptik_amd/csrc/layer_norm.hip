@@ -17,23 +17,17 @@
 #include "common.h"
 #include "kernels.h"
 #include "row4.h"
+#include "wave_sum.h"
 
 namespace shk {
 namespace {
 
-// Sums over the L lanes (a power of two) that hold one row.
-template <int L>
-__device__ __forceinline__ double team_sum(double v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 // Sums over a workgroup of NT threads of K values; `lds` is free again after the next barrier.
 template <int NT, int K>
 __device__ __forceinline__ void group_sum(double (&v)[K], double* lds) {
   constexpr int NW = NT / 64;
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+  for (int k = 0; k < K; ++k) v[k] = wave_total(v[k]);
   if (NW == 1) return;
   const int w = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) {
@@ -41,25 +35,25 @@ __device__ __forceinline__ void group_sum(double (&v)[K], double* lds) {
     for (int k = 0; k < K; ++k) lds[w * K + k] = v[k];
   }
   __syncthreads();
+  // every group of NW lanes reads the waves' sums, one a lane
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    double s = lds[k];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) s += lds[i * K + k];
-    v[k] = s;
-  }
+  for (int k = 0; k < K; ++k) v[k] = wave_uniform(team_total<NW>(lds[(threadIdx.x & (NW - 1)) * K + k]));
 }
 
 // A row in the registers of T threads, V groups of four floats each, T groups apart.
 template <int T, int V>
 struct Row {
   float4 v[V];
-  __device__ __forceinline__ void load(const float* p, int t, int64_t C) {
+  // `rest`: the floats from this thread's first group to the row's end
+  template <bool STREAM>
+  __device__ __forceinline__ void load(const float* row, int t, int rest) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int64_t c = 4 * (t + (int64_t)i * T);
-      v[i] = ld4<true>(p + c, C - c);
-    }
+    for (int i = 0; i < V; ++i) v[i] = ld4_at<STREAM>(row, 16u * t + 16u * T * i, rest - 4 * T * i);
+  }
+  __device__ __forceinline__ void load_or(const float* row, int t, int rest, float otherwise) {
+    if (row != nullptr) return load<false>(row, t, rest);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = make_float4(otherwise, otherwise, otherwise, otherwise);
   }
 };
 #define LN_EACH(i, j, c, C)                                      \
@@ -79,32 +73,33 @@ struct FwdArgs {
   double eps;
 };
 
-// T threads a row: a part of a wave (SUM: team_sum), or the whole workgroup.
+// T threads a row: a part of a wave, or the whole workgroup.
 template <int NT, int T, int V>
 __global__ void __launch_bounds__(NT) ln_fwd(FwdArgs a) {
   __shared__ double lds[2][NT / 64];
-  const int t = threadIdx.x % T;
+  const int t = threadIdx.x % T, rest = (int)a.C - 4 * t;
   Row<T, V> gm, bt;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int64_t c = 4 * (t + (int64_t)i * T);
-    gm.v[i] = a.gamma != nullptr ? ld4(a.gamma + c, a.C - c) : make_float4(1.f, 1.f, 1.f, 1.f);
-    bt.v[i] = a.beta != nullptr ? ld4(a.beta + c, a.C - c) : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
+  gm.load_or(a.gamma, t, rest, 1.0f);
+  bt.load_or(a.beta, t, rest, 0.0f);
   for (int64_t r = (int64_t)blockIdx.x * (NT / T) + threadIdx.x / T; r < a.R; r += (int64_t)gridDim.x * (NT / T)) {
     Row<T, V> x;
-    x.load(a.x + r * a.ldx, t, a.C);
+    x.template load<true>(a.x + r * a.ldx, t, rest);
     double s[1] = {0.0};
-    LN_EACH(i, j, c, a.C) s[0] += (double)at(x.v[i], j);
-    if constexpr (T < NT) s[0] = team_sum<T>(s[0]);
+#pragma unroll
+    for (int i = 0; i < V; ++i)  // (0 behind the row's end)
+      s[0] += ((double)x.v[i].x + (double)x.v[i].y) + ((double)x.v[i].z + (double)x.v[i].w);
+    if constexpr (T < NT) s[0] = team_total<T>(s[0]);
     else group_sum<NT, 1>(s, lds[0]);
     const double mean = s[0] / (double)a.C;
     double q[1] = {0.0};
-    LN_EACH(i, j, c, a.C) {
-      const double d = (double)at(x.v[i], j) - mean;
-      q[0] = fma(d, d, q[0]);
-    }
-    if constexpr (T < NT) q[0] = team_sum<T>(q[0]);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double d = j < rest - 4 * T * i ? (double)at(x.v[i], j) - mean : 0.0;
+        q[0] = fma(d, d, q[0]);
+      }
+    if constexpr (T < NT) q[0] = team_total<T>(q[0]);
     else group_sum<NT, 1>(q, lds[1]);
     const double rstd = 1.0 / sqrt(q[0] / (double)a.C + a.eps);
     float* y = a.y + r * a.ldy;
@@ -114,8 +109,7 @@ __global__ void __launch_bounds__(NT) ln_fwd(FwdArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         at(o, j) = fmaf((float)(((double)at(x.v[i], j) - mean) * rstd), at(gm.v[i], j), at(bt.v[i], j));
-      const int64_t c = 4 * (t + (int64_t)i * T);
-      st4<true>(y + c, a.C - c, o);
+      st4_at<true>(y, 16u * t + 16u * T * i, rest - 4 * T * i, o);
     }
   }
 }
@@ -173,55 +167,75 @@ struct BwdArgs {
   double eps;
 };
 
-// dy and dx may be the same memory: a thread writes the elements that it read.
-template <int NT, int T, int V>
-__global__ void __launch_bounds__(NT) ln_bwd(BwdArgs a) {
-  __shared__ double lds[4][NT / 64];
-  const int t = threadIdx.x % T;
-  Row<T, V> gm;
-  double dg[V][4], db[V][4];
+// Values that the compiler takes as new, so that it forms what depends on them again instead of
+// holding it in registers.
+template <int V>
+__device__ __forceinline__ void forget(float4 (&v)[V]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int64_t c = 4 * (t + (int64_t)i * T);
-    gm.v[i] = a.gamma != nullptr ? ld4(a.gamma + c, a.C - c) : make_float4(1.f, 1.f, 1.f, 1.f);
+  for (int i = 0; i < V; ++i) asm volatile("" : "+v"(v[i].x), "+v"(v[i].y), "+v"(v[i].z), "+v"(v[i].w));
+}
+
+// dy and dx may be the same memory: a thread writes the elements that it read. AHEAD: the next row is
+// on its way while this one is summed.
+template <int NT, int T, int V, bool AHEAD>
+__device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[NT / 64], double (&dg)[V][4],
+                                            double (&db)[V][4]) {
+  const int t = threadIdx.x % T, rest = (int)a.C - 4 * t;
+  Row<T, V> gm;
+  gm.load_or(a.gamma, t, rest, 1.0f);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) dg[i][j] = db[i][j] = 0.0;
-  }
   const int64_t step = (int64_t)gridDim.x * (NT / T);
   int64_t r = (int64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
   Row<T, V> x, dy, nx, ndy;
-  if (r < a.R) {
-    nx.load(a.x + r * a.ldx, t, a.C);
-    ndy.load(a.dy + r * a.lddy, t, a.C);
+  if (AHEAD && r < a.R) {
+    nx.template load<true>(a.x + r * a.ldx, t, rest);
+    ndy.template load<true>(a.dy + r * a.lddy, t, rest);
   }
   for (; r < a.R; r += step) {
-    x = nx;
-    dy = ndy;
-    if (r + step < a.R) {  // the next row is on its way while this one is summed
-      nx.load(a.x + (r + step) * a.ldx, t, a.C);
-      ndy.load(a.dy + (r + step) * a.lddy, t, a.C);
+    if (AHEAD) {
+      x = nx;
+      dy = ndy;
+      if (r + step < a.R) {
+        nx.template load<true>(a.x + (r + step) * a.ldx, t, rest);
+        ndy.template load<true>(a.dy + (r + step) * a.lddy, t, rest);
+      }
+    } else {
+      x.template load<true>(a.x + r * a.ldx, t, rest);
+      dy.template load<true>(a.dy + r * a.lddy, t, rest);
     }
     double s[1] = {0.0};
-    LN_EACH(i, j, c, a.C) s[0] += (double)at(x.v[i], j);
-    if constexpr (T < NT) s[0] = team_sum<T>(s[0]);
+#pragma unroll
+    for (int i = 0; i < V; ++i)  // (0 behind the row's end)
+      s[0] += ((double)x.v[i].x + (double)x.v[i].y) + ((double)x.v[i].z + (double)x.v[i].w);
+    if constexpr (T < NT) s[0] = team_total<T>(s[0]);
     else group_sum<NT, 1>(s, lds[0]);
     const double mean = s[0] / (double)a.C;
+    forget(x.v);
     double q[3] = {0.0, 0.0, 0.0};  // sums of d^2, g, g d with d = x - mean
-    LN_EACH(i, j, c, a.C) {
-      const double d = (double)at(x.v[i], j) - mean;
-      const double g = (double)at(dy.v[i], j) * (double)at(gm.v[i], j);
-      q[0] = fma(d, d, q[0]);
-      q[1] += g;
-      q[2] = fma(g, d, q[2]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double d = j < rest - 4 * T * i ? (double)at(x.v[i], j) - mean : 0.0;
+        const double g = (double)at(dy.v[i], j) * (double)at(gm.v[i], j);
+        q[0] = fma(d, d, q[0]);
+        q[1] += g;
+        q[2] = fma(g, d, q[2]);
+      }
     }
     if constexpr (T < NT) {
 #pragma unroll
-      for (int k = 0; k < 3; ++k) q[k] = team_sum<T>(q[k]);
+      for (int k = 0; k < 3; ++k) q[k] = team_total<T>(q[k]);
     } else {
       group_sum<NT, 3>(q, lds[1]);
     }
     const double rstd = 1.0 / sqrt(q[0] / (double)a.C + a.eps);
     const double c1 = q[1] / (double)a.C, c2 = rstd * rstd * (q[2] / (double)a.C);
+    forget(x.v);
+    forget(dy.v);
     float* dx = a.dx + r * a.lddx;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -234,10 +248,19 @@ __global__ void __launch_bounds__(NT) ln_bwd(BwdArgs a) {
         dg[i][j] = fma(v, d * rstd, dg[i][j]);
         db[i][j] += v;
       }
-      const int64_t c = 4 * (t + (int64_t)i * T);
-      st4<true>(dx + c, a.C - c, o);
+      st4_at<true>(dx, 16u * t + 16u * T * i, rest - 4 * T * i, o);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+}
+
+// Four waves on each SIMD where a workgroup holds a row; a wave that holds one has up to 256 registers.
+template <int NT, int T, int V, bool AHEAD = true>
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(T == 64 ? 2 : 4))) ln_bwd(BwdArgs a) {
+  __shared__ double lds[4][NT / 64];
+  const int t = threadIdx.x % T;
+  double dg[V][4], db[V][4];
+  ln_bwd_rows<NT, T, V, AHEAD>(a, lds, dg, db);
   if (a.part == nullptr) return;
   double* out = a.part + (int64_t)blockIdx.x * 2 * a.C;
   if constexpr (T == NT) {
@@ -436,7 +459,7 @@ hipError_t launch_layer_norm_grad(const LayerNormGradParams& p, double* scratch,
     else if (p.C <= 2048) hipLaunchKernelGGL((ln_bwd<256, 256, 2>), g, dim3(256), 0, s, a);
     else if (p.C <= 4096) hipLaunchKernelGGL((ln_bwd<512, 512, 2>), g, dim3(512), 0, s, a);
     else if (p.C <= 8192) hipLaunchKernelGGL((ln_bwd<1024, 1024, 2>), g, dim3(1024), 0, s, a);
-    else if (p.C <= LN_REGS) hipLaunchKernelGGL((ln_bwd<1024, 1024, 4>), g, dim3(1024), 0, s, a);
+    else if (p.C <= LN_REGS) hipLaunchKernelGGL((ln_bwd<1024, 1024, 4, false>), g, dim3(1024), 0, s, a);
     else {
       const dim3 rows((unsigned)std::min<int64_t>(p.R, 1 << 16));
       if (sums) {
