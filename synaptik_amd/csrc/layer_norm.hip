@@ -12,6 +12,13 @@
 // squares about it are binary64, as are all sums. dgamma and dbeta are summed beside dx: each
 // workgroup takes every G-th group of rows, keeps its columns' sums in registers and writes one
 // row of partial sums, which a second launch adds in a fixed order.
+//
+// All of a row's sums are formed at once, over d = x - x_0 instead of x - mean:
+//   delta = sum d / C = mean - x_0,  var = sum d^2 / C - delta^2,
+//   sum g (x - mean) = sum g d - delta sum g.
+// As x_0 is a value of the row, delta^2 <= C var, so the difference loses at most log2 (C + 1) of the
+// 53 bits of sums whose terms pass through some 30 roundings (a thread's values, then a tree): var
+// is within 2^-33 of its value at 16384 columns, and exactly 0 for a constant row.
 #include <algorithm>
 
 #include "common.h"
@@ -21,24 +28,6 @@
 
 namespace shk {
 namespace {
-
-// Sums over a workgroup of NT threads of K values; `lds` is free again after the next barrier.
-template <int NT, int K>
-__device__ __forceinline__ void group_sum(double (&v)[K], double* lds) {
-  constexpr int NW = NT / 64;
-#pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = wave_total(v[k]);
-  if (NW == 1) return;
-  const int w = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) lds[w * K + k] = v[k];
-  }
-  __syncthreads();
-  // every group of NW lanes reads the waves' sums, one a lane
-#pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = wave_uniform(team_total<NW>(lds[(threadIdx.x & (NW - 1)) * K + k]));
-}
 
 // A row in the registers of T threads, V groups of four floats each, T groups apart.
 template <int T, int V>
@@ -64,51 +53,63 @@ struct Row {
 __device__ __forceinline__ float& at(float4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 __device__ __forceinline__ float at(const float4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
+#ifndef LN_NT
+#define LN_NT true
+#endif
+// Sums of a row that T threads hold.
+template <int NT, int T, int K>
+__device__ __forceinline__ void row_sums(double (&v)[K], double* lds) {
+  if constexpr (T < NT) team_sums<T, K>(v);
+  else group_sums<NT, K>(v, lds);
+}
+// The mean of squares less the square of the mean, not below zero (NaN stays).
+__device__ __forceinline__ double variance(double squares, double delta) {
+  const double v = fma(-delta, delta, squares);
+  return v < 0.0 ? 0.0 : v;
+}
+
 struct FwdArgs {
   const float* x;
   const float* gamma;
   const float* beta;
   float* y;
   int64_t R, C, ldx, ldy;
-  double eps;
+  double eps, inv_C;
 };
 
 // T threads a row: a part of a wave, or the whole workgroup.
 template <int NT, int T, int V>
 __global__ void __launch_bounds__(NT) ln_fwd(FwdArgs a) {
-  __shared__ double lds[2][NT / 64];
+  __shared__ double lds[2][2 * (NT / 64)];
+  int turn = 0;
   const int t = threadIdx.x % T, rest = (int)a.C - 4 * t;
   Row<T, V> gm, bt;
   gm.load_or(a.gamma, t, rest, 1.0f);
   bt.load_or(a.beta, t, rest, 0.0f);
   for (int64_t r = (int64_t)blockIdx.x * (NT / T) + threadIdx.x / T; r < a.R; r += (int64_t)gridDim.x * (NT / T)) {
+    const float* row = a.x + r * a.ldx;
+    const float x0 = row[0];
     Row<T, V> x;
-    x.template load<true>(a.x + r * a.ldx, t, rest);
-    double s[1] = {0.0};
-#pragma unroll
-    for (int i = 0; i < V; ++i)  // (0 behind the row's end)
-      s[0] += ((double)x.v[i].x + (double)x.v[i].y) + ((double)x.v[i].z + (double)x.v[i].w);
-    if constexpr (T < NT) s[0] = team_total<T>(s[0]);
-    else group_sum<NT, 1>(s, lds[0]);
-    const double mean = s[0] / (double)a.C;
-    double q[1] = {0.0};
+    x.template load<LN_NT>(row, t, rest);
+    double s[2] = {0.0, 0.0};
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const double d = j < rest - 4 * T * i ? (double)at(x.v[i], j) - mean : 0.0;
-        q[0] = fma(d, d, q[0]);
+        const double d = (double)(j < rest - 4 * T * i ? at(x.v[i], j) : x0) - (double)x0;
+        s[0] += d;
+        s[1] = fma(d, d, s[1]);
       }
-    if constexpr (T < NT) q[0] = team_total<T>(q[0]);
-    else group_sum<NT, 1>(q, lds[1]);
-    const double rstd = 1.0 / sqrt(q[0] / (double)a.C + a.eps);
+    row_sums<NT, T>(s, lds[turn]);
+    turn ^= 1;
+    const double delta = s[0] * a.inv_C, rstd = 1.0 / sqrt(variance(s[1] * a.inv_C, delta) + a.eps);
     float* y = a.y + r * a.ldy;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        at(o, j) = fmaf((float)(((double)at(x.v[i], j) - mean) * rstd), at(gm.v[i], j), at(bt.v[i], j));
+        at(o, j) = fmaf((float)((((double)at(x.v[i], j) - (double)x0) - delta) * rstd), at(gm.v[i], j), at(bt.v[i], j));
       st4_at<true>(y, 16u * t + 16u * T * i, rest - 4 * T * i, o);
     }
   }
@@ -123,7 +124,7 @@ __device__ __forceinline__ void wide_stats(const float* x, int64_t C, double eps
     const float4 v = ld4(x + c, C - c);
     s[0] += ((double)v.x + (double)v.y) + ((double)v.z + (double)v.w);
   }
-  group_sum<LN_WIDE, 1>(s, lds[0]);
+  group_sums<LN_WIDE, 1>(s, lds[0]);
   mean = s[0] / (double)C;
   for (int64_t c = 4 * threadIdx.x; c < C; c += 4 * LN_WIDE) {
     const float4 v = ld4(x + c, C - c);
@@ -133,7 +134,7 @@ __device__ __forceinline__ void wide_stats(const float* x, int64_t C, double eps
       q[0] = fma(d, d, q[0]);
     }
   }
-  group_sum<LN_WIDE, 1>(q, lds[1]);
+  group_sums<LN_WIDE, 1>(q, lds[1]);
   rstd = 1.0 / sqrt(q[0] / (double)C + eps);
 }
 __global__ void __launch_bounds__(LN_WIDE) ln_fwd_wide(FwdArgs a) {
@@ -164,7 +165,7 @@ struct BwdArgs {
   double* part;   // [gridDim.x][2][C]: partial sums of dgamma and dbeta; null: neither is wanted
   double* stats;  // [R][2]: mean and rstd (wide rows)
   int64_t R, C, lddy, ldx, lddx;
-  double eps;
+  double eps, inv_C;
 };
 
 // Values that the compiler takes as new, so that it forms what depends on them again instead of
@@ -178,7 +179,7 @@ __device__ __forceinline__ void forget(float4 (&v)[V]) {
 // dy and dx may be the same memory: a thread writes the elements that it read. AHEAD: the next row is
 // on its way while this one is summed.
 template <int NT, int T, int V, bool AHEAD>
-__device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[NT / 64], double (&dg)[V][4],
+__device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[4 * (NT / 64)], double (&dg)[V][4],
                                             double (&db)[V][4]) {
   const int t = threadIdx.x % T, rest = (int)a.C - 4 * t;
   Row<T, V> gm;
@@ -190,50 +191,36 @@ __device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[NT /
   const int64_t step = (int64_t)gridDim.x * (NT / T);
   int64_t r = (int64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
   Row<T, V> x, dy, nx, ndy;
-  if (AHEAD && r < a.R) {
-    nx.template load<true>(a.x + r * a.ldx, t, rest);
-    ndy.template load<true>(a.dy + r * a.lddy, t, rest);
-  }
-  for (; r < a.R; r += step) {
-    if (AHEAD) {
-      x = nx;
-      dy = ndy;
-      if (r + step < a.R) {
-        nx.template load<true>(a.x + (r + step) * a.ldx, t, rest);
-        ndy.template load<true>(a.dy + (r + step) * a.lddy, t, rest);
-      }
-    } else {
-      x.template load<true>(a.x + r * a.ldx, t, rest);
-      dy.template load<true>(a.dy + r * a.lddy, t, rest);
-    }
-    double s[1] = {0.0};
+  float x0, nx0 = 0.0f;
+  auto fetch = [&](int64_t row) {
+    nx0 = a.x[row * a.ldx];
+    nx.template load<LN_NT>(a.x + row * a.ldx, t, rest);
+    ndy.template load<LN_NT>(a.dy + row * a.lddy, t, rest);
+  };
+  if (AHEAD && r < a.R) fetch(r);
+  for (int turn = 0; r < a.R; r += step, turn ^= 1) {
+    if (!AHEAD) fetch(r);
+    x = nx;
+    dy = ndy;
+    x0 = nx0;
+    if (AHEAD && r + step < a.R) fetch(r + step);
+    double s[4] = {0.0, 0.0, 0.0, 0.0};  // sums of d, d^2, g, g d
 #pragma unroll
-    for (int i = 0; i < V; ++i)  // (0 behind the row's end)
-      s[0] += ((double)x.v[i].x + (double)x.v[i].y) + ((double)x.v[i].z + (double)x.v[i].w);
-    if constexpr (T < NT) s[0] = team_total<T>(s[0]);
-    else group_sum<NT, 1>(s, lds[0]);
-    const double mean = s[0] / (double)a.C;
-    forget(x.v);
-    double q[3] = {0.0, 0.0, 0.0};  // sums of d^2, g, g d with d = x - mean
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const double d = j < rest - 4 * T * i ? (double)at(x.v[i], j) - mean : 0.0;
+        const double d = (double)(j < rest - 4 * T * i ? at(x.v[i], j) : x0) - (double)x0;
         const double g = (double)at(dy.v[i], j) * (double)at(gm.v[i], j);
-        q[0] = fma(d, d, q[0]);
-        q[1] += g;
-        q[2] = fma(g, d, q[2]);
+        s[0] += d;
+        s[1] = fma(d, d, s[1]);
+        s[2] += g;
+        s[3] = fma(g, d, s[3]);
       }
-    }
-    if constexpr (T < NT) {
-#pragma unroll
-      for (int k = 0; k < 3; ++k) q[k] = team_total<T>(q[k]);
-    } else {
-      group_sum<NT, 3>(q, lds[1]);
-    }
-    const double rstd = 1.0 / sqrt(q[0] / (double)a.C + a.eps);
-    const double c1 = q[1] / (double)a.C, c2 = rstd * rstd * (q[2] / (double)a.C);
+    row_sums<NT, T>(s, lds[turn]);
+    const double delta = s[0] * a.inv_C, rstd = 1.0 / sqrt(variance(s[1] * a.inv_C, delta) + a.eps);
+    // dx = rstd (g - c1 - (d - delta) c2)
+    const double c1 = s[2] * a.inv_C, c2 = rstd * rstd * (fma(-delta, s[2], s[3]) * a.inv_C);
+    const double slope = -rstd * c2, offset = rstd * fma(delta, c2, -c1), shift = -delta * rstd;
     forget(x.v);
     forget(dy.v);
     float* dx = a.dx + r * a.lddx;
@@ -242,13 +229,12 @@ __device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[NT /
       float4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const double d = (double)at(x.v[i], j) - mean, v = (double)at(dy.v[i], j);
-        const double g = v * (double)at(gm.v[i], j);
-        at(o, j) = (float)(rstd * (fma(-d, c2, g) - c1));
-        dg[i][j] = fma(v, d * rstd, dg[i][j]);
+        const double d = (double)at(x.v[i], j) - (double)x0, v = (double)at(dy.v[i], j);
+        at(o, j) = (float)fma(d, slope, fma(v * (double)at(gm.v[i], j), rstd, offset));
+        dg[i][j] = fma(v, fma(d, rstd, shift), dg[i][j]);
         db[i][j] += v;
       }
-      st4_at<true>(dx, 16u * t + 16u * T * i, rest - 4 * T * i, o);
+      st4_at<LN_NT>(dx, 16u * t + 16u * T * i, rest - 4 * T * i, o);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -257,7 +243,7 @@ __device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[NT /
 // Four waves on each SIMD where a workgroup holds a row; a wave that holds one has up to 256 registers.
 template <int NT, int T, int V, bool AHEAD = true>
 __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(T == 64 ? 2 : 4))) ln_bwd(BwdArgs a) {
-  __shared__ double lds[4][NT / 64];
+  __shared__ double lds[2][4 * (NT / 64)];
   const int t = threadIdx.x % T;
   double dg[V][4], db[V][4];
   ln_bwd_rows<NT, T, V, AHEAD>(a, lds, dg, db);
@@ -315,8 +301,8 @@ __global__ void __launch_bounds__(LN_WIDE) ln_bwd_wide(BwdArgs a) {
         q[1] = fma(g, (double)at(xv, j) - mean, q[1]);
       }
     }
-    group_sum<LN_WIDE, 2>(q, lds[2]);
-    const double c1 = q[0] / (double)a.C, c2 = rstd * rstd * (q[1] / (double)a.C);
+    group_sums<LN_WIDE, 2>(q, lds[2]);
+    const double c1 = q[0] * a.inv_C, c2 = rstd * rstd * (q[1] * a.inv_C);
     float* dx = a.dx + r * a.lddx;
     for (int64_t c = 4 * threadIdx.x; c < a.C; c += 4 * LN_WIDE) {
       const float4 xv = ld4(x + c, a.C - c), v = ld4(dy + c, a.C - c);
@@ -383,6 +369,9 @@ __global__ void __launch_bounds__(512) ln_finish(const double* __restrict__ part
   }
 }
 
+#ifndef LN_G
+#define LN_G 512
+#endif
 constexpr int64_t LN_REGS = 16384;  // columns up to which a row is held in registers
 
 // Rows that a workgroup of the backward pass takes at once, and the workgroups.
@@ -396,7 +385,7 @@ BwdShape bwd_shape(int64_t R, int64_t C) {
     b.groups = std::min<int64_t>(R, 64);
   } else if (C > 1024) {
     b.rows = 1;
-    b.groups = std::min<int64_t>(R, 512);
+    b.groups = std::min<int64_t>(R, C <= 2048 ? LN_G : 512);
   } else {
     int64_t lanes = 2;
     while (lanes < 64 && 4 * lanes < C) lanes *= 2;
@@ -417,7 +406,7 @@ void launch_fwd(const FwdArgs& a, hipStream_t s) {
 
 hipError_t launch_layer_norm(const LayerNormParams& p, hipStream_t s) {
   if (p.R <= 0 || p.C <= 0) return hipSuccess;
-  const FwdArgs a{p.x, p.gamma, p.beta, p.y, p.R, p.C, p.ldx, p.ldy, (double)p.eps};
+  const FwdArgs a{p.x, p.gamma, p.beta, p.y, p.R, p.C, p.ldx, p.ldy, (double)p.eps, 1.0 / (double)p.C};
   if (p.C <= 8) launch_fwd<256, 2, 1>(a, s);
   else if (p.C <= 16) launch_fwd<256, 4, 1>(a, s);
   else if (p.C <= 32) launch_fwd<256, 8, 1>(a, s);
@@ -445,7 +434,7 @@ hipError_t launch_layer_norm_grad(const LayerNormGradParams& p, double* scratch,
   const bool sums = p.dgamma != nullptr || p.dbeta != nullptr;
   const BwdShape b = bwd_shape(p.R, p.C);
   BwdArgs a{p.dy, p.x, p.gamma, p.dx, sums ? scratch : nullptr, scratch + b.groups * 2 * p.C, p.R, p.C,
-            p.lddy, p.ldx, p.lddx, (double)p.eps};
+            p.lddy, p.ldx, p.lddx, (double)p.eps, 1.0 / (double)p.C};
   if (p.R > 0) {
     const dim3 g((unsigned)b.groups);
     if (p.C <= 8) hipLaunchKernelGGL((ln_bwd<256, 2, 1>), g, dim3(256), 0, s, a);
