@@ -20,6 +20,7 @@
 #include "fexp.h"
 #include "kernels.h"
 #include "rowvec.h"
+#include "wave_sum.h"
 
 namespace shk {
 namespace {
@@ -47,22 +48,23 @@ __device__ __forceinline__ bool entry_there(const DistillArgs& a, int64_t at) {
   const int64_t i = entry_index(a, at);
   return i >= 0 && i < a.C && a.t[at] != -INFINITY;
 }
-// Rows among [first, end) with an entry: thread i's are every NT-th.
+// Of this thread's rows among [first, end), every NT-th, those with an entry.
 template <int NT>
-__device__ __forceinline__ double count_rows(const DistillArgs& a, int64_t first, int64_t end, double* dl) {
+__device__ __forceinline__ double count_rows(const DistillArgs& a, int64_t first, int64_t end) {
   int64_t n = 0;
   for (int64_t r = first + threadIdx.x; r < end; r += NT) {
     bool there = false;
     for (int j = 0; j < a.K && !there; ++j) there = entry_there(a, r * a.K + j);
     n += there;
   }
-  return block_sum<NT>((double)n, dl);
+  return (double)n;
 }
 __global__ void __launch_bounds__(256) distill_count(DistillArgs a, uint32_t* count) {
-  __shared__ double dl[4];
+  __shared__ double lds[4];
   const int64_t part = (a.R + gridDim.x - 1) / gridDim.x, first = min(a.R, (int64_t)blockIdx.x * part);
-  const double n = count_rows<256>(a, first, min(a.R, first + part), dl);
-  if (threadIdx.x == 0) count[blockIdx.x] = (uint32_t)n;
+  double n[1] = {count_rows<256>(a, first, min(a.R, first + part))};
+  group_sums<256, 1>(n, lds);
+  if (threadIdx.x == 0) count[blockIdx.x] = (uint32_t)n[0];
 }
 
 // exp(x) for x <= 0: zero where the result is no normal number (a class of such a weight is 2^-126
@@ -72,29 +74,42 @@ __device__ __forceinline__ float exp_weight(float x) {
   return x != x ? x : x < -87.0f ? 0.0f : e;
 }
 
-template <int NT, int V>  // V == 0: the row does not fit, and is read again for each step
-__global__ void __launch_bounds__(NT) distill_rows(DistillArgs a) {
+__device__ __forceinline__ float4 weights(const float4& z, float m, float inv_T) {
+  return make_float4(exp_weight((z.x - m) * inv_T), exp_weight((z.y - m) * inv_T), exp_weight((z.z - m) * inv_T),
+                     exp_weight((z.w - m) * inv_T));
+}
+__device__ __forceinline__ double total(const float4& v) {
+  return ((double)v.x + (double)v.y) + ((double)v.z + (double)v.w);
+}
+__device__ __forceinline__ float largest(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+__device__ __forceinline__ float4 scaled(const float4& v, float inv, float scale) {
+  return make_float4((v.x * inv) * scale, (v.y * inv) * scale, (v.z * inv) * scale, (v.w * inv) * scale);
+}
+
+// A workgroup a row, V groups of four classes a thread. V == 0: the row does not fit; one reading forms
+// the largest logit and the sum about the largest so far, a second one the gradient. Four waves on
+// each SIMD in every form.
+template <int NT, int V>
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) distill_rows(DistillArgs a) {
   constexpr int NW = NT / 64;
   extern __shared__ double entries[];  // K: p; then K indexes
-  __shared__ double red[3][NW];
+  __shared__ double red[4 * NW];
   __shared__ float fm[2][NW];
   __shared__ int found[NW];
   int* index = reinterpret_cast<int*>(entries + a.K);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  float scale = 0.0f;
-  if (a.grad != nullptr) {
-    double n = 0.0;
-    if (a.count == nullptr) n = count_rows<NT>(a, 0, a.R, red[0]);
-    else
-      for (int i = 0; i < a.parts; ++i) n += (double)a.count[i];
-    scale = (float)(a.scale / n);
+  const bool counts = a.grad != nullptr && a.count == nullptr;  // the rows with an entry, beside the first row's sums
+  double n = -1.0;
+  if (a.grad != nullptr && a.count != nullptr) {
+    n = 0.0;
+    for (int i = 0; i < a.parts; ++i) n += (double)a.count[i];
   }
   const int C = (int)a.C;
   for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
     const float* row = a.z + r * a.C;
     float* out = a.grad != nullptr ? a.grad + r * a.C : nullptr;
     const RowGroups view(row, C);
-    // the entries: their number, the largest logit
+    // the entries: whether there are any, the largest logit
     __syncthreads();  // the last row's entries have been read
     int any = 0;
     float mt = -INFINITY;
@@ -108,12 +123,14 @@ __global__ void __launch_bounds__(NT) distill_rows(DistillArgs a) {
       any |= there;
       if (there) mt = fmaxf(mt, t);  // (a NaN makes the sums NaN)
     }
-    any = wave_or(any);
-    if (lane == 0) found[w] = any;
-    __syncthreads();
-    any = 0;
+    any = __any(any);
+    if (NW > 1) {
+      if (lane == 0) found[w] = any;
+      __syncthreads();
+      any = 0;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) any |= found[i];
+      for (int i = 0; i < NW; ++i) any |= found[i];
+    }
     if (!any) {
       if (threadIdx.x == 0) a.row_loss[r] = NO_LOSS;
       if (out != nullptr)
@@ -122,7 +139,8 @@ __global__ void __launch_bounds__(NT) distill_rows(DistillArgs a) {
     }
     // largest values
     float4 v[V > 0 ? V : 1];
-    float m = -INFINITY;
+    float m = -INFINITY, thread_m = -INFINITY;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};  // sums of exp(z - m), e = exp(t - mt), e (t - mt - z + m); the rows counted
     if constexpr (V > 0) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -130,42 +148,42 @@ __global__ void __launch_bounds__(NT) distill_rows(DistillArgs a) {
         v[i] = q < view.groups ? view.load(row, q, -INFINITY)
                                : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       }
+      if (counts && n < 0.0) s[3] = count_rows<NT>(a, 0, a.R);
 #pragma unroll
-      for (int i = 0; i < V; ++i) m = fmaxf(m, fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w)));
+      for (int i = 0; i < V; ++i) m = fmaxf(m, largest(v[i]));
     } else {
+      if (counts && n < 0.0) s[3] = count_rows<NT>(a, 0, a.R);
       for (int q = threadIdx.x; q < view.groups; q += NT) {
         const float4 x = view.load(row, q, -INFINITY);
-        m = fmaxf(m, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
+        const float top = fmaxf(m, largest(x));
+        if (top > m) {  // (the sum so far is zero where m is -inf)
+          s[0] *= (double)exp_weight((m - top) * a.inv_T);
+          m = top;
+        }
+        s[0] += total(weights(x, m, a.inv_T));
       }
+      thread_m = m;
     }
+    m = wave_largest(m);
+    mt = wave_largest(mt);
+    if (NW > 1) {
+      if (lane == 0) { fm[0][w] = m; fm[1][w] = mt; }
+      __syncthreads();
+      m = fm[0][0];
+      mt = fm[1][0];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      m = fmaxf(m, __shfl_xor(m, o, 64));
-      mt = fmaxf(mt, __shfl_xor(mt, o, 64));
+      for (int i = 1; i < NW; ++i) { m = fmaxf(m, fm[0][i]); mt = fmaxf(mt, fm[1][i]); }
     }
-    if (lane == 0) { fm[0][w] = m; fm[1][w] = mt; }
-    __syncthreads();
-    m = fm[0][0];
-    mt = fm[1][0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) { m = fmaxf(m, fm[0][i]); mt = fmaxf(mt, fm[1][i]); }
-    // sums: of exp(z - m), of e = exp(t - mt), of e (log p - log q) but for the sums' logarithms
-    double s[3] = {0.0, 0.0, 0.0};
     if constexpr (V > 0) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[i].x = exp_weight((v[i].x - m) * a.inv_T);
-        v[i].y = exp_weight((v[i].y - m) * a.inv_T);
-        v[i].z = exp_weight((v[i].z - m) * a.inv_T);
-        v[i].w = exp_weight((v[i].w - m) * a.inv_T);
-        s[0] += ((double)v[i].x + (double)v[i].y) + ((double)v[i].z + (double)v[i].w);
+        v[i] = weights(v[i], m, a.inv_T);
+        s[0] += total(v[i]);
+        __builtin_amdgcn_sched_barrier(0);  // four exponentials at a time keep the registers down
       }
-    } else {
-      for (int q = threadIdx.x; q < view.groups; q += NT) {
-        const float4 x = view.load(row, q, -INFINITY);
-        s[0] += ((double)exp_weight((x.x - m) * a.inv_T) + (double)exp_weight((x.y - m) * a.inv_T)) +
-                ((double)exp_weight((x.z - m) * a.inv_T) + (double)exp_weight((x.w - m) * a.inv_T));
-      }
+    } else if (thread_m != m) {
+      // a thread all of whose logits are -inf has summed NaN: its part is zero unless the row's largest is -inf
+      s[0] = thread_m == -INFINITY && m > -INFINITY ? 0.0 : s[0] * (double)exp_weight((thread_m - m) * a.inv_T);
     }
     for (int j = threadIdx.x; j < a.K; j += NT) {
       double e = 0.0;
@@ -178,41 +196,23 @@ __global__ void __launch_bounds__(NT) distill_rows(DistillArgs a) {
       }
       entries[j] = e;
     }
-#pragma unroll
-    for (int k = 0; k < 3; ++k) s[k] = wave_sum(s[k]);
-    if (lane == 0) {
-#pragma unroll
-      for (int k = 0; k < 3; ++k) red[k][w] = s[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      s[k] = red[k][0];
-#pragma unroll
-      for (int i = 1; i < NW; ++i) s[k] += red[k][i];
-    }
+    group_sums<NT, 4>(s, red);
+    if (counts && n < 0.0) n = s[3];
     if (threadIdx.x == 0) {
       const float loss = (float)(s[2] / s[1] - log(s[1]) + log(s[0]));
       a.row_loss[r] = loss == 0.0f ? 0.0f : loss;
     }
     if (out == nullptr) continue;
-    const float inv = (float)(1.0 / s[0]);
+    const float inv = (float)(1.0 / s[0]), scale = (float)(a.scale / n);
     if constexpr (V > 0) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int q = threadIdx.x + i * NT;
-        if (q < view.groups)
-          view.store(out, q, make_float4((v[i].x * inv) * scale, (v[i].y * inv) * scale, (v[i].z * inv) * scale,
-                                         (v[i].w * inv) * scale));
+        if (q < view.groups) view.store(out, q, scaled(v[i], inv, scale));
       }
     } else {
-      for (int q = threadIdx.x; q < view.groups; q += NT) {
-        const float4 x = view.load(row, q, -INFINITY);
-        view.store(out, q, make_float4((exp_weight((x.x - m) * a.inv_T) * inv) * scale,
-                                       (exp_weight((x.y - m) * a.inv_T) * inv) * scale,
-                                       (exp_weight((x.z - m) * a.inv_T) * inv) * scale,
-                                       (exp_weight((x.w - m) * a.inv_T) * inv) * scale));
-      }
+      for (int q = threadIdx.x; q < view.groups; q += NT)
+        view.store(out, q, scaled(weights(view.load(row, q, -INFINITY), m, a.inv_T), inv, scale));
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above precede those below
     __syncthreads();
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(NT) distill_rows(DistillArgs a) {
 // The loss: binary64 sum of the row losses, over the number of rows that have one.
 __global__ void __launch_bounds__(1024) distill_finish(const float* __restrict__ row_loss, int64_t R, double T2,
                                                        float* loss) {
-  __shared__ double ds[16], dn[16];
+  __shared__ double lds[2][16];
   double s = 0.0, n = 0.0;
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < R; i += 1024) {
@@ -238,19 +238,9 @@ __global__ void __launch_bounds__(1024) distill_finish(const float* __restrict__
     s += (double)v;
     n += __float_as_uint(v) == 0x80000000u ? 0.0 : 1.0;
   }
-  s = wave_sum(s);
-  n = wave_sum(n);
-  if ((threadIdx.x & 63) == 0) {
-    ds[threadIdx.x >> 6] = s;
-    dn[threadIdx.x >> 6] = n;
-  }
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int i = 1; i < 16; ++i) {
-    s += ds[i];
-    n += dn[i];
-  }
-  loss[0] = (float)(s * T2 / n);
+  double v[2] = {s, n};
+  group_sums<1024, 2>(v, &lds[0][0]);
+  if (threadIdx.x == 0) loss[0] = (float)(v[0] * T2 / v[1]);
 }
 
 constexpr int64_t COUNT_ROWS = 1024;  // rows that each workgroup counts by itself
@@ -287,7 +277,8 @@ hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* statu
     a.count = count;
     a.parts = COUNT_PARTS;
   }
-  if (p.C <= 256 * 4 - 4) launch_rows<256, 1>(a, s);
+  if (p.C <= 64 * 4 - 4) launch_rows<64, 1>(a, s);
+  else if (p.C <= 64 * 4 * 4 - 4) launch_rows<64, 4>(a, s);
   else if (p.C <= 256 * 4 * 4 - 4) launch_rows<256, 4>(a, s);
   else if (p.C <= 256 * 4 * 8 - 4) launch_rows<256, 8>(a, s);
   else if (p.C <= 512 * 4 * 8 - 4) launch_rows<512, 8>(a, s);

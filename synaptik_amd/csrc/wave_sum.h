@@ -3,6 +3,8 @@
 // formed together: each of the first steps halves the values that a lane still adds up, so that four
 // sums over 64 lanes take 7 additions instead of 24. The order is fixed.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace shk {
@@ -72,6 +74,21 @@ __device__ __forceinline__ double wave_sums(const double (&v)[K]) {
     const double keep = high ? b : a, give = high ? a : b;
     return add_lanes<4, 64>(keep + dpp_get<DPP_XOR2>(give));
   }
+}
+
+// The largest value over 64 lanes, the same in every lane; NaN counts as absent. All lanes are active.
+__device__ __forceinline__ float wave_largest(float v) {
+  const auto other = [&](auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v = fmaxf(v, other(std::integral_constant<int, DPP_XOR1>()));
+  v = fmaxf(v, other(std::integral_constant<int, DPP_XOR2>()));
+  v = fmaxf(v, other(std::integral_constant<int, DPP_MIRROR8>()));
+  v = fmaxf(v, other(std::integral_constant<int, DPP_MIRROR16>()));
+  const auto row = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  v = fmaxf(__int_as_float(row[0]), __int_as_float(row[1]));
+  const auto half = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return fmaxf(__int_as_float(half[0]), __int_as_float(half[1]));
 }
 
 // Sums of K values over a workgroup of NT threads, the same in every thread; `lds`: K NT / 64 doubles,
