@@ -19,6 +19,7 @@
 #include "common.h"
 #include "fexp.h"
 #include "kernels.h"
+#include "row4.h"
 #include "rowvec.h"
 #include "wave_sum.h"
 
@@ -86,6 +87,29 @@ __device__ __forceinline__ float4 scaled(const float4& v, float inv, float scale
   return make_float4((v.x * inv) * scale, (v.y * inv) * scale, (v.z * inv) * scale, (v.w * inv) * scale);
 }
 
+// The V = ceil(C / 4 NT) groups of four classes of a row of C >= 4 that a thread holds, NT groups apart:
+// all but the last lie within the row for every thread; the last is there for some (`mine`), and
+// begins at C - 4 at the latest, so that the row's last group overlaps the one before where C is no
+// multiple of four. Both hold the same results for the classes they share, which count in sums once.
+template <int NT, int V>
+struct RowOf {
+  int over;  // classes of the last group that the one before has too
+  bool mine;
+  uint32_t end;    // byte offsets
+  __device__ __forceinline__ RowOf(int C) {
+    const int c = 4 * ((int)threadIdx.x + (V - 1) * NT);
+    mine = c < C;
+    over = max(0, c - (C - 4));
+    end = 4u * (uint32_t)min(c, C - 4);
+  }
+  __device__ __forceinline__ uint32_t at(int i) const { return 16u * (threadIdx.x + (uint32_t)(i * NT)); }
+  // The sum of what the last group has alone (its classes weigh nothing where it is not this thread's).
+  __device__ __forceinline__ double new_part(const float4& v) const {
+    return ((over < 1 ? (double)v.x : 0.0) + (over < 2 ? (double)v.y : 0.0)) +
+           ((over < 3 ? (double)v.z : 0.0) + (over < 4 ? (double)v.w : 0.0));
+  }
+};
+
 // A workgroup a row, V groups of four classes a thread. V == 0: the row does not fit; one reading forms
 // the largest logit and the sum about the largest so far, a second one the gradient. Four waves on
 // each SIMD in every form.
@@ -138,15 +162,15 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
       continue;
     }
     // largest values
+    const RowOf<NT, V> in(C);
     float4 v[V > 0 ? V : 1];
     float m = -INFINITY, thread_m = -INFINITY;
     double s[4] = {0.0, 0.0, 0.0, 0.0};  // sums of exp(z - m), e = exp(t - mt), e (t - mt - z + m); the rows counted
     if constexpr (V > 0) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int q = threadIdx.x + i * NT;
-        v[i] = q < view.groups ? view.load(row, q, -INFINITY)
-                               : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (i < V - 1) v[i] = ld4_at<true>(row, in.at(i), 4);
+        else v[i] = in.mine ? ld4_at<true>(row, in.end, 4) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       }
       if (counts && n < 0.0) s[3] = count_rows<NT>(a, 0, a.R);
 #pragma unroll
@@ -178,7 +202,7 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         v[i] = weights(v[i], m, a.inv_T);
-        s[0] += total(v[i]);
+        s[0] += i < V - 1 ? total(v[i]) : in.new_part(v[i]);
         __builtin_amdgcn_sched_barrier(0);  // four exponentials at a time keep the registers down
       }
     } else if (thread_m != m) {
@@ -207,8 +231,8 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
     if constexpr (V > 0) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int q = threadIdx.x + i * NT;
-        if (q < view.groups) view.store(out, q, scaled(v[i], inv, scale));
+        if (i < V - 1) st4_at<true>(out, in.at(i), 4, scaled(v[i], inv, scale));
+        else if (in.mine) st4_at<true>(out, in.end, 4, scaled(v[i], inv, scale));
       }
     } else {
       for (int q = threadIdx.x; q < view.groups; q += NT)
@@ -251,6 +275,15 @@ void launch_rows(const DistillArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((distill_rows<NT, V>), dim3((unsigned)std::min<int64_t>(a.R, 1 << 20)), dim3(NT), 12 * a.K, s, a);
 }
 
+// V groups a thread, from V to MOST by the row's width.
+template <int NT, int V, int MOST>
+void launch_groups(const DistillArgs& a, hipStream_t s) {
+  if constexpr (V < MOST) {
+    if (a.C > 4 * NT * V) return launch_groups<NT, V + 1, MOST>(a, s);
+  }
+  launch_rows<NT, V>(a, s);
+}
+
 }  // namespace
 
 int64_t distill_scratch_bytes(int64_t R) { return 4 * ((R + 3) / 4 * 4) + 4 * COUNT_PARTS; }
@@ -277,13 +310,13 @@ hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* statu
     a.count = count;
     a.parts = COUNT_PARTS;
   }
-  if (p.C <= 64 * 4 - 4) launch_rows<64, 1>(a, s);
-  else if (p.C <= 64 * 4 * 4 - 4) launch_rows<64, 4>(a, s);
-  else if (p.C <= 256 * 4 * 4 - 4) launch_rows<256, 4>(a, s);
-  else if (p.C <= 256 * 4 * 8 - 4) launch_rows<256, 8>(a, s);
-  else if (p.C <= 512 * 4 * 8 - 4) launch_rows<512, 8>(a, s);
-  else if (p.C <= 512 * 4 * 16 - 4) launch_rows<512, 16>(a, s);
-  else if (p.C <= 1024 * 4 * 16 - 4) launch_rows<1024, 16>(a, s);
+  // The smallest workgroup that holds the row in at most 16 groups (64 registers) a thread, or 8 up to
+  // 8192 classes: more waves for the row's latency.
+  if (p.C < 4) launch_rows<64, 0>(a, s);
+  else if (p.C <= 64 * 4 * 4) launch_groups<64, 1, 4>(a, s);
+  else if (p.C <= 256 * 4 * 8) launch_groups<256, 2, 8>(a, s);
+  else if (p.C <= 512 * 4 * 16) launch_groups<512, 5, 16>(a, s);
+  else if (p.C <= 1024 * 4 * 16) launch_groups<1024, 9, 16>(a, s);
   else launch_rows<1024, 0>(a, s);
   hipLaunchKernelGGL(distill_finish, dim3(1), dim3(1024), 0, s, (const float*)a.row_loss, p.R,
                      (double)p.T * (double)p.T, p.loss);
