@@ -49,23 +49,46 @@ __device__ __forceinline__ bool entry_there(const DistillArgs& a, int64_t at) {
   const int64_t i = entry_index(a, at);
   return i >= 0 && i < a.C && a.t[at] != -INFINITY;
 }
-// Of this thread's rows among [first, end), every NT-th, those with an entry.
+// Rows with an entry that this thread finds among all of them, R at most COUNT_ROWS: the entries are read
+// in order, each that is there marks its row, and the marks are counted. `marks` is read and written by
+// the whole workgroup, with barriers.
+constexpr int COUNT_ROWS = 1024, COUNT_ENTRIES = 1 << 14;
 template <int NT>
-__device__ __forceinline__ double count_rows(const DistillArgs& a, int64_t first, int64_t end) {
-  int64_t n = 0;
-  for (int64_t r = first + threadIdx.x; r < end; r += NT) {
-    bool there = false;
-    for (int j = 0; j < a.K && !there; ++j) there = entry_there(a, r * a.K + j);
-    n += there;
-  }
+__device__ __forceinline__ double count_rows(const DistillArgs& a, uint8_t* marks) {
+  const uint32_t R = (uint32_t)a.R, total = R * (uint32_t)a.K;
+  const uint32_t inv = (uint32_t)((0x100000000ull + a.K - 1) / a.K);  // ceil(2^32 / K): e / K exactly below 2^22
+  for (uint32_t r = threadIdx.x; r < R; r += NT) marks[r] = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (uint32_t e = threadIdx.x; e < total; e += NT)
+    if (entry_there(a, e)) marks[a.K == 1 ? e : __umulhi(e, inv)] = 1;
+  __syncthreads();
+  int n = 0;
+  for (uint32_t r = threadIdx.x; r < R; r += NT) n += marks[r];
   return (double)n;
 }
-__global__ void __launch_bounds__(256) distill_count(DistillArgs a, uint32_t* count) {
-  __shared__ double lds[4];
+// Rows with an entry of each of the launch's parts of the rows: a wave reads a row's entries at once.
+__global__ void __launch_bounds__(1024) distill_count(DistillArgs a, uint32_t* count) {
+  __shared__ uint32_t found[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t part = (a.R + gridDim.x - 1) / gridDim.x, first = min(a.R, (int64_t)blockIdx.x * part);
-  double n[1] = {count_rows<256>(a, first, min(a.R, first + part))};
-  group_sums<256, 1>(n, lds);
-  if (threadIdx.x == 0) count[blockIdx.x] = (uint32_t)n[0];
+  const int64_t end = min(a.R, first + part);
+  uint32_t n = 0;
+  for (int64_t r = first + w; r < end; r += 64) {
+    bool there[4] = {false, false, false, false};
+    for (int j = lane; j < a.K; j += 64) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) there[u] |= r + 16 * u < end && entry_there(a, (r + 16 * u) * a.K + j);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) n += __any(there[u]) ? 1u : 0u;
+  }
+  if (lane == 0) found[w] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) n += found[i];
+    count[blockIdx.x] = n;
+  }
 }
 
 // exp(x) for x <= 0: zero where the result is no normal number (a class of such a weight is 2^-126
@@ -120,6 +143,7 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
   __shared__ double red[4 * NW];
   __shared__ float fm[2][NW];
   __shared__ int found[NW];
+  __shared__ uint8_t marks[COUNT_ROWS];
   int* index = reinterpret_cast<int*>(entries + a.K);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const bool counts = a.grad != nullptr && a.count == nullptr;  // the rows with an entry, beside the first row's sums
@@ -172,11 +196,11 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
         if (i < V - 1) v[i] = ld4_at<true>(row, in.at(i), 4);
         else v[i] = in.mine ? ld4_at<true>(row, in.end, 4) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       }
-      if (counts && n < 0.0) s[3] = count_rows<NT>(a, 0, a.R);
+      if (counts && n < 0.0) s[3] = count_rows<NT>(a, marks);
 #pragma unroll
       for (int i = 0; i < V; ++i) m = fmaxf(m, largest(v[i]));
     } else {
-      if (counts && n < 0.0) s[3] = count_rows<NT>(a, 0, a.R);
+      if (counts && n < 0.0) s[3] = count_rows<NT>(a, marks);
       for (int q = threadIdx.x; q < view.groups; q += NT) {
         const float4 x = view.load(row, q, -INFINITY);
         const float top = fmaxf(m, largest(x));
@@ -267,7 +291,6 @@ __global__ void __launch_bounds__(1024) distill_finish(const float* __restrict__
   if (threadIdx.x == 0) loss[0] = (float)(v[0] * T2 / v[1]);
 }
 
-constexpr int64_t COUNT_ROWS = 1024;  // rows that each workgroup counts by itself
 constexpr int COUNT_PARTS = 64;
 
 template <int NT, int V>
@@ -304,9 +327,9 @@ hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* statu
   a.inv_T = (float)(1.0 / (double)p.T);
   a.inv_T64 = 1.0 / (double)p.T;
   a.scale = (double)p.g * (double)p.T;
-  if (p.grad != nullptr && p.R > COUNT_ROWS) {
+  if (p.grad != nullptr && (p.R > COUNT_ROWS || p.R * p.K > COUNT_ENTRIES)) {
     uint32_t* count = reinterpret_cast<uint32_t*>(a.row_loss + (p.R + 3) / 4 * 4);
-    hipLaunchKernelGGL(distill_count, dim3(COUNT_PARTS), dim3(256), 0, s, a, count);
+    hipLaunchKernelGGL(distill_count, dim3(COUNT_PARTS), dim3(1024), 0, s, a, count);
     a.count = count;
     a.parts = COUNT_PARTS;
   }

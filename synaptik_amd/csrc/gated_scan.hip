@@ -10,8 +10,8 @@
 // take TS consecutive positions each, form their runs' steps, read each other's from LDS, and
 // carry on from their own first state: one pass over the data, whose positions' gates stay in
 // registers. Where there are too few channels for the CUs, the positions are cut into chunks: a
-// launch forms the chunks' steps, a second carries the state through them, a third is the pass
-// above from each chunk's first state.
+// launch forms the chunks' steps, a second joins those before each chunk and is the pass above from
+// there.
 //
 // States and products are binary32, as the outputs are; a gate and its complement come from one
 // binary64 exponential, so that 1 - f keeps its bits where f is near one. A sequence shorter than T
@@ -69,9 +69,8 @@ struct ScanArgs {
   float* last;          // [B, D]: the state behind the last step; null: not wanted
   const void* lengths;  // [B]; null: all T
   uint32_t* status;
-  float* step_f;        // [chunks][B D]: the chunks' steps, and their first states
-  float* step_b;
-  float* state;
+  float2* step;         // [chunks][B D]: the chunks' steps
+  float* state;         // [B D]: a copy of the first states
   int64_t B, T, D, chunk, chunks;  // chunk: positions of one; chunks > 1: split
   int64_t waves, parts;  // groups of up to 64 channels: of all sequences, of one
   int pack, lanes;       // sequences a wave takes, lanes of each
@@ -98,7 +97,9 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
   const int64_t width = a.T * a.D;  // floats of a sequence
   const int64_t blocks = (a.waves + CW - 1) / CW;
   for (int64_t unit = blockIdx.x; unit < blocks * a.chunks; unit += gridDim.x) {
-    const int64_t piece = unit / blocks, wave = (unit % blocks) * CW + (CW > 1 ? w : 0);
+    // (the chunks' second reading begins with those that the first one read last)
+    const int64_t piece = MODE == CHUNK ? a.chunks - 1 - unit / blocks : unit / blocks;
+    const int64_t wave = (unit % blocks) * CW + (CW > 1 ? w : 0);
     // this wave's channels: 64 of one sequence, or those of `pack` short ones
     const int64_t first_seq = wave / a.parts * a.pack, part = wave % a.parts;
     const int sub = a.pack > 1 ? lane / a.lanes : 0, c = (int)part * 64 + (a.pack > 1 ? lane % a.lanes : lane);
@@ -120,11 +121,11 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
       __builtin_nontemporal_store(v, reinterpret_cast<float*>(reinterpret_cast<char*>(x) + at));
     };
     const float* const src[4] = {a.z, BACK ? a.dh : a.u, a.u, a.h};
+    // steps p0 .. p0 + TS - 1 are positions of every lane's sequence in this piece
+    auto whole = [&](int p0) { return p0 + TS <= hi && __all(!live || (from <= p0 && p0 + TS <= to)); };
     float next[READS][TS];
     auto load = [&](int p0) {
-      // (behind step p0 + TS - 1 lies the position whose state is read with the last)
-      const bool whole = p0 + TS <= (BACK ? min(hi, T - 1) : hi) && __all(!live || (from <= p0 && p0 + TS <= to));
-      if (whole) {
+      if (whole(p0) && (READS < 4 || p0 + TS < T)) {  // (before position 0 there is h0)
         if (live) {
 #pragma unroll
           for (int r = 0; r < READS; ++r) {
@@ -152,26 +153,51 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
 
     float state = 0.0f, all = 1.0f;
     if (MODE == WHOLE) state = a.first != nullptr ? a.first[n] : 0.0f;
-    if (MODE == CHUNK) state = a.state[piece * a.B * a.D + n];
     load(lo + tw * TS);
     int turn = 0;
+    if (MODE == CHUNK) {
+      // the steps of the chunks before: each wave joins consecutive ones, all join the waves'
+      state = a.state[n];
+      const int64_t share = (piece + NW - 1) / NW, end = min(piece, (tw + 1) * share);
+      float run_f = 1.0f, run_b = 0.0f;
+#pragma unroll 8
+      for (int64_t i = min(piece, tw * share); i < end; ++i) {
+        const float2 g = a.step[i * a.B * a.D + n];
+        run_b = fmaf(g.x, run_b, g.y);
+        run_f *= g.x;
+      }
+      steps[turn][w][lane] = make_float2(run_f, run_b);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NW; ++j) {
+        const float2 g = steps[turn][j][lane];
+        state = fmaf(g.x, state, g.y);
+      }
+      turn ^= 1;
+    }
     for (int p0 = lo; p0 < hi; p0 += NW * TS, turn ^= 1) {
       const int q0 = p0 + tw * TS;
       float f[TS], b[TS], k[TS], v[TS], m[TS];
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
         gates(next[0][i], f[i], k[i]);
-        const bool in = q0 + i < hi && q0 + i >= from && q0 + i < to;
         if (BACK) {
           v[i] = next[1][i];
-          if (MODE != STEPS) m[i] = in ? (next[3][i] - next[2][i]) * (f[i] * k[i]) : 0.0f;
-          k[i] = in ? k[i] : 0.0f;
-          v[i] = in ? v[i] : 0.0f;
+          if (MODE != STEPS) m[i] = (next[3][i] - next[2][i]) * (f[i] * k[i]);
         } else {
-          b[i] = in ? k[i] * next[1][i] : 0.0f;
+          b[i] = k[i] * next[1][i];
         }
-        f[i] = in ? f[i] : 1.0f;
         __builtin_amdgcn_sched_barrier(0);  // one gate's binary64 values at a time
+      }
+      if (!whole(q0)) {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
+          const bool in = q0 + i < hi && q0 + i >= from && q0 + i < to;
+          f[i] = in ? f[i] : 1.0f;
+          if (!BACK) b[i] = in ? b[i] : 0.0f;
+          else if (MODE != STEPS) m[i] = in ? m[i] : 0.0f;
+          if (BACK) { k[i] = in ? k[i] : 0.0f; v[i] = in ? v[i] : 0.0f; }
+        }
       }
       if (p0 + NW * TS < hi) load(q0 + NW * TS);
       float s = state;
@@ -216,27 +242,14 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
       if (NW == 1 && MODE != STEPS) state = s;
     }
     if (tw == 0 && live) {
-      if (MODE == WHOLE && a.last != nullptr) a.last[n] = state;
       if (MODE == STEPS) {
-        a.step_f[piece * a.B * a.D + n] = all;
-        a.step_b[piece * a.B * a.D + n] = state;
+        a.step[piece * a.B * a.D + n] = make_float2(all, state);
+        if (piece == 0) a.state[n] = a.first != nullptr ? a.first[n] : 0.0f;
+      } else if (piece == a.chunks - 1 && a.last != nullptr) {
+        a.last[n] = state;  // (which may be `first`: the chunks read its copy)
       }
     }
     if (NW > 1) __syncthreads();  // the steps in LDS have been read
-  }
-}
-
-// The state before each chunk, and behind the last.
-__global__ void __launch_bounds__(64) scan_carry(ScanArgs a) {
-  const int64_t channels = a.B * a.D;
-  for (int64_t n = (int64_t)blockIdx.x * 64 + threadIdx.x; n < channels; n += (int64_t)gridDim.x * 64) {
-    float state = a.first != nullptr ? a.first[n] : 0.0f;
-#pragma unroll 8
-    for (int64_t i = 0; i < a.chunks; ++i) {
-      a.state[i * channels + n] = state;
-      state = fmaf(a.step_f[i * channels + n], state, a.step_b[i * channels + n]);
-    }
-    if (a.last != nullptr) a.last[n] = state;
   }
 }
 
@@ -251,13 +264,16 @@ int64_t scan_waves(int64_t B, int64_t T, int64_t D) {
   const int64_t pack = 64 / scan_lanes(B, T, D);
   return (B + pack - 1) / pack * ((D + 63) / 64);
 }
+#ifndef SCAN_WHOLE
+#define SCAN_WHOLE 256
+#endif
 // Positions of a chunk: all of them where the channels fill the CUs or there is little to split.
-constexpr int64_t SCAN_GROUPS = 512, SCAN_LEAST = 512;
+constexpr int64_t SCAN_GROUPS = 1024, SCAN_LEAST = 128, SCAN_TILE = 64;
 int64_t scan_chunk(int64_t B, int64_t T, int64_t D) {
   const int64_t groups = scan_waves(B, T, D);
-  if (groups >= SCAN_GROUPS / 2 || T < 2 * SCAN_LEAST) return T;
+  if (groups >= SCAN_WHOLE || T < 2 * SCAN_LEAST) return T;
   const int64_t chunks = std::min(T / SCAN_LEAST, (SCAN_GROUPS + groups - 1) / groups);
-  return chunks <= 1 ? T : ((T + chunks - 1) / chunks + 255) / 256 * 256;
+  return chunks <= 1 ? T : ((T + chunks - 1) / chunks + SCAN_TILE - 1) / SCAN_TILE * SCAN_TILE;
 }
 
 template <bool BACK>
@@ -274,12 +290,10 @@ hipError_t launch_scan(ScanArgs a, float* scratch, hipStream_t s) {
   a.chunk = std::max<int64_t>(1, scan_chunk(a.B, a.T, a.D));
   a.chunks = std::max<int64_t>(1, (a.T + a.chunk - 1) / a.chunk);
   if (a.chunks > 1) {
-    a.step_f = scratch;
-    a.step_b = scratch + a.chunks * channels;
+    a.step = reinterpret_cast<float2*>(scratch);
     a.state = scratch + 2 * a.chunks * channels;
-    hipLaunchKernelGGL((scan_kernel<BACK, STEPS, 16, 1, TS>), blocks(1), dim3(1024), 0, s, a);
-    hipLaunchKernelGGL(scan_carry, dim3((unsigned)((channels + 63) / 64)), dim3(64), 0, s, a);
-    hipLaunchKernelGGL((scan_kernel<BACK, CHUNK, 16, 1, TS>), blocks(1), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((scan_kernel<BACK, STEPS, 8, 1, TS>), blocks(1), dim3(512), 0, s, a);
+    hipLaunchKernelGGL((scan_kernel<BACK, CHUNK, 8, 1, TS>), blocks(1), dim3(512), 0, s, a);
   } else if (a.T <= 8) {
     hipLaunchKernelGGL((scan_kernel<BACK, WHOLE, 1, 4, 4>), blocks(4), dim3(256), 0, s, a);
   } else if (a.T <= 8 * TS) {
@@ -295,7 +309,7 @@ hipError_t launch_scan(ScanArgs a, float* scratch, hipStream_t s) {
 int64_t gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D) {
   if (B <= 0 || T <= 0 || D <= 0) return 0;
   const int64_t chunk = scan_chunk(B, T, D), chunks = (T + chunk - 1) / chunk;
-  return chunks > 1 ? 12 * chunks * B * D : 0;
+  return chunks > 1 ? 4 * (2 * chunks + 1) * B * D : 0;
 }
 
 hipError_t launch_gated_scan(const GatedScanParams& p, float* scratch, uint32_t* status, hipStream_t s) {
