@@ -77,10 +77,10 @@ void launch_rows(const Tokens& t, const float* w, float* y, int64_t D, int64_t l
 
 // ---- sorting ----
 constexpr int EG_BITS = 9, EG_BINS = 1 << EG_BITS;
-constexpr int EG_KEYS = 16;                    // keys a thread
-constexpr int EG_SORT = 256 * EG_KEYS;         // keys a workgroup
+constexpr int EG_KEYS = 4;                     // keys a thread
+constexpr int EG_SORT = 1024 * EG_KEYS;        // keys a workgroup
 constexpr int64_t EG_SCAN_TILES = 64;          // up to here a workgroup adds the others' counts itself
-constexpr int EG_SMALL_KEYS = 4, EG_SMALL = 1024 * EG_SMALL_KEYS;  // keys that one workgroup sorts
+constexpr int EG_SMALL_KEYS = 8, EG_SMALL = 1024 * EG_SMALL_KEYS;  // keys that one workgroup sorts
 constexpr int EG_TILE = 32;                    // sorted rows a wave sums
 
 // Among the wave's active lanes: those whose digit is this lane's.
@@ -207,22 +207,22 @@ __global__ void __launch_bounds__(1024) eg_sort_small(Tokens t, int passes, uint
 }
 
 // Digit counts of each EG_SORT keys: count[tile][bin]. The first pass reads the tokens.
-__global__ void __launch_bounds__(256) eg_count(Tokens t, const uint32_t* __restrict__ keys, int shift,
+__global__ void __launch_bounds__(1024) eg_count(Tokens t, const uint32_t* __restrict__ keys, int shift,
                                                 uint32_t* __restrict__ count) {
   __shared__ uint32_t h[4][EG_BINS];
-  for (int i = threadIdx.x; i < 4 * EG_BINS; i += 256) (&h[0][0])[i] = 0;
+  for (int i = threadIdx.x; i < 4 * EG_BINS; i += 1024) (&h[0][0])[i] = 0;
   __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * EG_SORT;
-#pragma unroll 4
+#pragma unroll
   for (int i = 0; i < EG_KEYS; ++i) {
-    const int64_t n = first + i * 256 + threadIdx.x;
+    const int64_t n = first + i * 1024 + threadIdx.x;
     if (n < t.N) {
       const uint32_t key = keys != nullptr ? keys[n] : t.key(n, true);
-      atomicAdd(&h[threadIdx.x >> 6][(key >> shift) & (EG_BINS - 1)], 1u);
+      atomicAdd(&h[(threadIdx.x >> 6) & 3][(key >> shift) & (EG_BINS - 1)], 1u);
     }
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < EG_BINS; b += 256)
+  for (int b = threadIdx.x; b < EG_BINS; b += 1024)
     count[(int64_t)blockIdx.x * EG_BINS + b] = (h[0][b] + h[1][b]) + (h[2][b] + h[3][b]);
 }
 
@@ -248,56 +248,53 @@ __global__ void __launch_bounds__(256) eg_scan(uint32_t* __restrict__ count, int
 }
 
 // Moves each key and its row to its place by one digit.
-__global__ void __launch_bounds__(256) eg_scatter(Tokens t, const uint32_t* __restrict__ keys,
+__global__ void __launch_bounds__(1024) eg_scatter(Tokens t, const uint32_t* __restrict__ keys,
                                                   const uint32_t* __restrict__ rows, int shift,
                                                   const uint32_t* __restrict__ count, int64_t tiles,
                                                   uint32_t* __restrict__ keys_out, uint32_t* __restrict__ rows_out) {
-  constexpr int K = EG_KEYS;
-  __shared__ uint32_t h[4][EG_BINS];
+  constexpr int K = EG_KEYS, NW = 16;
+  __shared__ uint32_t h[NW][EG_BINS];
   __shared__ uint32_t base[EG_BINS], before[EG_BINS];
   __shared__ uint32_t sums[EG_BINS / 128];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t first = (int64_t)blockIdx.x * EG_SORT + w * 64 * K + lane;
-  uint32_t key[K], digit[K], rank[K];
+  uint32_t key[K], row[K], digit[K], rank[K];
   bool active[K];
 #pragma unroll
   for (int i = 0; i < K; ++i) {
     const int64_t n = first + i * 64;
     active[i] = n < t.N;
     key[i] = !active[i] ? 0u : keys != nullptr ? keys[n] : t.key(n, false);
+    row[i] = !active[i] ? 0u : rows != nullptr ? rows[n] : (uint32_t)n;
     digit[i] = (key[i] >> shift) & (EG_BINS - 1);
   }
-  for (int i = threadIdx.x; i < 4 * EG_BINS; i += 256) (&h[0][0])[i] = 0;
-  if (tiles <= EG_SCAN_TILES) {
-    uint32_t all[2] = {0, 0}, mine[2] = {0, 0};
+  for (int i = threadIdx.x; i < NW * EG_BINS; i += 1024) (&h[0][0])[i] = 0;
+  if (threadIdx.x < EG_BINS) {
+    const uint32_t* c = count + threadIdx.x;
+    uint32_t all = 0, mine = 0;
+    if (tiles <= EG_SCAN_TILES) {
 #pragma unroll 8
-    for (int64_t i = 0; i < tiles; ++i) {
-      const uint32_t* c = count + i * EG_BINS + threadIdx.x;
-      const uint32_t a = c[0], b = c[256];
-      all[0] += a;
-      all[1] += b;
-      mine[0] += i < blockIdx.x ? a : 0u;
-      mine[1] += i < blockIdx.x ? b : 0u;
+      for (int64_t i = 0; i < tiles; ++i) {
+        const uint32_t v = c[i * EG_BINS];
+        all += v;
+        mine += i < blockIdx.x ? v : 0u;
+      }
+    } else {
+      all = c[tiles * EG_BINS];
+      mine = c[(int64_t)blockIdx.x * EG_BINS];
     }
-    for (int j = 0; j < 2; ++j) {
-      base[threadIdx.x + 256 * j] = all[j];
-      before[threadIdx.x + 256 * j] = mine[j];
-    }
-  } else {
-    for (int b = threadIdx.x; b < EG_BINS; b += 256) {
-      base[b] = count[tiles * EG_BINS + b];
-      before[b] = count[(int64_t)blockIdx.x * EG_BINS + b];
-    }
+    base[threadIdx.x] = all;
+    before[threadIdx.x] = mine;
   }
   __syncthreads();
-  scan_bins<256>(base, sums);
   wave_ranks<K>(digit, active, h[w], rank);
-  __syncthreads();
-  for (int b = threadIdx.x; b < EG_BINS; b += 256) {
-    uint32_t run = base[b] + before[b];
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t c = h[i][b];
-      h[i][b] = run;
+  scan_bins<1024>(base, sums);
+  if (threadIdx.x < EG_BINS) {
+    uint32_t run = base[threadIdx.x] + before[threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const uint32_t c = h[i][threadIdx.x];
+      h[i][threadIdx.x] = run;
       run += c;
     }
   }
@@ -307,7 +304,7 @@ __global__ void __launch_bounds__(256) eg_scatter(Tokens t, const uint32_t* __re
     if (active[i]) {
       const uint32_t to = h[w][digit[i]] + rank[i];
       keys_out[to] = key[i];
-      rows_out[to] = rows != nullptr ? rows[first + i * 64] : (uint32_t)(first + i * 64);
+      rows_out[to] = row[i];
     }
   }
 }
@@ -452,10 +449,19 @@ __global__ void __launch_bounds__(256) eg_join(SumArgs a) {
       for (int j = 0; j < 4; ++j)
         if (c + j < a.D) acc[j] = a.part[(2 * tile + 1) * a.D + c + j];
     }
-    for (int64_t i = from; i < to; ++i) {
+    constexpr int U = 8;
+    for (int64_t i0 = from; i0 < to; i0 += U) {
+      double v[U][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c + j < a.D) acc[j] += a.part[2 * i * a.D + c + j];
+      for (int u = 0; u < U; ++u) {
+        const double* p = a.part + 2 * min(i0 + u, to - 1) * a.D + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[u][j] = i0 + u < to && c + j < a.D ? p[j] : 0.0;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += v[u][j];
     }
     __syncthreads();  // (the last round's sums have been read)
 #pragma unroll
@@ -538,10 +544,10 @@ hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* stat
       const uint32_t* ki = i == 0 ? nullptr : keys[at];
       const uint32_t* ri = i == 0 ? nullptr : rows[at];
       const int to = i == 0 ? 0 : 1 - at;
-      hipLaunchKernelGGL(eg_count, dim3((unsigned)tiles), dim3(256), 0, s, t, ki, i * EG_BITS, count);
+      hipLaunchKernelGGL(eg_count, dim3((unsigned)tiles), dim3(1024), 0, s, t, ki, i * EG_BITS, count);
       if (tiles > EG_SCAN_TILES)
         hipLaunchKernelGGL(eg_scan, dim3(EG_BINS / 64), dim3(256), 0, s, count, tiles);
-      hipLaunchKernelGGL(eg_scatter, dim3((unsigned)tiles), dim3(256), 0, s, t, ki, ri, i * EG_BITS,
+      hipLaunchKernelGGL(eg_scatter, dim3((unsigned)tiles), dim3(1024), 0, s, t, ki, ri, i * EG_BITS,
                          (const uint32_t*)count, tiles, keys[to], rows[to]);
       at = to;
     }
