@@ -7,12 +7,13 @@
 // to dW. Bound: both move each row once.
 //
 // The gradient's order of summation is fixed: the rows' ordinals are sorted by token (stable, by
-// digits of EG_BITS bits), the sorted list is cut every EG_TILE rows wherever a token's rows begin
+// digits of EG_BITS bits), the sorted list is cut every 8 or 32 rows wherever a token's rows begin
 // or end, a wave sums a piece's rows in ascending order in binary64, and a token whose rows lie
 // in several pieces gets its parts added in ascending order. So a frequent token costs no more than
 // as many rows of different ones, nothing is added by atomics, and results do not depend on what
 // runs when.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
@@ -81,7 +82,7 @@ constexpr int EG_KEYS = 4;                     // keys a thread
 constexpr int EG_SORT = 1024 * EG_KEYS;        // keys a workgroup
 constexpr int64_t EG_SCAN_TILES = 64;          // up to here a workgroup adds the others' counts itself
 constexpr int EG_SMALL_KEYS = 8, EG_SMALL = 1024 * EG_SMALL_KEYS;  // keys that one workgroup sorts
-constexpr int EG_TILE = 32;                    // sorted rows a wave sums
+constexpr int64_t EG_FLAGS = 1 << 20;          // table rows up to which a byte each says whether a token names it
 
 // Among the wave's active lanes: those whose digit is this lane's.
 __device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool active) {
@@ -137,15 +138,22 @@ __device__ __forceinline__ void scan_bins(uint32_t* v, uint32_t* wave_sum_lds) {
   __syncthreads();
 }
 
-// Sorted keys and row ordinals of up to EG_SMALL rows in one launch.
+// Zeros in the bytes of `flags` (none: null) that thread `at` of `of` takes.
+__device__ __forceinline__ void clear_flags(uint8_t* flags, int64_t V, int64_t at, int64_t of) {
+  if (flags == nullptr) return;
+  for (int64_t i = 16 * at; i < V; i += 16 * of) *reinterpret_cast<uint4*>(flags + i) = make_uint4(0, 0, 0, 0);
+}
+
+// Sorted keys and row ordinals of up to 1024 K rows in one launch.
+template <int K>
 __global__ void __launch_bounds__(1024) eg_sort_small(Tokens t, int passes, uint32_t* __restrict__ keys,
-                                                      uint32_t* __restrict__ rows) {
-  constexpr int K = EG_SMALL_KEYS, NW = 16;
+                                                      uint32_t* __restrict__ rows, uint8_t* flags) {
+  constexpr int NW = 16;
   __shared__ uint32_t count[NW][EG_BINS];
   __shared__ uint32_t base[EG_BINS];
   __shared__ uint32_t sums[EG_BINS / 128];
-  __shared__ uint32_t lk[EG_SMALL];
-  __shared__ uint16_t lr[EG_SMALL];
+  __shared__ uint32_t lk[1024 * K];
+  __shared__ uint16_t lr[1024 * K];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int N = (int)t.N;
   uint32_t key[K];
@@ -158,20 +166,24 @@ __global__ void __launch_bounds__(1024) eg_sort_small(Tokens t, int passes, uint
     key[i] = active[i] ? t.key(n, true) : 0u;
     row[i] = (uint16_t)n;
   }
+  clear_flags(flags, t.V, threadIdx.x, 1024);
   for (int p = 0; p < passes; ++p) {
     uint32_t digit[K], rank[K];
 #pragma unroll
     for (int i = 0; i < K; ++i) digit[i] = (key[i] >> (p * EG_BITS)) & (EG_BINS - 1);
-    for (int i = threadIdx.x; i < NW * EG_BINS; i += 1024) (&count[0][0])[i] = 0;
+#pragma unroll
+    for (int i = 0; i < NW * EG_BINS / 1024; ++i) (&count[0][0])[threadIdx.x + 1024 * i] = 0;
     __syncthreads();
     wave_ranks<K>(digit, active, count[w], rank);
     __syncthreads();
     if (threadIdx.x < EG_BINS) {
-      uint32_t sum = 0;
+      uint32_t c[NW], sum = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) c[i] = count[i][threadIdx.x];
+#pragma unroll
       for (int i = 0; i < NW; ++i) {
-        const uint32_t c = count[i][threadIdx.x];
         count[i][threadIdx.x] = sum;
-        sum += c;
+        sum += c[i];
       }
       base[threadIdx.x] = sum;
     }
@@ -194,7 +206,6 @@ __global__ void __launch_bounds__(1024) eg_sort_small(Tokens t, int passes, uint
         row[i] = lr[n];
       }
     }
-    __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < K; ++i) {
@@ -202,14 +213,16 @@ __global__ void __launch_bounds__(1024) eg_sort_small(Tokens t, int passes, uint
     if (active[i]) {
       keys[n] = key[i];
       rows[n] = row[i];
+      if (flags != nullptr && key[i] < t.V) flags[key[i]] = 1;  // (cleared before the barriers above)
     }
   }
 }
 
 // Digit counts of each EG_SORT keys: count[tile][bin]. The first pass reads the tokens.
 __global__ void __launch_bounds__(1024) eg_count(Tokens t, const uint32_t* __restrict__ keys, int shift,
-                                                uint32_t* __restrict__ count) {
+                                                 uint32_t* __restrict__ count, uint8_t* flags) {
   __shared__ uint32_t h[4][EG_BINS];
+  clear_flags(flags, t.V, (int64_t)blockIdx.x * 1024 + threadIdx.x, (int64_t)gridDim.x * 1024);
   for (int i = threadIdx.x; i < 4 * EG_BINS; i += 1024) (&h[0][0])[i] = 0;
   __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * EG_SORT;
@@ -249,9 +262,10 @@ __global__ void __launch_bounds__(256) eg_scan(uint32_t* __restrict__ count, int
 
 // Moves each key and its row to its place by one digit.
 __global__ void __launch_bounds__(1024) eg_scatter(Tokens t, const uint32_t* __restrict__ keys,
-                                                  const uint32_t* __restrict__ rows, int shift,
-                                                  const uint32_t* __restrict__ count, int64_t tiles,
-                                                  uint32_t* __restrict__ keys_out, uint32_t* __restrict__ rows_out) {
+                                                   const uint32_t* __restrict__ rows, int shift,
+                                                   const uint32_t* __restrict__ count, int64_t tiles,
+                                                   uint32_t* __restrict__ keys_out,
+                                                   uint32_t* __restrict__ rows_out, uint8_t* flags) {
   constexpr int K = EG_KEYS, NW = 16;
   __shared__ uint32_t h[NW][EG_BINS];
   __shared__ uint32_t base[EG_BINS], before[EG_BINS];
@@ -305,6 +319,7 @@ __global__ void __launch_bounds__(1024) eg_scatter(Tokens t, const uint32_t* __r
       const uint32_t to = h[w][digit[i]] + rank[i];
       keys_out[to] = key[i];
       rows_out[to] = row[i];
+      if (flags != nullptr && key[i] < t.V) flags[key[i]] = 1;
     }
   }
 }
@@ -316,6 +331,7 @@ struct SumArgs {
   const uint32_t* rows;  // the row of dY of each
   float* dw;
   double* part;          // [tiles][2][D]: a piece that begins before its tile, one that ends behind it
+  const uint8_t* flags;  // [V]: whether a token names the row; null: the sorted keys are searched
   int64_t N, V, D, ldy, tiles, segments;  // segments of 256 columns
   double scale;
   int accumulate;
@@ -332,7 +348,8 @@ __device__ __forceinline__ void eg_result(const SumArgs& a, uint32_t key, int64_
   st4<true>(p, a.D - c, o);
 }
 
-// A wave's part: rows [first, last) of the sorted list, 256 columns from c0 on.
+// A wave's part: EG_TILE rows of the sorted list, 256 columns.
+template <int EG_TILE>
 __device__ __forceinline__ void eg_sum_tile(const SumArgs& a, int64_t tile, int64_t segment) {
   const int lane = threadIdx.x & 63;
   const int64_t first = tile * EG_TILE, count = min((int64_t)EG_TILE, a.N - first);
@@ -383,19 +400,24 @@ __device__ __forceinline__ void eg_sum_tile(const SumArgs& a, int64_t tile, int6
   }
 }
 
-// Zeros in the rows of `EG_FILL` table rows from v0 on that no token names.
+// Zeros in those of EG_FILL table rows from v0 on that no token names.
 constexpr int EG_FILL = 16;
 __device__ __forceinline__ void eg_fill_rows(const SumArgs& a, int64_t v0) {
   const int lane = threadIdx.x & 63;
   const int64_t v = v0 + (lane % EG_FILL);
-  // the first of the sorted keys that is not below v
-  int64_t lo = 0, hi = a.N;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (a.keys[mid] < v) lo = mid + 1;
-    else hi = mid;
+  bool absent = v < a.V;
+  if (a.flags != nullptr) {
+    absent = absent && a.flags[v] == 0;
+  } else {
+    // the first of the sorted keys that is not below v
+    int64_t lo = 0, hi = a.N;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (a.keys[mid] < v) lo = mid + 1;
+      else hi = mid;
+    }
+    absent = absent && !(lo < a.N && a.keys[lo] == v);
   }
-  const bool absent = v < a.V && !(lo < a.N && a.keys[lo] == v);
   uint32_t todo = (uint32_t)__ballot(absent) & ((1u << EG_FILL) - 1);
   while (todo != 0) {
     const int j = __ffs(todo) - 1;
@@ -405,12 +427,13 @@ __device__ __forceinline__ void eg_fill_rows(const SumArgs& a, int64_t v0) {
   }
 }
 
+template <int EG_TILE>
 __global__ void __launch_bounds__(256) eg_sum(SumArgs a, int64_t sum_groups) {
   const int w = threadIdx.x >> 6;
   if (blockIdx.x < sum_groups) {
     const int64_t units = a.tiles * a.segments;
     for (int64_t u = (int64_t)blockIdx.x * 4 + w; u < units; u += sum_groups * 4)
-      eg_sum_tile(a, u / a.segments, u % a.segments);
+      eg_sum_tile<EG_TILE>(a, u / a.segments, u % a.segments);
     return;
   }
   const int64_t waves = ((int64_t)gridDim.x - sum_groups) * 4;
@@ -421,6 +444,7 @@ __global__ void __launch_bounds__(256) eg_sum(SumArgs a, int64_t sum_groups) {
 // Adds up the parts of a token whose rows lie in several tiles. One workgroup for the tile in which
 // the token's rows begin and 256 columns; its four waves take consecutive quarters of the tiles
 // behind, whose parts are the first pieces there.
+template <int EG_TILE>
 __global__ void __launch_bounds__(256) eg_join(SumArgs a) {
   __shared__ double part[4][256];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -432,14 +456,20 @@ __global__ void __launch_bounds__(256) eg_join(SumArgs a) {
     if (key >= a.V || a.keys[end] != key) continue;
     const int64_t first = tile * EG_TILE;
     if (first > 0 && a.keys[first - 1] == key) continue;  // began in an earlier tile
-    // tiles whose last key is this token's, which sorted keys have in a row
-    int64_t lo = tile + 1, hi = a.tiles;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.keys[min(a.N, (mid + 1) * EG_TILE) - 1] == key) lo = mid + 1;
-      else hi = mid;
+    // the first tile behind whose last key is not this token's (64 at a time)
+    int64_t lo = tile + 1;
+    while (lo < a.tiles) {
+      const int64_t i = lo + lane;
+      const bool same = i < a.tiles && a.keys[min(a.N, (i + 1) * EG_TILE) - 1] == key;
+      const uint64_t other = ~__ballot(same);
+      if (other != 0) {
+        lo += __ffsll((unsigned long long)other) - 1;
+        break;
+      }
+      lo += 64;
     }
     // the last tile with a part: lo itself if its first row is the token's
+    lo = min(lo, a.tiles);
     const int64_t stop = lo < a.tiles && a.keys[lo * EG_TILE] == key ? lo + 1 : lo;
     const int64_t n = stop - (tile + 1), quarter = (n + 3) / 4;
     const int64_t from = tile + 1 + min(n, w * quarter), to = tile + 1 + min(n, (w + 1) * quarter);
@@ -480,10 +510,12 @@ int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // What embed_grad keeps: two lists of keys and rows, digit counts, parts of sums.
 struct Layout {
-  int64_t keys[2], rows[2], count, part, bytes;
+  int64_t keys[2], rows[2], count, flags, part, bytes;
 };
-Layout layout(int64_t N, int64_t D) {
-  const int64_t sort = (N + EG_SORT - 1) / EG_SORT, tiles = (N + EG_TILE - 1) / EG_TILE;
+// Sorted rows that a wave sums: 32, or 8 where that leaves fewer than eight waves for each CU.
+int64_t tile_rows(int64_t N, int64_t D) { return (N + 31) / 32 * ((D + 255) / 256) < 2048 ? 8 : 32; }
+Layout layout(int64_t N, int64_t V, int64_t D) {
+  const int64_t sort = (N + EG_SORT - 1) / EG_SORT, rows = tile_rows(N, D), tiles = (N + rows - 1) / rows;
   Layout l{};
   int64_t off = 0;
   auto take = [&](int64_t bytes) {
@@ -496,6 +528,7 @@ Layout layout(int64_t N, int64_t D) {
     l.rows[i] = take(4 * N);
   }
   l.count = take(4 * (sort + 1) * EG_BINS);
+  l.flags = take(V <= EG_FLAGS ? V : 0);
   l.part = take(tiles > 1 ? 16 * tiles * D : 0);
   l.bytes = off;
   return l;
@@ -523,32 +556,43 @@ hipError_t launch_embed(const EmbedParams& p, uint32_t* status, hipStream_t s) {
   return hipGetLastError();
 }
 
-int64_t embed_grad_scratch_bytes(int64_t N, int64_t D) { return layout(N, D).bytes; }
+int64_t embed_grad_scratch_bytes(int64_t N, int64_t V, int64_t D) { return layout(N, V, D).bytes; }
 
 hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* status, hipStream_t s) {
   if (p.V <= 0 || p.D <= 0 || (p.N <= 0 && p.accumulate)) return hipSuccess;
   const Tokens t = tokens_of(p, status);
-  const Layout l = layout(p.N, p.D);
+  const Layout l = layout(p.N, p.V, p.D);
   char* base = static_cast<char*>(scratch);
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(base + l.keys[0]), reinterpret_cast<uint32_t*>(base + l.keys[1])};
   uint32_t* rows[2] = {reinterpret_cast<uint32_t*>(base + l.rows[0]), reinterpret_cast<uint32_t*>(base + l.rows[1])};
   uint32_t* count = reinterpret_cast<uint32_t*>(base + l.count);
+  // (rows are cleared here only where the table's gradient is not added to)
+  uint8_t* flags = !p.accumulate && p.N > 0 && p.V <= EG_FLAGS ? reinterpret_cast<uint8_t*>(base + l.flags) : nullptr;
   int passes = 1;  // digits of the keys 0 .. V
   while (passes * EG_BITS < 32 && (p.V >> (passes * EG_BITS)) != 0) ++passes;
   int at = 0;
   if (p.N > 0 && p.N <= EG_SMALL) {
-    hipLaunchKernelGGL(eg_sort_small, dim3(1), dim3(1024), 0, s, t, passes, keys[0], rows[0]);
+    auto sort = [&](auto k) {
+      constexpr int K = decltype(k)::value;
+      hipLaunchKernelGGL(eg_sort_small<K>, dim3(1), dim3(1024), 0, s, t, passes, keys[0], rows[0], flags);
+    };
+    if (p.N <= 1024) sort(std::integral_constant<int, 1>());
+    else if (p.N <= 2048) sort(std::integral_constant<int, 2>());
+    else if (p.N <= 4096) sort(std::integral_constant<int, 4>());
+    else if (p.N <= 6144) sort(std::integral_constant<int, 6>());
+    else sort(std::integral_constant<int, EG_SMALL_KEYS>());
   } else if (p.N > 0) {
     const int64_t tiles = (p.N + EG_SORT - 1) / EG_SORT;
     for (int i = 0; i < passes; ++i) {
       const uint32_t* ki = i == 0 ? nullptr : keys[at];
       const uint32_t* ri = i == 0 ? nullptr : rows[at];
       const int to = i == 0 ? 0 : 1 - at;
-      hipLaunchKernelGGL(eg_count, dim3((unsigned)tiles), dim3(1024), 0, s, t, ki, i * EG_BITS, count);
+      hipLaunchKernelGGL(eg_count, dim3((unsigned)tiles), dim3(1024), 0, s, t, ki, i * EG_BITS, count,
+                         i == 0 ? flags : nullptr);
       if (tiles > EG_SCAN_TILES)
         hipLaunchKernelGGL(eg_scan, dim3(EG_BINS / 64), dim3(256), 0, s, count, tiles);
       hipLaunchKernelGGL(eg_scatter, dim3((unsigned)tiles), dim3(1024), 0, s, t, ki, ri, i * EG_BITS,
-                         (const uint32_t*)count, tiles, keys[to], rows[to]);
+                         (const uint32_t*)count, tiles, keys[to], rows[to], i == 0 ? flags : nullptr);
       at = to;
     }
   }
@@ -562,16 +606,24 @@ hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* stat
   a.V = p.V;
   a.D = p.D;
   a.ldy = p.ldy;
-  a.tiles = (p.N + EG_TILE - 1) / EG_TILE;
+  a.flags = flags;
+  const int64_t tile = tile_rows(p.N, p.D);
+  a.tiles = (p.N + tile - 1) / tile;
   a.segments = (p.D + 255) / 256;
   a.scale = (double)p.scale;
   a.accumulate = p.accumulate;
   constexpr int64_t MOST = 1 << 20;  // workgroups of either half
   const int64_t sums = std::min<int64_t>((a.tiles * a.segments + 3) / 4, MOST);
   const int64_t fills = p.accumulate ? 0 : std::min<int64_t>((p.V + 4 * EG_FILL - 1) / (4 * EG_FILL), MOST);
-  hipLaunchKernelGGL(eg_sum, dim3((unsigned)(sums + fills)), dim3(256), 0, s, a, sums);
-  if (a.tiles > 1)
-    hipLaunchKernelGGL(eg_join, dim3((unsigned)std::min<int64_t>((a.tiles - 1) * a.segments, MOST)), dim3(256), 0, s, a);
+  auto go = [&](auto rows_of_tile) {
+    constexpr int TILE = decltype(rows_of_tile)::value;
+    hipLaunchKernelGGL(eg_sum<TILE>, dim3((unsigned)(sums + fills)), dim3(256), 0, s, a, sums);
+    if (a.tiles > 1)
+      hipLaunchKernelGGL(eg_join<TILE>, dim3((unsigned)std::min<int64_t>((a.tiles - 1) * a.segments, MOST)), dim3(256),
+                         0, s, a);
+  };
+  if (tile == 8) go(std::integral_constant<int, 8>());
+  else go(std::integral_constant<int, 32>());
   return hipGetLastError();
 }
 

@@ -291,7 +291,7 @@ struct EmbedParams {
 };
 hipError_t launch_embed(const EmbedParams& p, uint32_t* status, hipStream_t s);
 hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* status, hipStream_t s);
-int64_t embed_grad_scratch_bytes(int64_t N, int64_t D);
+int64_t embed_grad_scratch_bytes(int64_t N, int64_t V, int64_t D);
 
 // Layer norm over the last axis (layer_norm.hip): y [R, C] from x [R, C]; gamma, beta [C] may be null.
 // y may be x with the same row stride.

@@ -595,8 +595,8 @@ int32_t validate_token_step(Validator& v, size_t idx, const Step& st, uint64_t* 
         return v.err;
       if (!apart(s[2], {s[0], s[1]})) return aliases(grad ? table : row);
       if (grad) {
-        // (16 bytes for each column of every 32nd row at most, far below 2^63 with N rows of D held above)
-        need(shk::embed_grad_scratch_bytes(N, D));
+        // (16 bytes for each column of every 8th row at most, below 2^63 with N rows of D held above)
+        need(shk::embed_grad_scratch_bytes(N, V, D));
       }
       return SHK_HIP_STATUS_OK;
     }
