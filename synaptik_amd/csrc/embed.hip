@@ -400,6 +400,16 @@ __device__ __forceinline__ void eg_sum_tile(const SumArgs& a, int64_t tile, int6
   }
 }
 
+// Zeros in the table rows v0 + j for the bits j of `todo` (the same in the wave).
+__device__ __forceinline__ void eg_clear(const SumArgs& a, int64_t v0, uint32_t todo) {
+  while (todo != 0) {
+    const int j = __ffs(todo) - 1;
+    todo &= todo - 1;
+    float* row = a.dw + (v0 + j) * a.D;
+    for (int64_t c = 4 * (threadIdx.x & 63); c < a.D; c += 256)
+      st4<true>(row + c, a.D - c, make_float4(0.f, 0.f, 0.f, 0.f));
+  }
+}
 // Zeros in those of EG_FILL table rows from v0 on that no token names.
 constexpr int EG_FILL = 16;
 __device__ __forceinline__ void eg_fill_rows(const SumArgs& a, int64_t v0) {
@@ -418,13 +428,7 @@ __device__ __forceinline__ void eg_fill_rows(const SumArgs& a, int64_t v0) {
     }
     absent = absent && !(lo < a.N && a.keys[lo] == v);
   }
-  uint32_t todo = (uint32_t)__ballot(absent) & ((1u << EG_FILL) - 1);
-  while (todo != 0) {
-    const int j = __ffs(todo) - 1;
-    todo &= todo - 1;
-    float* row = a.dw + (v0 + j) * a.D;
-    for (int64_t c = 4 * lane; c < a.D; c += 256) st4<true>(row + c, a.D - c, make_float4(0.f, 0.f, 0.f, 0.f));
-  }
+  eg_clear(a, v0, (uint32_t)__ballot(absent) & ((1u << EG_FILL) - 1));
 }
 
 template <int EG_TILE>
@@ -439,6 +443,81 @@ __global__ void __launch_bounds__(256) eg_sum(SumArgs a, int64_t sum_groups) {
   const int64_t waves = ((int64_t)gridDim.x - sum_groups) * 4;
   for (int64_t v = (((int64_t)blockIdx.x - sum_groups) * 4 + w) * EG_FILL; v < a.V; v += waves * EG_FILL)
     eg_fill_rows(a, v);
+}
+
+// Up to EG_DIRECT rows in one launch, without sorting: every wave holds all keys, four a lane. A wave of
+// the first `sum_groups` workgroups takes one row of dY and 256 columns, and sums the rows of its
+// token if it is the first of them; the others clear table rows. [130, 617] over 10007 rows takes one
+// launch instead of three.
+constexpr int EG_DIRECT = 256;
+__global__ void __launch_bounds__(256) eg_direct(Tokens t, SumArgs a, int64_t sum_groups) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint32_t none = (uint32_t)a.V;
+  uint32_t key[EG_DIRECT / 64];
+#pragma unroll
+  for (int i = 0; i < EG_DIRECT / 64; ++i) {
+    const int64_t n = i * 64 + lane;
+    key[i] = n < t.N ? t.key(n, blockIdx.x == 0 && w == 0) : none;
+  }
+  if (blockIdx.x < sum_groups) {
+    const int64_t units = a.N * a.segments;
+    for (int64_t u = (int64_t)blockIdx.x * 4 + w; u < units; u += sum_groups * 4) {
+      const int n = (int)(u / a.segments);
+      const int64_t c = (u % a.segments) * 256 + 4 * lane;
+      uint32_t mine = none;
+#pragma unroll
+      for (int i = 0; i < EG_DIRECT / 64; ++i)
+        if (i == n / 64) mine = (uint32_t)__builtin_amdgcn_readlane((int)key[i], n % 64);
+      if (mine >= none) continue;
+      uint64_t same[EG_DIRECT / 64];
+      bool first = true;
+#pragma unroll
+      for (int i = 0; i < EG_DIRECT / 64; ++i) {
+        same[i] = __ballot(key[i] == mine);
+        if (i < n / 64) first = first && same[i] == 0;
+        else if (i == n / 64) first = first && (same[i] & ((1ull << (n % 64)) - 1)) == 0;
+      }
+      if (!first) continue;
+      double acc[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+      for (int i = 0; i < EG_DIRECT / 64; ++i) {
+        uint64_t todo = same[i];
+        while (todo != 0) {
+          constexpr int U = 8;
+          float4 v[U];
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (todo != 0) {
+              const int64_t row = i * 64 + __ffsll((unsigned long long)todo) - 1;
+              todo &= todo - 1;
+              v[k] = ld4(a.dy + row * a.ldy + c, a.D - c);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            acc[0] += (double)v[k].x;
+            acc[1] += (double)v[k].y;
+            acc[2] += (double)v[k].z;
+            acc[3] += (double)v[k].w;
+          }
+        }
+      }
+      if (c < a.D) eg_result(a, mine, c, acc);
+    }
+    return;
+  }
+  const int64_t waves = ((int64_t)gridDim.x - sum_groups) * 4;
+  for (int64_t v0 = (((int64_t)blockIdx.x - sum_groups) * 4 + w) * EG_FILL; v0 < a.V; v0 += waves * EG_FILL) {
+    int named = 0;
+#pragma unroll
+    for (int i = 0; i < EG_DIRECT / 64; ++i) {
+      const uint32_t at = key[i] - (uint32_t)v0;
+      if (at < EG_FILL) named |= 1 << at;
+    }
+    const int rows = (int)min((int64_t)EG_FILL, a.V - v0);
+    eg_clear(a, v0, ~(uint32_t)wave_or(named) & ((1u << rows) - 1));
+  }
 }
 
 // Adds up the parts of a token whose rows lie in several tiles. One workgroup for the tile in which
@@ -567,11 +646,32 @@ hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* stat
   uint32_t* rows[2] = {reinterpret_cast<uint32_t*>(base + l.rows[0]), reinterpret_cast<uint32_t*>(base + l.rows[1])};
   uint32_t* count = reinterpret_cast<uint32_t*>(base + l.count);
   // (rows are cleared here only where the table's gradient is not added to)
-  uint8_t* flags = !p.accumulate && p.N > 0 && p.V <= EG_FLAGS ? reinterpret_cast<uint8_t*>(base + l.flags) : nullptr;
+  uint8_t* flags = !p.accumulate && p.V <= EG_FLAGS ? reinterpret_cast<uint8_t*>(base + l.flags) : nullptr;
   int passes = 1;  // digits of the keys 0 .. V
   while (passes * EG_BITS < 32 && (p.V >> (passes * EG_BITS)) != 0) ++passes;
   int at = 0;
-  if (p.N > 0 && p.N <= EG_SMALL) {
+  SumArgs a{};
+  a.dy = p.w;
+  a.dw = p.y;
+  a.part = reinterpret_cast<double*>(base + l.part);
+  a.N = p.N;
+  a.V = p.V;
+  a.D = p.D;
+  a.ldy = p.ldy;
+  a.flags = flags;
+  const int64_t tile = tile_rows(p.N, p.D);
+  a.tiles = (p.N + tile - 1) / tile;
+  a.segments = (p.D + 255) / 256;
+  a.scale = (double)p.scale;
+  a.accumulate = p.accumulate;
+  constexpr int64_t MOST = 1 << 20;  // workgroups of either half
+  const int64_t fills = p.accumulate ? 0 : std::min<int64_t>((p.V + 4 * EG_FILL - 1) / (4 * EG_FILL), MOST);
+  if (p.N <= EG_DIRECT) {
+    const int64_t rows_of = std::min<int64_t>((p.N * a.segments + 3) / 4, MOST);
+    hipLaunchKernelGGL(eg_direct, dim3((unsigned)(rows_of + fills)), dim3(256), 0, s, t, a, rows_of);
+    return hipGetLastError();
+  }
+  if (p.N <= EG_SMALL) {
     auto sort = [&](auto k) {
       constexpr int K = decltype(k)::value;
       hipLaunchKernelGGL(eg_sort_small<K>, dim3(1), dim3(1024), 0, s, t, passes, keys[0], rows[0], flags);
@@ -581,7 +681,7 @@ hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* stat
     else if (p.N <= 4096) sort(std::integral_constant<int, 4>());
     else if (p.N <= 6144) sort(std::integral_constant<int, 6>());
     else sort(std::integral_constant<int, EG_SMALL_KEYS>());
-  } else if (p.N > 0) {
+  } else {
     const int64_t tiles = (p.N + EG_SORT - 1) / EG_SORT;
     for (int i = 0; i < passes; ++i) {
       const uint32_t* ki = i == 0 ? nullptr : keys[at];
@@ -596,25 +696,9 @@ hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* stat
       at = to;
     }
   }
-  SumArgs a{};
-  a.dy = p.w;
   a.keys = keys[at];
   a.rows = rows[at];
-  a.dw = p.y;
-  a.part = reinterpret_cast<double*>(base + l.part);
-  a.N = p.N;
-  a.V = p.V;
-  a.D = p.D;
-  a.ldy = p.ldy;
-  a.flags = flags;
-  const int64_t tile = tile_rows(p.N, p.D);
-  a.tiles = (p.N + tile - 1) / tile;
-  a.segments = (p.D + 255) / 256;
-  a.scale = (double)p.scale;
-  a.accumulate = p.accumulate;
-  constexpr int64_t MOST = 1 << 20;  // workgroups of either half
   const int64_t sums = std::min<int64_t>((a.tiles * a.segments + 3) / 4, MOST);
-  const int64_t fills = p.accumulate ? 0 : std::min<int64_t>((p.V + 4 * EG_FILL - 1) / (4 * EG_FILL), MOST);
   auto go = [&](auto rows_of_tile) {
     constexpr int TILE = decltype(rows_of_tile)::value;
     hipLaunchKernelGGL(eg_sum<TILE>, dim3((unsigned)(sums + fills)), dim3(256), 0, s, a, sums);

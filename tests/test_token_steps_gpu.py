@@ -101,7 +101,9 @@ def tokens_like(rng, kind, N, V):
 @pytest.mark.parametrize("kind", ["even", "frequent", "one", "half", "sorted"])
 @pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 600, 5), (31, 4, 3), (32, 2, 260), (33, 1, 8), (64, 7, 64), (65, 512, 300),
                                    (300, 513, 17), (4096, 1000, 12), (4097, 70000, 5), (5001, 511, 61),
-                                   (9000, 262144, 4), (20000, 300000, 3)])
+                                   (9000, 262144, 4), (20000, 300000, 3), (256, 300, 40), (257, 40, 33), (1024, 77, 20),
+                                   (1025, 5, 9), (2049, 1100, 30), (6145, 90, 7), (8192, 2000, 11), (8193, 33, 6),
+                                   (130, 1200000, 3), (600, 1200000, 2)])
 def test_embed_grad(ctx, N, V, D, kind):
     rng = np.random.default_rng(N + V)
     tokens = tokens_like(rng, kind, N, V)
