@@ -12,12 +12,11 @@
 // Bound: the logits are read once and the gradient is written once. A row is held in registers from
 // its load to its gradient. The gradient is first stored as that of a teacher without entries; after
 // a barrier the entries' threads store theirs (all threads of one index the same sum, in the
-// entries' order). The exponentials of the C classes are binary32 (fexp.h), their sum and all that
+// entries' order). The exponentials of the C classes are binary32, their sum and all that
 // concerns the K entries is binary64: the loss is a small difference of logarithms.
 #include <algorithm>
 
 #include "common.h"
-#include "fexp.h"
 #include "kernels.h"
 #include "row4.h"
 #include "rowvec.h"
@@ -38,8 +37,8 @@ struct DistillArgs {
   uint32_t* status;
   int64_t R, C;
   int K, is64, parts;
-  float inv_T;           // 1 / T
-  double inv_T64, scale; // g T
+  float per_T;           // log2(e) / T
+  double inv_T, scale;   // 1 / T, g T
 };
 
 __device__ __forceinline__ int64_t entry_index(const DistillArgs& a, int64_t at) {
@@ -91,16 +90,13 @@ __global__ void __launch_bounds__(1024) distill_count(DistillArgs a, uint32_t* c
   }
 }
 
-// exp(x) for x <= 0: zero where the result is no normal number (a class of such a weight is 2^-126
-// of the largest at most), NaN for NaN.
-__device__ __forceinline__ float exp_weight(float x) {
-  const float e = exp_f32_in_range(fmaxf(x, -87.0f));
-  return x != x ? x : x < -87.0f ? 0.0f : e;
-}
-
-__device__ __forceinline__ float4 weights(const float4& z, float m, float inv_T) {
-  return make_float4(exp_weight((z.x - m) * inv_T), exp_weight((z.y - m) * inv_T), exp_weight((z.z - m) * inv_T),
-                     exp_weight((z.w - m) * inv_T));
+// exp(x / T) for x = z - m <= 0 by the hardware's power of two (1 ulp; a result that is no normal number,
+// 2^-126 of the largest weight at most, is zero, NaN stays): six instructions' time where the
+// polynomial of fexp.h takes twenty. [4096, 32003] took 247 us with that.
+__device__ __forceinline__ float exp_weight(float x, float per_T) { return __builtin_amdgcn_exp2f(x * per_T); }
+__device__ __forceinline__ float4 weights(const float4& z, float m, float per_T) {
+  return make_float4(exp_weight(z.x - m, per_T), exp_weight(z.y - m, per_T), exp_weight(z.z - m, per_T),
+                     exp_weight(z.w - m, per_T));
 }
 __device__ __forceinline__ double total(const float4& v) {
   return ((double)v.x + (double)v.y) + ((double)v.z + (double)v.w);
@@ -189,26 +185,26 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
     const RowOf<NT, V> in(C);
     float4 v[V > 0 ? V : 1];
     float m = -INFINITY, thread_m = -INFINITY;
-    double s[4] = {0.0, 0.0, 0.0, 0.0};  // sums of exp(z - m), e = exp(t - mt), e (t - mt - z + m); the rows counted
+    double s[2] = {0.0, 0.0};  // the sum of exp(z - m); the rows counted
     if constexpr (V > 0) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         if (i < V - 1) v[i] = ld4_at<true>(row, in.at(i), 4);
         else v[i] = in.mine ? ld4_at<true>(row, in.end, 4) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       }
-      if (counts && n < 0.0) s[3] = count_rows<NT>(a, marks);
+      if (counts && n < 0.0) s[1] = count_rows<NT>(a, marks);
 #pragma unroll
       for (int i = 0; i < V; ++i) m = fmaxf(m, largest(v[i]));
     } else {
-      if (counts && n < 0.0) s[3] = count_rows<NT>(a, marks);
+      if (counts && n < 0.0) s[1] = count_rows<NT>(a, marks);
       for (int q = threadIdx.x; q < view.groups; q += NT) {
         const float4 x = view.load(row, q, -INFINITY);
         const float top = fmaxf(m, largest(x));
         if (top > m) {  // (the sum so far is zero where m is -inf)
-          s[0] *= (double)exp_weight((m - top) * a.inv_T);
+          s[0] *= (double)exp_weight(m - top, a.per_T);
           m = top;
         }
-        s[0] += total(weights(x, m, a.inv_T));
+        s[0] += total(weights(x, m, a.per_T));
       }
       thread_m = m;
     }
@@ -225,43 +221,49 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
     if constexpr (V > 0) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[i] = weights(v[i], m, a.inv_T);
+        v[i] = weights(v[i], m, a.per_T);
         s[0] += i < V - 1 ? total(v[i]) : in.new_part(v[i]);
         __builtin_amdgcn_sched_barrier(0);  // four exponentials at a time keep the registers down
       }
     } else if (thread_m != m) {
       // a thread all of whose logits are -inf has summed NaN: its part is zero unless the row's largest is -inf
-      s[0] = thread_m == -INFINITY && m > -INFINITY ? 0.0 : s[0] * (double)exp_weight((thread_m - m) * a.inv_T);
+      s[0] = thread_m == -INFINITY && m > -INFINITY ? 0.0 : s[0] * (double)exp_weight(thread_m - m, a.per_T);
     }
-    for (int j = threadIdx.x; j < a.K; j += NT) {
-      double e = 0.0;
-      if (index[j] >= 0) {
-        const double t = ((double)a.t[r * a.K + j] - (double)mt) * a.inv_T64;
-        e = exp(t);
-        const double z = ((double)row[index[j]] - (double)m) * a.inv_T64;
-        s[1] += e;
-        if (e != 0.0) s[2] += e * (t - z);
+    group_sums<NT, 2>(s, red);
+    if (counts && n < 0.0) n = s[1];
+    const float scale = (float)(a.scale / n);
+    if (out != nullptr) {
+      const float inv = (float)(1.0 / s[0]);
+      if constexpr (V > 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (i < V - 1) st4_at<true>(out, in.at(i), 4, scaled(v[i], inv, scale));
+          else if (in.mine) st4_at<true>(out, in.end, 4, scaled(v[i], inv, scale));
+        }
+      } else {
+        for (int q = threadIdx.x; q < view.groups; q += NT)
+          view.store(out, q, scaled(weights(view.load(row, q, -INFINITY), m, a.per_T), inv, scale));
       }
-      entries[j] = e;
     }
-    group_sums<NT, 4>(s, red);
-    if (counts && n < 0.0) n = s[3];
+    // the entries, whose binary64 values need the registers that held the row
+    double e[2] = {0.0, 0.0};  // sums of exp(t - mt) and of that times (t - mt - z + m)
+    for (int j = threadIdx.x; j < a.K; j += NT) {
+      double p = 0.0;
+      if (index[j] >= 0) {
+        const double t = ((double)a.t[r * a.K + j] - (double)mt) * a.inv_T;
+        p = exp(t);
+        const double z = ((double)row[index[j]] - (double)m) * a.inv_T;
+        e[0] += p;
+        if (p != 0.0) e[1] += p * (t - z);
+      }
+      entries[j] = p;
+    }
+    group_sums<NT, 2>(e, red + 2 * NW);
     if (threadIdx.x == 0) {
-      const float loss = (float)(s[2] / s[1] - log(s[1]) + log(s[0]));
+      const float loss = (float)(e[1] / e[0] - log(e[0]) + log(s[0]));
       a.row_loss[r] = loss == 0.0f ? 0.0f : loss;
     }
     if (out == nullptr) continue;
-    const float inv = (float)(1.0 / s[0]), scale = (float)(a.scale / n);
-    if constexpr (V > 0) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (i < V - 1) st4_at<true>(out, in.at(i), 4, scaled(v[i], inv, scale));
-        else if (in.mine) st4_at<true>(out, in.end, 4, scaled(v[i], inv, scale));
-      }
-    } else {
-      for (int q = threadIdx.x; q < view.groups; q += NT)
-        view.store(out, q, scaled(weights(view.load(row, q, -INFINITY), m, a.inv_T), inv, scale));
-    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above precede those below
     __syncthreads();
     for (int j = threadIdx.x; j < a.K; j += NT) {
@@ -269,8 +271,8 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
       if (mine < 0) continue;
       double p = 0.0;
       for (int i = 0; i < a.K; ++i) p += index[i] == mine ? entries[i] : 0.0;
-      const double q = (double)exp_weight((row[mine] - m) * a.inv_T) / s[0];
-      out[mine] = (float)(q - p / s[1]) * scale;
+      const double q = (double)exp_weight(row[mine] - m, a.per_T) / s[0];
+      out[mine] = (float)(q - p / e[0]) * scale;
     }
   }
 }
@@ -324,8 +326,8 @@ hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* statu
   a.C = p.C;
   a.K = (int)p.K;
   a.is64 = p.is64;
-  a.inv_T = (float)(1.0 / (double)p.T);
-  a.inv_T64 = 1.0 / (double)p.T;
+  a.per_T = (float)(1.4426950408889634 / (double)p.T);
+  a.inv_T = 1.0 / (double)p.T;
   a.scale = (double)p.g * (double)p.T;
   if (p.grad != nullptr && (p.R > COUNT_ROWS || p.R * p.K > COUNT_ENTRIES)) {
     uint32_t* count = reinterpret_cast<uint32_t*>(a.row_loss + (p.R + 3) / 4 * 4);

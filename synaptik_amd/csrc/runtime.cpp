@@ -681,8 +681,8 @@ int32_t validate_token_step(Validator& v, size_t idx, const Step& st, uint64_t* 
     default: {  // OP_DISTILL
       const int64_t R = a[0], C = a[1], K = a[2], is64 = a[3];
       const float T = r.farg[0];
-      if (!extent_ok(R) || C <= 0 || C > INT32_MAX - 1024 || K <= 0 || !flag_ok(is64) || !(T > 0.0f) ||
-          !std::isfinite(T) || !std::isfinite(1.0f / T))
+      if (!extent_ok(R) || C <= 0 || C > INT32_MAX - 1024 || K <= 0 || !flag_ok(is64) ||
+          !(T > 0.0f) || !std::isnormal(T))
         return bad_shape("distillation");
       if (K > shk::DISTILL_MOST)
         return fail(SHK_HIP_STATUS_UNSUPPORTED_SHAPE, "step %zu: more than %lld teacher entries a row", idx,

@@ -421,7 +421,7 @@ class ProgramBuilder:
 
         An entry of index -1 or logit -inf is absent; a row without entries has a zero gradient
         (none has one: the loss is NaN). Any other index outside [0, C) fails the run
-        (INDEX_OUT_OF_BOUNDS). Entries of one class add up. T is positive, and 1 / T finite."""
+        (INDEX_OUT_OF_BOUNDS). Entries of one class add up. T is a positive normal number."""
         return self._add(OP_DISTILL, [logits, indices, teacher, loss, grad],
                          [R, C, K, self._is64(indices)], [temperature, g])
 
