@@ -11,8 +11,8 @@
 //
 // Bound: the logits are read once and the gradient is written once. A row is held in registers from
 // its load to its gradient. The gradient is first stored as that of a teacher without entries; after
-// a barrier the entries' threads store theirs (all threads of one index the same sum, in the
-// entries' order). The exponentials of the C classes are binary32, their sum and all that
+// a barrier the entries' threads store theirs; where a class is named twice (which a table in LDS shows),
+// all threads of one class the same sum, in the entries' order. The exponentials of the C classes are binary32, their sum and all that
 // concerns the K entries is binary64: the loss is a small difference of logarithms.
 #include <algorithm>
 
@@ -36,7 +36,7 @@ struct DistillArgs {
   const uint32_t* count; // [parts]: rows that have an entry; null: counted here
   uint32_t* status;
   int64_t R, C;
-  int K, is64, parts;
+  int K, is64, parts, slots, shift;
   float per_T;           // log2(e) / T
   double inv_T, scale;   // 1 / T, g T
 };
@@ -135,12 +135,14 @@ struct RowOf {
 template <int NT, int V>
 __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) distill_rows(DistillArgs a) {
   constexpr int NW = NT / 64;
-  extern __shared__ double entries[];  // K: p; then K indexes
+  extern __shared__ double entries[];  // K: p; then K indexes and the table
   __shared__ double red[4 * NW];
   __shared__ float fm[2][NW];
   __shared__ int found[NW];
   __shared__ uint8_t marks[COUNT_ROWS];
+  __shared__ int twice;  // whether two entries name one class
   int* index = reinterpret_cast<int*>(entries + a.K);
+  int* table = index + a.K;  // a.slots, a power of two of 2 K or more: the classes that were seen
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const bool counts = a.grad != nullptr && a.count == nullptr;  // the rows with an entry, beside the first row's sums
   double n = -1.0;
@@ -153,8 +155,10 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
     const float* row = a.z + r * a.C;
     float* out = a.grad != nullptr ? a.grad + r * a.C : nullptr;
     const RowGroups view(row, C);
-    // the entries: whether there are any, the largest logit
-    __syncthreads();  // the last row's entries have been read
+    // the entries: whether there are any, whether a class is named twice, the largest logit
+    for (int i = threadIdx.x; i < a.slots; i += NT) table[i] = -1;
+    if (threadIdx.x == 0) twice = 0;
+    __syncthreads();  // (the last row's entries have been read)
     int any = 0;
     float mt = -INFINITY;
     for (int j = threadIdx.x; j < a.K; j += NT) {
@@ -165,7 +169,14 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
       const bool there = inside && t != -INFINITY;
       index[j] = there ? (int)i : -1;
       any |= there;
-      if (there) mt = fmaxf(mt, t);  // (a NaN makes the sums NaN)
+      if (!there) continue;
+      mt = fmaxf(mt, t);  // (a NaN makes the sums NaN)
+      if (a.grad == nullptr) continue;
+      for (uint32_t at = (uint32_t)i * 0x9e3779b1u >> a.shift;; at = (at + 1) & (a.slots - 1)) {
+        const int old = atomicCAS(&table[at], -1, (int)i);  // (half of the slots stay free: the search ends)
+        if (old == (int)i) twice = 1;
+        if (old == -1 || old == (int)i) break;
+      }
     }
     any = __any(any);
     if (NW > 1) {
@@ -269,8 +280,11 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
     for (int j = threadIdx.x; j < a.K; j += NT) {
       const int mine = index[j];
       if (mine < 0) continue;
-      double p = 0.0;
-      for (int i = 0; i < a.K; ++i) p += index[i] == mine ? entries[i] : 0.0;
+      double p = entries[j];
+      if (twice) {
+        p = 0.0;
+        for (int i = 0; i < a.K; ++i) p += index[i] == mine ? entries[i] : 0.0;
+      }
       const double q = (double)exp_weight(row[mine] - m, a.per_T) / s[0];
       out[mine] = (float)(q - p / e[0]) * scale;
     }
@@ -297,7 +311,7 @@ constexpr int COUNT_PARTS = 64;
 
 template <int NT, int V>
 void launch_rows(const DistillArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((distill_rows<NT, V>), dim3((unsigned)std::min<int64_t>(a.R, 1 << 20)), dim3(NT), 12 * a.K, s, a);
+  hipLaunchKernelGGL((distill_rows<NT, V>), dim3((unsigned)std::min<int64_t>(a.R, 1 << 20)), dim3(NT), 12 * a.K + 4 * a.slots, s, a);
 }
 
 // V groups a thread, from V to MOST by the row's width.
@@ -326,6 +340,12 @@ hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* statu
   a.C = p.C;
   a.K = (int)p.K;
   a.is64 = p.is64;
+  a.slots = 2;
+  a.shift = 31;
+  while (a.slots < 2 * a.K) {
+    a.slots *= 2;
+    --a.shift;
+  }
   a.per_T = (float)(1.4426950408889634 / (double)p.T);
   a.inv_T = 1.0 / (double)p.T;
   a.scale = (double)p.g * (double)p.T;

@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
     };
     auto put = [&](float* x, float v) {
       float* p = reinterpret_cast<float*>(reinterpret_cast<char*>(x) + at);
-      if (STREAM) __builtin_nontemporal_store(v, p);
+      if (STREAM && (BACK || MODE == CHUNK)) __builtin_nontemporal_store(v, p);
       else *p = v;
     };
     const float* const src[4] = {a.z, BACK ? a.dh : a.u, a.u, a.h};

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(NT) ln_fwd(FwdArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         at(o, j) = fmaf((float)((((double)at(x.v[i], j) - (double)x0) - delta) * rstd), at(gm.v[i], j), at(bt.v[i], j));
-      st4_at<STREAM>(y, 16u * t + 16u * T * i, rest - 4 * T * i, o);
+      st4_at(y, 16u * t + 16u * T * i, rest - 4 * T * i, o);
     }
   }
 }
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(LN_WIDE) ln_fwd_wide(FwdArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         at(o, j) = fmaf((float)(((double)at(v, j) - mean) * rstd), at(gm, j), at(bt, j));
-      st4<true>(y + c, a.C - c, o);
+      st4(y + c, a.C - c, o);
     }
   }
 }
@@ -231,7 +231,7 @@ __device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[4 * 
         dg[i][j] = fma(v, fma(d, rstd, shift), dg[i][j]);
         db[i][j] += v;
       }
-      st4_at<STREAM>(dx, 16u * t + 16u * T * i, rest - 4 * T * i, o);
+      st4_at<STREAM && T == NT>(dx, 16u * t + 16u * T * i, rest - 4 * T * i, o);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(LN_WIDE) ln_bwd_wide(BwdArgs a) {
         const double g = (double)at(v, j) * (double)at(gm, j);
         at(o, j) = (float)(rstd * (fma(-((double)at(xv, j) - mean), c2, g) - c1));
       }
-      st4<true>(dx + c, a.C - c, o);
+      st4(dx + c, a.C - c, o);
     }
   }
 }
@@ -389,8 +389,11 @@ BwdShape bwd_shape(int64_t R, int64_t C) {
   return b;
 }
 
-// Tensors beyond what the last-level cache holds go past it: the backward pass of [16384, 4096], 805
-// MB, takes 154 us so and 170 us through the caches; that of [3001, 1531], 55 MB, 26.6 and 21.8 us.
+// Tensors beyond what the last-level cache holds are read past the caches, and where a workgroup holds a
+// row, dx is written so: the backward pass of [16384, 4096], 805 MB, takes 143 us, 150 us with plain
+// writes and 170 us with plain reads too; that of [3001, 1531], 55 MB, 26.6 us so and 20 us through the
+// caches. Waves that hold rows write [65536, 1000] in 149 us, past the caches in 156; the forward
+// pass of [16384, 4096] takes 98 and 102 us.
 bool streams(int64_t bytes) { return bytes > 256 << 20; }
 
 template <int NT, int T, int V>
