@@ -345,7 +345,7 @@ __device__ __forceinline__ void eg_result(const SumArgs& a, uint32_t key, int64_
     const float4 old = ld4(p, a.D - c);
     o = make_float4(old.x + o.x, old.y + o.y, old.z + o.z, old.w + o.w);
   }
-  st4(p, a.D - c, o);
+  st4<true>(p, a.D - c, o);
 }
 
 // A wave's part: EG_TILE rows of the sorted list, 256 columns.
@@ -407,7 +407,7 @@ __device__ __forceinline__ void eg_clear(const SumArgs& a, int64_t v0, uint32_t 
     todo &= todo - 1;
     float* row = a.dw + (v0 + j) * a.D;
     for (int64_t c = 4 * (threadIdx.x & 63); c < a.D; c += 256)
-      st4(row + c, a.D - c, make_float4(0.f, 0.f, 0.f, 0.f));
+      st4<true>(row + c, a.D - c, make_float4(0.f, 0.f, 0.f, 0.f));
   }
 }
 // Zeros in those of EG_FILL table rows from v0 on that no token names.

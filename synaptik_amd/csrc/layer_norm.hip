@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(NT) ln_fwd(FwdArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         at(o, j) = fmaf((float)((((double)at(x.v[i], j) - (double)x0) - delta) * rstd), at(gm.v[i], j), at(bt.v[i], j));
-      st4_at(y, 16u * t + 16u * T * i, rest - 4 * T * i, o);
+      st4_at<STREAM>(y, 16u * t + 16u * T * i, rest - 4 * T * i, o);
     }
   }
 }
@@ -176,15 +176,26 @@ __device__ __forceinline__ void forget(float4 (&v)[V]) {
 // dy and dx may be the same memory: a thread writes the elements that it read. AHEAD: the next row is
 // on its way while this one is summed.
 template <int NT, int T, int V, bool AHEAD, bool STREAM>
-__device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[4 * (NT / 64)], double (&dg)[V][4],
-                                            double (&db)[V][4]) {
+__device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[4 * (NT / 64)], double (*dbs)[NT],
+                                            double (&dg)[V][4], double (&db)[V][4]) {
   const int t = threadIdx.x % T, rest = (int)a.C - 4 * t;
   Row<T, V> gm;
-  gm.load_or(a.gamma, t, rest, 1.0f);
+  if (AHEAD) gm.load_or(a.gamma, t, rest, 1.0f);
+  // (up to 16384 columns leave no registers for them: they come from the caches twice a row, and the sums of
+  // dbeta lie in LDS)
+  auto gamma = [&](int i) {
+    if (AHEAD) return gm.v[i];
+    return a.gamma != nullptr ? ld4_at(a.gamma, 16u * t + 16u * T * i, rest - 4 * T * i)
+                              : make_float4(1.f, 1.f, 1.f, 1.f);
+  };
 #pragma unroll
   for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) dg[i][j] = db[i][j] = 0.0;
+    for (int j = 0; j < 4; ++j) {
+      dg[i][j] = 0.0;
+      if (AHEAD) db[i][j] = 0.0;
+      else dbs[4 * i + j][threadIdx.x] = 0.0;
+    }
   const int64_t step = (int64_t)gridDim.x * (NT / T);
   int64_t r = (int64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
   Row<T, V> x, dy, nx, ndy;
@@ -203,16 +214,19 @@ __device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[4 * 
     if (AHEAD && r + step < a.R) fetch(r + step);
     double s[4] = {0.0, 0.0, 0.0, 0.0};  // sums of d, d^2, g, g d
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int i = 0; i < V; ++i) {
+      const float4 gi = gamma(i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const double d = (double)(j < rest - 4 * T * i ? at(x.v[i], j) : x0) - (double)x0;
-        const double g = (double)at(dy.v[i], j) * (double)at(gm.v[i], j);
+        const double g = (double)at(dy.v[i], j) * (double)at(gi, j);
         s[0] += d;
         s[1] = fma(d, d, s[1]);
         s[2] += g;
         s[3] = fma(g, d, s[3]);
       }
+      if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
+    }
     row_sums<NT, T>(s, lds[turn]);
     const double delta = s[0] * a.inv_C, rstd = 1.0 / sqrt(variance(s[1] * a.inv_C, delta) + a.eps);
     // dx = rstd (g - c1 - (d - delta) c2)
@@ -223,15 +237,17 @@ __device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[4 * 
     float* dx = a.dx + r * a.lddx;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+      const float4 gi = gamma(i);
       float4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const double d = (double)at(x.v[i], j) - (double)x0, v = (double)at(dy.v[i], j);
-        at(o, j) = (float)fma(d, slope, fma(v * (double)at(gm.v[i], j), rstd, offset));
+        at(o, j) = (float)fma(d, slope, fma(v * (double)at(gi, j), rstd, offset));
         dg[i][j] = fma(v, fma(d, rstd, shift), dg[i][j]);
-        db[i][j] += v;
+        if (AHEAD) db[i][j] += v;
+        else dbs[4 * i + j][threadIdx.x] += v;
       }
-      st4_at<STREAM && T == NT>(dx, 16u * t + 16u * T * i, rest - 4 * T * i, o);
+      st4_at<STREAM>(dx, 16u * t + 16u * T * i, rest - 4 * T * i, o);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -243,7 +259,16 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(T == 64
   __shared__ double lds[2][4 * (NT / 64)];
   const int t = threadIdx.x % T;
   double dg[V][4], db[V][4];
-  ln_bwd_rows<NT, T, V, AHEAD, STREAM>(a, lds, dg, db);
+  if constexpr (AHEAD) {
+    ln_bwd_rows<NT, T, V, AHEAD, STREAM>(a, lds, nullptr, dg, db);
+  } else {
+    __shared__ double dbs[4 * V][NT];
+    ln_bwd_rows<NT, T, V, AHEAD, STREAM>(a, lds, dbs, dg, db);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) db[i][j] = dbs[4 * i + j][threadIdx.x];
+  }
   if (a.part == nullptr) return;
   double* out = a.part + (int64_t)blockIdx.x * 2 * a.C;
   if constexpr (T == NT) {
@@ -379,7 +404,8 @@ BwdShape bwd_shape(int64_t R, int64_t C) {
     b.groups = std::min<int64_t>(R, 64);
   } else if (C > 1024) {
     b.rows = 1;
-    b.groups = std::min<int64_t>(R, 512);
+    // (a CU holds one workgroup of 1024 threads; each writes 16 C bytes of partial sums)
+    b.groups = std::min<int64_t>(R, C > 4096 ? 256 : 512);
   } else {
     int64_t lanes = 2;
     while (lanes < 64 && 4 * lanes < C) lanes *= 2;
@@ -389,11 +415,9 @@ BwdShape bwd_shape(int64_t R, int64_t C) {
   return b;
 }
 
-// Tensors beyond what the last-level cache holds are read past the caches, and where a workgroup holds a
-// row, dx is written so: the backward pass of [16384, 4096], 805 MB, takes 143 us, 150 us with plain
-// writes and 170 us with plain reads too; that of [3001, 1531], 55 MB, 26.6 us so and 20 us through the
-// caches. Waves that hold rows write [65536, 1000] in 149 us, past the caches in 156; the forward
-// pass of [16384, 4096] takes 98 and 102 us.
+// Tensors beyond what the last-level cache holds go past it: the backward pass of [16384, 4096], 805
+// MB, takes 161 us so, 174 us with plain writes and more with plain reads; [65536, 1000] 169 and 187
+// us. That of [3001, 1531], 55 MB, takes 27 us so and 20 us through the caches.
 bool streams(int64_t bytes) { return bytes > 256 << 20; }
 
 template <int NT, int T, int V>
