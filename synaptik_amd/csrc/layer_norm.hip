@@ -439,6 +439,8 @@ void launch_bwd(const BwdArgs& a, int64_t groups, hipStream_t s) {
 hipError_t launch_layer_norm(const LayerNormParams& p, hipStream_t s) {
   if (p.R <= 0 || p.C <= 0) return hipSuccess;
   const FwdArgs a{p.x, p.gamma, p.beta, p.y, p.R, p.C, p.ldx, p.ldy, (double)p.eps, 1.0 / (double)p.C};
+  // A wave or less a row up to 1024 columns ([65536, 1000] 106 us, a workgroup a row 142 us), then eight
+  // columns a thread ([16384, 4096] 107 us, sixteen 111 us).
   if (p.C <= 8) launch_fwd<256, 2, 1>(a, s);
   else if (p.C <= 16) launch_fwd<256, 4, 1>(a, s);
   else if (p.C <= 32) launch_fwd<256, 8, 1>(a, s);
@@ -448,8 +450,8 @@ hipError_t launch_layer_norm(const LayerNormParams& p, hipStream_t s) {
   else if (p.C <= 512) launch_fwd<256, 64, 2>(a, s);
   else if (p.C <= 1024) launch_fwd<256, 64, 4>(a, s);
   else if (p.C <= 2048) launch_fwd<256, 256, 2>(a, s);
-  else if (p.C <= 4096) launch_fwd<256, 256, 4>(a, s);
-  else if (p.C <= 8192) launch_fwd<512, 512, 4>(a, s);
+  else if (p.C <= 4096) launch_fwd<512, 512, 2>(a, s);
+  else if (p.C <= 8192) launch_fwd<1024, 1024, 2>(a, s);
   else if (p.C <= LN_REGS) launch_fwd<1024, 1024, 4>(a, s);
   else
     hipLaunchKernelGGL(ln_fwd_wide, dim3((unsigned)std::min<int64_t>(p.R, 1 << 16)), dim3(LN_WIDE), 0, s, a);
