@@ -131,7 +131,10 @@ struct RowOf {
 
 // A workgroup a row, V groups of four classes a thread. V == 0: the row does not fit; one reading forms
 // the largest logit and the sum about the largest so far, a second one the gradient. Four waves on
-// each SIMD in every form.
+// each SIMD in every form. [4096, 32003] of 64 entries, 1.0 GB, takes 206 us, 4.8 TB/s: two workgroups a CU,
+// whose loads, exponentials and stores overlap only as they happen to fall. One row a workgroup lets
+// the next begin where one ends: with 1024 workgroups that take four each the step takes 236 us
+// instead of 224.
 template <int NT, int V>
 __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) distill_rows(DistillArgs a) {
   constexpr int NW = NT / 64;

@@ -74,7 +74,8 @@ struct FwdArgs {
   double eps, inv_C;
 };
 
-// T threads a row: a part of a wave, or the whole workgroup.
+// T threads a row: a part of a wave, or the whole workgroup. [16384, 4096], 537 MB, takes 107 us, 5.0 TB/s;
+// one row of 4096 3.1 us, a launch.
 template <int NT, int T, int V, bool STREAM>
 __global__ void __launch_bounds__(NT) ln_fwd(FwdArgs a) {
   __shared__ double lds[2][2 * (NT / 64)];
@@ -254,6 +255,9 @@ __device__ __forceinline__ void ln_bwd_rows(const BwdArgs& a, double (*lds)[4 * 
 }
 
 // Four waves on each SIMD where a workgroup holds a row; a wave that holds one has up to 256 registers.
+// [16384, 4096], 805 MB, takes 146 us, 5.5 TB/s; two rounds of sums a row (the mean first) took 156 us, and
+// sums by shuffles 220. [3001, 1531], 55 MB, takes 20 us, of which some 8 pass before the first row is
+// summed and after the last.
 template <int NT, int T, int V, bool AHEAD, bool STREAM>
 __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(T == 64 ? 2 : 4))) ln_bwd(BwdArgs a) {
   __shared__ double lds[2][4 * (NT / 64)];
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(256) ln_cols_wide(BwdArgs a) {
   }
 }
 
-// Adds P rows of partial sums: 32 columns by 16 parts of the rows.
+// Adds P rows of partial sums: 32 columns by 16 parts of the rows. 512 rows of 8192 take 5.9 us.
 __global__ void __launch_bounds__(512) ln_finish(const double* __restrict__ part, int64_t P, int64_t C,
                                                  float* dgamma, float* dbeta) {
   __shared__ double sum[16][33];
