@@ -360,7 +360,7 @@ class ProgramBuilder:
     def embed(self, W, tokens, Y, N, V, D, *, scale=1.0, pad=None, ldy=None) -> Step:
         """Y [N, D] = scale * W[tokens] of a table W [V, D] and N tokens (i32 or i64), a zero row where
         the token is `pad`. Any other token outside [0, V) fails the run (INDEX_OUT_OF_BOUNDS); its
-        row is zero."""
+        row is zero. Where D is zero nothing is read."""
         return self._add(OP_EMBED, [W, tokens, Y],
                          [N, V, D, ldy if ldy is not None else D, self._is64(tokens), int(pad is not None),
                           pad if pad is not None else 0], [scale])
@@ -370,7 +370,7 @@ class ProgramBuilder:
         """dW [V, D]: row v is scale times the sum of the rows of dY [N, D] whose token is v (in
         binary64, in a fixed order), zero where there are none. With `accumulate` the sums are added
         to dW (a table that is the output layer's weight too) and other rows are left as they are.
-        Tokens as for embed; one out of bounds adds nothing."""
+        Tokens as for embed; one out of bounds adds nothing. Where dW is empty nothing is read."""
         return self._add(OP_EMBED_GRAD, [dY, tokens, dW],
                          [N, V, D, ldy if ldy is not None else D, self._is64(tokens), int(pad is not None),
                           pad if pad is not None else 0, int(accumulate)], [scale])
@@ -399,7 +399,7 @@ class ProgramBuilder:
         lengths [B] (i32 or i64) are the positions that each sequence has: those behind are not
         read, H is zero there, and `last` is the state at the end, h0 for a length of zero. A length
         outside [0, T] fails the run (INDEX_OUT_OF_BOUNDS). A state that is not finite stays not
-        finite (an infinity may become NaN)."""
+        finite (an infinity may become NaN). Where B or D is zero nothing is read."""
         return self._add(OP_GATED_SCAN, [Z, U, h0, lengths, H, last], [B, T, D, self._is64(lengths)])
 
     def gated_scan_grad(self, dH, Z, U, H, dZ, dU, B, T, D, *, h0=None, dlast=None, dh0=None,
@@ -421,7 +421,8 @@ class ProgramBuilder:
 
         An entry of index -1 or logit -inf is absent; a row without entries has a zero gradient
         (none has one: the loss is NaN). Any other index outside [0, C) fails the run
-        (INDEX_OUT_OF_BOUNDS). Entries of one class add up. T is a positive normal number."""
+        (INDEX_OUT_OF_BOUNDS). Entries of one class add up. T is a positive normal
+        number. Without rows nothing is written."""
         return self._add(OP_DISTILL, [logits, indices, teacher, loss, grad],
                          [R, C, K, self._is64(indices)], [temperature, g])
 
