@@ -11,9 +11,10 @@
 //
 // Bound: the logits are read once and the gradient is written once. A row is held in registers from
 // its load to its gradient. The gradient is first stored as that of a teacher without entries; after
-// a barrier the entries' threads store theirs; where a class is named twice (which a table in LDS shows),
-// all threads of one class the same sum, in the entries' order. The exponentials of the C classes are binary32, their sum and all that
-// concerns the K entries is binary64: the loss is a small difference of logarithms.
+// a barrier the entries' threads store theirs; where a class is named twice (which a table in LDS
+// shows), all threads of one class the same sum, in the entries' order. The exponentials of the C
+// classes are binary32, their sum and all that concerns the K entries is binary64: the loss is a small
+// difference of logarithms.
 #include <algorithm>
 
 #include "common.h"
@@ -159,9 +160,10 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
     float* out = a.grad != nullptr ? a.grad + r * a.C : nullptr;
     const RowGroups view(row, C);
     // the entries: whether there are any, whether a class is named twice, the largest logit
+    if (r != blockIdx.x) __syncthreads();  // (the last row's have been read)
     for (int i = threadIdx.x; i < a.slots; i += NT) table[i] = -1;
     if (threadIdx.x == 0) twice = 0;
-    __syncthreads();  // (the last row's entries have been read)
+    __syncthreads();
     int any = 0;
     float mt = -INFINITY;
     for (int j = threadIdx.x; j < a.K; j += NT) {

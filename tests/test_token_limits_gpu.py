@@ -154,6 +154,32 @@ def test_distill_of_more_rows_than_a_launch_has_workgroups(ctx):
     o.within(outs[0].download(), np.array([loss]), np.array([o.U * (3 * 10 + 2 + 2 * abs(loss))]))
 
 
+def test_classes_named_twice_in_more_rows_than_a_launch_has_workgroups(ctx):
+    """A workgroup's rows with a class named twice beside rows without: each by its own entries."""
+    R, C, K = (1 << 20) + 70000, 300, 3
+    rng = np.random.default_rng(3)
+    kinds = 64
+    z, t = rng.standard_normal((kinds, C)).astype(np.float32), rng.standard_normal((kinds, K)).astype(np.float32)
+    index = np.stack([rng.permutation(C)[:K] for _ in range(kinds)]).astype(np.int32)
+    index[::2, 2] = index[::2, 0]
+    kind = rng.integers(0, kinds, R).astype(np.int32)
+    pb = ProgramBuilder()
+    sw, sk, sz = pb.input(kinds * C), pb.input(R, "i32"), pb.internal(R * C)
+    si, st, sl, sg = pb.input(R * K, "i32"), pb.input(R * K), pb.output(1), pb.output(R * C)
+    pb.embed(sw, sk, sz, R, kinds, C)
+    pb.distill(sz, si, st, sl, R, C, K, grad=sg, g=float(R))
+    prog = HipProgram(ctx, pb.image())
+    outs = [ctx.buffer(4), ctx.buffer(4 * R * C)]
+    prog.run([ctx.upload(z), ctx.upload(kind), ctx.upload(index[kind]), ctx.upload(t[kind])], outs)
+    prog.close()
+    each = [o.distill(z[v:v + 1], index[v:v + 1], t[v:v + 1]) for v in range(kinds)]
+    want = np.concatenate([e[1] for e in each])
+    bound = np.concatenate([e[3] for e in each]) + 2 * o.U * np.abs(want)  # (g T / n is 1 but for two roundings)
+    for first in (0, 70000 - 500, 1 << 19, 1 << 20, R - 1000):
+        got = outs[1].download(count=1000 * C, offset=4 * C * first).reshape(1000, C)
+        o.within(got, want[kind[first:first + 1000]], bound[kind[first:first + 1000]])
+
+
 def test_layer_norm_of_more_rows_than_a_launch_has_workgroups(ctx):
     R, C = 65536 + 70, 1025
     rng = np.random.default_rng(2)
