@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);  // one gate's binary64 values at a time
       }
-      if (!whole(q0)) {
+      const bool inside = whole(q0);
+      if (!inside) {
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
           const bool in = q0 + i < hi && q0 + i >= from && q0 + i < to;
@@ -238,8 +239,10 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
           if (q0 + i >= hi) break;
           if (BACK) {
             const float g = v[i] + s;
-            put(x[0], g * m[i]);
-            put(x[1], g * k[i]);
+            float dz = g * m[i], du = g * k[i];
+            if (!inside && q0 + i < from) dz = du = 0.0f;  // (a gradient that is not finite stays at the end)
+            put(x[0], dz);
+            put(x[1], du);
             s = f[i] * g;
           } else {
             s = fmaf(f[i], s, b[i]);

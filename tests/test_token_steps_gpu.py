@@ -405,6 +405,38 @@ def test_states_in_place(ctx, B, T, D):
     prog.close()
 
 
+@pytest.mark.parametrize("T,D", [(4, 20), (50, 70), (1300, 64)])
+def test_values_that_are_not_finite_stay_within_their_sequence(ctx, T, D):
+    """A NaN or infinity in one channel of one sequence, in its inputs, its first state or its last state's
+    gradient: other channels are finite, and behind a sequence's end all is zero."""
+    B = 4
+    rng = np.random.default_rng(T)
+    z, u = floats(rng, B, T, D), floats(rng, B, T, D)
+    lengths = np.array([T, T // 2, 0, T - 1])
+    h0, dlast, dh = floats(rng, B, D), floats(rng, B, D), floats(rng, B, T, D)
+    h = o.gated_scan(z, u, h0, lengths)[0].astype(np.float32)
+    z[0, 1, 3], h0[1, 5], dlast[1, 6], dlast[2, 7], dlast[3, 8], u[3, 0, 9] = np.nan, np.inf, np.nan, np.inf, np.inf, np.nan
+    pb = ProgramBuilder()
+    sz, su, sd, sh = (pb.input(z.size) for _ in range(4))
+    s0, sl, sn = pb.input(B * D), pb.input(B * D), pb.input(B, "i32")
+    out, last, dz, du, dh0 = pb.output(z.size), pb.output(B * D), pb.output(z.size), pb.output(z.size), pb.output(B * D)
+    pb.gated_scan(sz, su, out, B, T, D, h0=s0, last=last, lengths=sn)
+    pb.gated_scan_grad(sd, sz, su, sh, dz, du, B, T, D, h0=s0, dlast=sl, dh0=dh0, lengths=sn)
+    got = run(ctx, pb, [z, u, dh, h, h0, dlast, lengths.astype(np.int32)], [out, last, dz, du, dh0])
+    behind = np.arange(T)[None] >= lengths[:, None]
+    touched = np.zeros((B, D), bool)
+    for b, c in ((0, 3), (1, 5), (1, 6), (2, 7), (3, 8), (3, 9)):
+        touched[b, c] = True
+    for i in (0, 2, 3):
+        a = got[i].reshape(B, T, D)
+        assert (a[behind] == 0).all()
+        assert np.isfinite(a[np.broadcast_to(~touched[:, None], a.shape)]).all()
+    for i in (1, 4):
+        assert np.isfinite(got[i].reshape(B, D)[~touched]).all()
+    assert np.isnan(got[0].reshape(B, T, D)[0, 1:, 3]).all() and not np.isfinite(got[1].reshape(B, D)[1, 5])
+    assert not np.isfinite(got[4].reshape(B, D)[[1, 2, 3], [6, 7, 8]]).any()
+
+
 @pytest.mark.parametrize("T,D", [(5, 20), (1200, 64)])
 def test_lengths_out_of_bounds_fail_the_run(ctx, T, D):
     rng = np.random.default_rng(T)
