@@ -53,7 +53,8 @@ enum {
      * TrainingParameter.java:488-525) */
     SHK_HIP_STATUS_ARITHMETIC = 15,
     /* a categorical target index lay outside the class extent (Java: IllegalArgumentException,
-     * CpuLossReferenceKernel.java:264) */
+     * CpuLossReferenceKernel.java:264), or a token, a sequence's length or a teacher's class lay
+     * outside its own */
     SHK_HIP_STATUS_INDEX_OUT_OF_BOUNDS = 16
 };
 

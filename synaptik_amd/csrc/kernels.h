@@ -11,7 +11,7 @@ namespace shk {
 enum DeviceStatus : uint32_t {
   DEV_OK = 0,
   DEV_NON_FINITE = 1,       // an optimizer intermediate or candidate was not finite
-  DEV_INDEX_OUT_OF_BOUNDS = 2,  // a categorical target index lies outside the class extent
+  DEV_INDEX_OUT_OF_BOUNDS = 2,  // a categorical target, token, length or teacher's class lies outside its extent
   DEV_NOT_POSITIVE = 4,     // an adaptive bias correction or denominator was not positive
   DEV_INVALID_BOOL = 8,     // a published BOOL element held a byte other than 0 or 1
 };
