@@ -216,11 +216,12 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
       for (int q = threadIdx.x; q < view.groups; q += NT) {
         const float4 x = view.load(row, q, -INFINITY);
         const float top = fmaxf(m, largest(x));
-        if (top > m) {  // (the sum so far is zero where m is -inf)
+        if (top > m) {  // (the sum so far is zero, or NaN, where m is -inf)
           s[0] *= (double)exp_weight(m - top, a.per_T);
           m = top;
         }
-        s[0] += total(weights(x, m, a.per_T));
+        // about 0 while all logits were -inf, which weigh nothing there (about themselves they are NaN)
+        s[0] += total(weights(x, m > -INFINITY ? m : 0.0f, a.per_T));
       }
       thread_m = m;
     }
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
         __builtin_amdgcn_sched_barrier(0);  // four exponentials at a time keep the registers down
       }
     } else if (thread_m != m) {
-      // a thread all of whose logits are -inf has summed NaN: its part is zero unless the row's largest is -inf
+      // (a thread all of whose logits are -inf has summed nothing)
       s[0] = thread_m == -INFINITY && m > -INFINITY ? 0.0 : s[0] * (double)exp_weight(thread_m - m, a.per_T);
     }
     group_sums<NT, 2>(s, red);
