@@ -243,8 +243,7 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
         __builtin_amdgcn_sched_barrier(0);  // four exponentials at a time keep the registers down
       }
     } else if (thread_m != m) {
-      // (a thread all of whose logits are -inf has summed nothing)
-      s[0] = thread_m == -INFINITY && m > -INFINITY ? 0.0 : s[0] * (double)exp_weight(thread_m - m, a.per_T);
+      s[0] *= (double)exp_weight(thread_m - m, a.per_T);  // (zero or NaN already where thread_m is -inf)
     }
     group_sums<NT, 2>(s, red);
     if (counts && n < 0.0) n = s[1];

@@ -50,3 +50,21 @@ def test_narrow_rows_with_one_class_left(ctx, C):
     keep = rng.integers(0, C, 9)
     z[np.arange(9), keep] = floats(rng, 9) * 3
     check_distill(ctx, z, keep[:, None], floats(rng, 9, 1))
+
+
+@pytest.mark.parametrize("C", WIDTHS)
+@pytest.mark.parametrize("where", ["first", "last", "every"])
+def test_nan_beside_masked_classes(ctx, C, where):
+    """A row with a NaN is NaN throughout, also where a thread's other classes are all masked: eight
+    classes of every 4096 hold a whole group of four of one thread, however the row is aligned."""
+    rng = np.random.default_rng(C)
+    z = (floats(rng, 3, C) * 4).astype(np.float32)
+    blocks = np.arange(20, C - 8, 4096)
+    nan = {"first": blocks[:1], "last": blocks[-1:], "every": blocks}[where]
+    for b in blocks:
+        z[:, b:b + 8] = -np.inf
+    for b in nan:
+        z[:, b:b + 8] = np.nan
+    for r in range(3):
+        check_distill(ctx, z[r:r + 1], np.array([[1, 2, 3]]), np.ones((1, 3), np.float32))
+    check_distill(ctx, z, np.tile([1, 2, 3], (3, 1)), np.ones((3, 3), np.float32))
