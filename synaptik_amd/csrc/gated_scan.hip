@@ -13,11 +13,20 @@
 // launch forms the chunks' steps, a second joins those before each chunk and is the pass above from
 // there.
 //
-// States and products are binary32, as the outputs are; a gate and its complement come from one
-// binary64 exponential, so that 1 - f keeps its bits where f is near one. A sequence shorter than T
-// holds its state behind its end (f = 1, b = 0): its last state, and the gradient that enters there,
-// need no case of their own. Positions behind the end are not read; their outputs are zero.
+// A gate and its complement come from one binary64 exponential, so that 1 - f keeps its bits where f is
+// near one. Rounded to binary32, f and 1 - f no longer add up to one: f is off by up to 3e-8, which a
+// memory of 1 / (1 - f) positions adds up. So a run's product of gates is binary64, and so is the state that
+// is handed from run to run: binary32 is what happens within the TS positions of one run, each run's result
+// from s = 0, and the outputs. With z from 6 to 12 and u constant, begun with the state u, h was off by up to
+// 8e-5 of u after 2048 positions and 1.3e-3 after 65536 with binary32 throughout, and is off by 2e-7. That
+// costs 0 to 4 % of the time. (A call of up to 8 positions has no runs to join and is binary64 throughout;
+// from call to call states are the binary32 values in memory.)
+//
+// A sequence shorter than T holds its state behind its end (z = inf there: f = 1, 1 - f = 0): its last
+// state, and the gradient that enters there, need no case of their own. Positions behind the end are not
+// read; their outputs are zero.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
@@ -25,14 +34,14 @@
 namespace shk {
 namespace {
 
-// f = 1 / (1 + e) and k = e / (1 + e) with e = exp(-z), in binary64 and rounded once to binary32. e is
+// f = 1 / (1 + e) and k = e / (1 + e) with e = exp(-z), in binary64, k rounded once to binary32. e is
 // 2^n exp(r), z = -(n ln2 + r), |r| <= 0.3466 (Cody and Waite, as in fexp64.h), with the Taylor
 // polynomial to r^9 / 9!: what it leaves out is 0.3466^10 / 10! = 7e-12 of e, a ten-thousandth of a
-// unit in the last place of the results. The reciprocal's estimate takes one Newton step. A gate beyond
-// |z| = 110 is 0 or 1 within binary32 either way. This takes 30 vector operations, the functions of
+// unit in binary32's last place of either. The reciprocal's estimate takes one Newton step. A gate beyond
+// |z| = 700 leaves nothing of any binary32 state, or all of it, either way. This takes 30 vector operations, the functions of
 // fexp64.h, which serve an exactness that two further roundings make moot here, 45.
-__device__ __forceinline__ void gates(float z, float& f, float& k) {
-  const double x = -(double)clamp_f(z, -110.0f, 110.0f);
+__device__ __forceinline__ void gates(float z, double& f, float& k) {
+  const double x = -(double)clamp_f(z, -700.0f, 700.0f);
   const double kd = fma(x, 0x1.71547652b82fep+0, 0x1.8p52);  // n in the low half
   const double n = kd - 0x1.8p52;
   double r = fma(-n, 0x1.62e42fefa39efp-1, x);
@@ -47,20 +56,20 @@ __device__ __forceinline__ void gates(float z, float& f, float& k) {
   q = fma(q, r, 0.5);
   q = fma(q, r, 1.0);
   q = fma(q, r, 1.0);
-  // 2^n: n from -159 to 159, added to the exponent
+  // 2^n: n from -1010 to 1010, added to the exponent
   const uint32_t hi = (uint32_t)__double2hiint(q) + ((uint32_t)__double2loint(kd) << 20);
   const double e = __hiloint2double(z != z ? 0x7ff80000 : (int)hi, __double2loint(q)), d = 1.0 + e;
   double y = __builtin_amdgcn_rcp(d);
   y = fma(fma(-d, y, 1.0), y, y);
-  f = (float)y;
+  f = y;
   k = (float)(e * y);
 }
 
-// What bounds it: memory, if the 35 to 53 vector operations a position and channel (30 of them the gate) run beside the
+// What bounds it: memory, if the 36 to 55 vector operations a position and channel (30 of them the gate) run beside the
 // loads. So a wave's next positions are on their way while it works on these, addresses are the wave's
-// (a scalar base, a lane's offset), and nothing spills. [16, 4096, 1024] backward, 1.6 GB, takes 303 us in
-// one pass, 5.3 TB/s (lanes' own 64-bit addresses and spills: 2030 us); [1, 65536, 512] forward, 403 MB,
-// 49 us for the chunks' steps and 65 us for the pass, whose first reading the caches keep part of.
+// (a scalar base, a lane's offset), and nothing spills. [16, 4096, 1024] backward, 1.6 GB, takes 308 us in
+// one pass, 5.2 TB/s (lanes' own 64-bit addresses and spills: 2030 us); [1, 65536, 512] forward, 403 MB,
+// 51 us for the chunks' steps and 67 us for the pass, whose first reading the caches keep part of.
 enum Mode { WHOLE, STEPS, CHUNK };  // the one pass; a chunk's step alone; a chunk from its first state
 
 struct ScanArgs {
@@ -74,7 +83,7 @@ struct ScanArgs {
   float* last;          // [B, D]: the state behind the last step; null: not wanted
   const void* lengths;  // [B]; null: all T
   uint32_t* status;
-  float2* step;         // [chunks][B D]: the chunks' steps
+  double2* step;        // [chunks][B D]: the chunks' steps
   float* state;         // [B D]: a copy of the first states
   int64_t B, T, D, chunk, chunks;  // chunk: positions of one; chunks > 1: split
   int64_t waves, parts;  // groups of up to 64 channels: of all sequences, of one
@@ -96,7 +105,9 @@ __device__ __forceinline__ int64_t scan_length(const ScanArgs& a, int64_t b, boo
 template <bool BACK, int MODE, int NW, int CW, int TS, bool STREAM = false>
 __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
   constexpr int READS = !BACK || MODE == STEPS ? 2 : 4;  // z and u; z and dh; z, dh, u and h_{t-1}
-  __shared__ float2 steps[2][NW * CW][64];
+  static_assert(NW > 1 || MODE == WHOLE);
+  using F = std::conditional_t<NW == 1, double, float>;  // within a run (a wave by itself has one run)
+  __shared__ double2 steps[2][NW * CW][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tw = NW > 1 ? w : 0;
   const int64_t width = a.T * a.D;  // floats of a sequence
@@ -150,7 +161,7 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
         const bool in = live && p < hi && p >= from && p < to;
 #pragma unroll
         for (int r = 0; r < READS; ++r) {
-          next[r][i] = 0.0f;
+          next[r][i] = r == 0 ? INFINITY : 0.0f;  // a position that is not there holds the state
           if (in) {
             if (r < 3 || p < T - 1) next[r][i] = get(row(src[r], p) - (r == 3 ? a.D : 0));
             else next[r][i] = a.h0 != nullptr ? a.h0[n] : 0.0f;
@@ -159,77 +170,77 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
       }
     };
 
-    float state = 0.0f, all = 1.0f;
-    if (MODE == WHOLE) state = a.first != nullptr ? a.first[n] : 0.0f;
+    double state = 0.0, all = 1.0;
+    if (MODE == WHOLE) state = a.first != nullptr ? (double)a.first[n] : 0.0;
     load(lo + tw * TS);
     int turn = 0;
     if (MODE == CHUNK) {
       // the steps of the chunks before: each wave joins consecutive ones, all join the waves'
-      state = a.state[n];
+      state = (double)a.state[n];
       const int64_t share = (piece + NW - 1) / NW, end = min(piece, (tw + 1) * share);
-      float run_f = 1.0f, run_b = 0.0f;
-#pragma unroll 8
+      double run_f = 1.0, run_b = 0.0;
+#pragma unroll 4
       for (int64_t i = min(piece, tw * share); i < end; ++i) {
-        const float2 g = a.step[i * a.B * a.D + n];
-        run_b = fmaf(g.x, run_b, g.y);
+        const double2 g = a.step[i * a.B * a.D + n];
+        run_b = fma(g.x, run_b, g.y);
         run_f *= g.x;
       }
-      steps[turn][w][lane] = make_float2(run_f, run_b);
+      steps[turn][w][lane] = make_double2(run_f, run_b);
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < NW; ++j) {
-        const float2 g = steps[turn][j][lane];
-        state = fmaf(g.x, state, g.y);
+        const double2 g = steps[turn][j][lane];
+        state = fma(g.x, state, g.y);
       }
       turn ^= 1;
     }
     for (int p0 = lo; p0 < hi; p0 += NW * TS, turn ^= 1) {
       const int q0 = p0 + tw * TS;
-      float f[TS], b[TS], k[TS], v[TS], m[TS];
+      F f[TS], b[TS], k[TS], v[TS], m[TS];
+      double run_f = 1.0;
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
-        gates(next[0][i], f[i], k[i]);
+        double gate;
+        float let;
+        gates(next[0][i], gate, let);
+        f[i] = (F)gate;
+        k[i] = (F)let;
+        run_f *= gate;
         if (BACK) {
-          v[i] = next[1][i];
-          if (MODE != STEPS) m[i] = (next[3][i] - next[2][i]) * (f[i] * k[i]);
+          v[i] = (F)next[1][i];
+          if (MODE != STEPS) m[i] = ((F)next[3][i] - (F)next[2][i]) * (f[i] * k[i]);
         } else {
-          b[i] = k[i] * next[1][i];
+          b[i] = k[i] * (F)next[1][i];
         }
         __builtin_amdgcn_sched_barrier(0);  // one gate's binary64 values at a time
       }
       const bool inside = whole(q0);
-      if (!inside) {
+      // (what these are without: z = inf, the rest 0. Forming them apart keeps the registers below 128.)
+      if (BACK && MODE != STEPS && !inside) {
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
           const bool in = q0 + i < hi && q0 + i >= from && q0 + i < to;
-          f[i] = in ? f[i] : 1.0f;
-          if (!BACK) b[i] = in ? b[i] : 0.0f;
-          else if (MODE != STEPS) m[i] = in ? m[i] : 0.0f;
-          if (BACK) { k[i] = in ? k[i] : 0.0f; v[i] = in ? v[i] : 0.0f; }
+          f[i] = in ? f[i] : (F)1;
+          m[i] = in ? m[i] : (F)0;
+          k[i] = in ? k[i] : (F)0;
+          v[i] = in ? v[i] : (F)0;
         }
       }
       if (p0 + NW * TS < hi) load(q0 + NW * TS);
-      float s = state;
-      if (NW > 1 || MODE == STEPS) {
-        float run_f = 1.0f, run_b = 0.0f;
+      F s = (F)state;
+      if (NW > 1) {
+        F run_b = 0;
 #pragma unroll
-        for (int i = 0; i < TS; ++i) {
-          run_b = BACK ? f[i] * (run_b + v[i]) : fmaf(f[i], run_b, b[i]);
-          run_f *= f[i];
-        }
-        if (NW > 1) {
-          steps[turn][w][lane] = make_float2(run_f, run_b);
-          __syncthreads();
-#pragma unroll
-          for (int j = 0; j < NW; ++j) {
-            const float2 g = steps[turn][j][lane];
-            if (j == tw) s = state;
-            state = fmaf(g.x, state, g.y);
-            all *= g.x;
-          }
-        } else {
-          state = fmaf(run_f, state, run_b);
-          all *= run_f;
+        for (int i = 0; i < TS; ++i) run_b = BACK ? f[i] * (run_b + v[i]) : fma(f[i], run_b, b[i]);
+        steps[turn][w][lane] = make_double2(run_f, (double)run_b);
+        __syncthreads();
+        if (MODE == STEPS && tw != 0) continue;  // (one wave keeps the chunk's step)
+#pragma unroll 4  // (all at once take 32 more registers)
+        for (int j = 0; j < NW; ++j) {
+          const double2 g = steps[turn][j][lane];
+          if (j == tw) s = (F)state;
+          state = fma(g.x, state, g.y);
+          all *= g.x;
         }
       }
       if (MODE != STEPS && live) {
@@ -238,26 +249,26 @@ __global__ void __launch_bounds__(64 * NW * CW) scan_kernel(ScanArgs a) {
         for (int i = 0; i < TS; ++i, x[0] += dir, x[1] += BACK ? dir : 0) {
           if (q0 + i >= hi) break;
           if (BACK) {
-            const float g = v[i] + s;
-            float dz = g * m[i], du = g * k[i];
+            const F g = v[i] + s;
+            float dz = (float)(g * m[i]), du = (float)(g * k[i]);
             if (!inside && q0 + i < from) dz = du = 0.0f;  // (a gradient that is not finite stays at the end)
             put(x[0], dz);
             put(x[1], du);
             s = f[i] * g;
           } else {
-            s = fmaf(f[i], s, b[i]);
-            put(x[0], q0 + i < to ? s : 0.0f);
+            s = fma(f[i], s, b[i]);
+            put(x[0], q0 + i < to ? (float)s : 0.0f);
           }
         }
       }
-      if (NW == 1 && MODE != STEPS) state = s;
+      if (NW == 1) state = s;
     }
     if (tw == 0 && live) {
       if (MODE == STEPS) {
-        a.step[piece * a.B * a.D + n] = make_float2(all, state);
+        a.step[piece * a.B * a.D + n] = make_double2(all, state);
         if (piece == 0) a.state[n] = a.first != nullptr ? a.first[n] : 0.0f;
       } else if (piece == a.chunks - 1 && a.last != nullptr) {
-        a.last[n] = state;  // (which may be `first`: the chunks read its copy)
+        a.last[n] = (float)state;  // (which may be `first`: the chunks read its copy)
       }
     }
     if (NW > 1) __syncthreads();  // the steps in LDS have been read
@@ -277,7 +288,7 @@ int64_t scan_waves(int64_t B, int64_t T, int64_t D) {
 }
 // Positions of a chunk: all of them from SCAN_SPLIT groups of channels on, where the one pass takes
 // no longer than two, whose first reads again two thirds (forward) or a third of what the pass moves:
-// [8, 4096, 1024], 128 groups, takes 119 us forward and 198 back in one, 114 and 204 us in two. Else as
+// a call of [8, 4096, 1024], 128 groups, takes 133 us forward and 203 back in one, 134 and 219 in two. Else as
 // many chunks as the CUs hold workgroups at once, three each forward and two back.
 constexpr int64_t SCAN_SPLIT = 128, SCAN_LEAST = 128, SCAN_TILE = 64;
 int64_t scan_chunk(int64_t B, int64_t T, int64_t D, bool back) {
@@ -288,7 +299,7 @@ int64_t scan_chunk(int64_t B, int64_t T, int64_t D, bool back) {
 }
 int64_t scan_bytes(int64_t B, int64_t T, int64_t D, bool back) {
   const int64_t chunk = scan_chunk(B, T, D, back), chunks = (T + chunk - 1) / chunk;
-  return chunks > 1 ? 4 * (2 * chunks + 1) * B * D : 0;
+  return chunks > 1 ? 4 * (4 * chunks + 1) * B * D : 0;
 }
 
 template <bool BACK>
@@ -309,8 +320,8 @@ hipError_t launch_scan(ScanArgs a, float* scratch, hipStream_t s) {
   // What the chunks' first reading takes stays there for the second.
   const bool lines = a.D % 32 == 0 && (BACK ? 24 : 12) * channels * a.T > 256 << 20;
   if (a.chunks > 1) {
-    a.step = reinterpret_cast<float2*>(scratch);
-    a.state = scratch + 2 * a.chunks * channels;
+    a.step = reinterpret_cast<double2*>(scratch);
+    a.state = scratch + 4 * a.chunks * channels;
     hipLaunchKernelGGL((scan_kernel<BACK, STEPS, 8, 1, TS>), blocks(1), dim3(512), 0, s, a);
     if (lines) hipLaunchKernelGGL((scan_kernel<BACK, CHUNK, 8, 1, TS, true>), blocks(1), dim3(512), 0, s, a);
     else hipLaunchKernelGGL((scan_kernel<BACK, CHUNK, 8, 1, TS>), blocks(1), dim3(512), 0, s, a);
