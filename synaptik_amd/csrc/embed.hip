@@ -598,27 +598,37 @@ __global__ void __launch_bounds__(256) eg_join(SumArgs a) {
 
 int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
-// What embed_grad keeps: two lists of keys and rows, digit counts, parts of sums.
+// Digits of the keys 0 .. V.
+int key_digits(int64_t V) {
+  int n = 1;
+  while (n * EG_BITS < 32 && (V >> (n * EG_BITS)) != 0) ++n;
+  return n;
+}
+// What embed_grad keeps, for more rows than EG_DIRECT: a list of keys and rows, a second one where a sort
+// goes from one to the other, with its digit counts; flags where rows are cleared; parts of sums.
 struct Layout {
   int64_t keys[2], rows[2], count, flags, part, bytes;
 };
 // Sorted rows that a wave sums: 32, or 8 where that leaves fewer than eight waves for each CU.
 int64_t tile_rows(int64_t N, int64_t D) { return (N + 31) / 32 * ((D + 255) / 256) < 2048 ? 8 : 32; }
-Layout layout(int64_t N, int64_t V, int64_t D) {
-  const int64_t sort = (N + EG_SORT - 1) / EG_SORT, rows = tile_rows(N, D), tiles = (N + rows - 1) / rows;
+Layout layout(int64_t N, int64_t V, int64_t D, bool accumulate) {
   Layout l{};
+  if (N <= EG_DIRECT || V <= 0 || D <= 0) return l;
+  const int64_t sort = (N + EG_SORT - 1) / EG_SORT, rows = tile_rows(N, D), tiles = (N + rows - 1) / rows;
   int64_t off = 0;
   auto take = [&](int64_t bytes) {
     const int64_t at = off;
     off += round16(bytes);
     return at;
   };
+  const bool launches = N > EG_SMALL;  // one for each digit's counts, one for its places
   for (int i = 0; i < 2; ++i) {
-    l.keys[i] = take(4 * N);
-    l.rows[i] = take(4 * N);
+    const int64_t n = i == 0 || (launches && key_digits(V) > 1) ? N : 0;
+    l.keys[i] = take(4 * n);
+    l.rows[i] = take(4 * n);
   }
-  l.count = take(4 * (sort + 1) * EG_BINS);
-  l.flags = take(V <= EG_FLAGS ? V : 0);
+  l.count = take(launches ? 4 * (sort + 1) * EG_BINS : 0);
+  l.flags = take(!accumulate && V <= EG_FLAGS ? V : 0);
   l.part = take(tiles > 1 ? 16 * tiles * D : 0);
   l.bytes = off;
   return l;
@@ -646,20 +656,21 @@ hipError_t launch_embed(const EmbedParams& p, uint32_t* status, hipStream_t s) {
   return hipGetLastError();
 }
 
-int64_t embed_grad_scratch_bytes(int64_t N, int64_t V, int64_t D) { return layout(N, V, D).bytes; }
+int64_t embed_grad_scratch_bytes(int64_t N, int64_t V, int64_t D, bool accumulate) {
+  return layout(N, V, D, accumulate).bytes;
+}
 
 hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* status, hipStream_t s) {
   if (p.V <= 0 || p.D <= 0 || (p.N <= 0 && p.accumulate)) return hipSuccess;
   const Tokens t = tokens_of(p, status);
-  const Layout l = layout(p.N, p.V, p.D);
+  const Layout l = layout(p.N, p.V, p.D, p.accumulate != 0);
   char* base = static_cast<char*>(scratch);
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(base + l.keys[0]), reinterpret_cast<uint32_t*>(base + l.keys[1])};
   uint32_t* rows[2] = {reinterpret_cast<uint32_t*>(base + l.rows[0]), reinterpret_cast<uint32_t*>(base + l.rows[1])};
   uint32_t* count = reinterpret_cast<uint32_t*>(base + l.count);
   // (rows are cleared here only where the table's gradient is not added to)
   uint8_t* flags = !p.accumulate && p.V <= EG_FLAGS ? reinterpret_cast<uint8_t*>(base + l.flags) : nullptr;
-  int passes = 1;  // digits of the keys 0 .. V
-  while (passes * EG_BITS < 32 && (p.V >> (passes * EG_BITS)) != 0) ++passes;
+  const int passes = key_digits(p.V);
   int at = 0;
   SumArgs a{};
   a.dy = p.w;

@@ -341,9 +341,8 @@ hipError_t launch_scan(ScanArgs a, float* scratch, hipStream_t s) {
 
 }  // namespace
 
-int64_t gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D) {
-  if (B <= 0 || T <= 0 || D <= 0) return 0;
-  return std::max(scan_bytes(B, T, D, false), scan_bytes(B, T, D, true));
+int64_t gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D, bool back) {
+  return B <= 0 || T <= 0 || D <= 0 ? 0 : scan_bytes(B, T, D, back);
 }
 
 hipError_t launch_gated_scan(const GatedScanParams& p, float* scratch, uint32_t* status, hipStream_t s) {

@@ -291,7 +291,7 @@ struct EmbedParams {
 };
 hipError_t launch_embed(const EmbedParams& p, uint32_t* status, hipStream_t s);
 hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* status, hipStream_t s);
-int64_t embed_grad_scratch_bytes(int64_t N, int64_t V, int64_t D);
+int64_t embed_grad_scratch_bytes(int64_t N, int64_t V, int64_t D, bool accumulate);
 
 // Layer norm over the last axis (layer_norm.hip): y [R, C] from x [R, C]; gamma, beta [C] may be null.
 // y may be x with the same row stride.
@@ -316,7 +316,7 @@ struct LayerNormGradParams {
   float eps;
 };
 hipError_t launch_layer_norm_grad(const LayerNormGradParams& p, double* scratch, hipStream_t s);
-int64_t layer_norm_grad_scratch_bytes(int64_t R, int64_t C);
+int64_t layer_norm_grad_scratch_bytes(int64_t R, int64_t C);  // (none without dgamma and dbeta)
 
 // Gated linear recurrence of sequences [B, T, D] (gated_scan.hip): h from the gates' inputs z, the
 // inputs u and the first states h0 [B, D] (null: zero); last [B, D] (null: not wanted) may be h0.
@@ -348,7 +348,7 @@ struct GatedScanGradParams {
   int len64;
 };
 hipError_t launch_gated_scan_grad(const GatedScanGradParams& p, float* scratch, uint32_t* status, hipStream_t s);
-int64_t gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D);
+int64_t gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D, bool back);
 
 // Divergence from a teacher's K largest logits of each row (distill.hip), and its gradient (null: not
 // wanted).

@@ -596,7 +596,7 @@ int32_t validate_token_step(Validator& v, size_t idx, const Step& st, uint64_t* 
       if (!apart(s[2], {s[0], s[1]})) return aliases(grad ? table : row);
       if (grad) {
         // (16 bytes for each column of every 8th row at most, below 2^63 with N rows of D held above)
-        need(shk::embed_grad_scratch_bytes(N, V, D));
+        need(shk::embed_grad_scratch_bytes(N, V, D, a[7] != 0));
       }
       return SHK_HIP_STATUS_OK;
     }
@@ -630,7 +630,7 @@ int32_t validate_token_step(Validator& v, size_t idx, const Step& st, uint64_t* 
       if (!apart(s[3], {s[1], s[2], s[4], s[5]}) || (s[3] == s[0] && lddy != lddx)) return aliases("dX");
       if (!apart(s[4], {s[0], s[1], s[2], s[5]})) return aliases("dgamma");
       if (!apart(s[5], {s[0], s[1], s[2]})) return aliases("dbeta");
-      need(shk::layer_norm_grad_scratch_bytes(R, C));
+      if (s[4] >= 0 || s[5] >= 0) need(shk::layer_norm_grad_scratch_bytes(R, C));
       return SHK_HIP_STATUS_OK;
     }
     case OP_GATED_SCAN: case OP_GATED_SCAN_GRAD: {
@@ -675,7 +675,7 @@ int32_t validate_token_step(Validator& v, size_t idx, const Step& st, uint64_t* 
         if (!apart(s[7], {s[0], s[1], s[2], s[3], s[4], s[5], e.dh0, e.lengths})) return aliases("dU");
         if (!apart(e.dh0, {s[0], s[1], s[2], s[3], s[4], e.lengths})) return aliases("dh0");
       }
-      need(shk::gated_scan_scratch_bytes(B, T, D));
+      need(shk::gated_scan_scratch_bytes(B, T, D, grad));
       return SHK_HIP_STATUS_OK;
     }
     default: {  // OP_DISTILL
