@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "flag.h"
 #include "kernels.h"
 #include "row4.h"
 #include "rowvec.h"
@@ -35,7 +36,7 @@ struct DistillArgs {
   float* grad;           // null: the loss alone
   float* row_loss;       // [R]
   const uint32_t* count; // [parts]: rows that have an entry; null: counted here
-  uint32_t* status;
+  FlagWord flag;
   int64_t R, C;
   int K, is64, parts, slots, shift;
   float per_T;           // log2(e) / T
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
       const int64_t i = entry_index(a, r * a.K + j);
       const float t = a.t[r * a.K + j];
       const bool inside = i >= 0 && i < a.C;
-      if (!inside && i != -1) atomicOr(a.status, (uint32_t)DEV_INDEX_OUT_OF_BOUNDS);
+      if (!inside && i != -1) flag_out_of_bounds(a.flag);
       const bool there = inside && t != -INFINITY;
       index[j] = there ? (int)i : -1;
       any |= there;
@@ -332,7 +333,7 @@ void launch_groups(const DistillArgs& a, hipStream_t s) {
 
 int64_t distill_scratch_bytes(int64_t R) { return 4 * ((R + 3) / 4 * 4) + 4 * COUNT_PARTS; }
 
-hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* status, hipStream_t s) {
+hipError_t launch_distill(const DistillParams& p, void* scratch, FlagWord flag, hipStream_t s) {
   if (p.R <= 0) return hipSuccess;
   DistillArgs a{};
   a.z = p.logits;
@@ -340,7 +341,7 @@ hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* statu
   a.t = p.teacher;
   a.grad = p.grad;
   a.row_loss = static_cast<float*>(scratch);
-  a.status = status;
+  a.flag = flag;
   a.R = p.R;
   a.C = p.C;
   a.K = (int)p.K;

@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "flag.h"
 #include "kernels.h"
 #include "row4.h"
 
@@ -27,12 +28,12 @@ struct Tokens {
   const void* t;
   int64_t N, V, pad;
   int is64, has_pad;
-  uint32_t* status;
-  __device__ __forceinline__ uint32_t key(int64_t n, bool flag) const {
+  FlagWord flag;
+  __device__ __forceinline__ uint32_t key(int64_t n, bool flags) const {
     const int64_t v = is64 ? static_cast<const int64_t*>(t)[n] : (int64_t) static_cast<const int32_t*>(t)[n];
     if (has_pad && v == pad) return (uint32_t)V;
     if (v >= 0 && v < V) return (uint32_t)v;
-    if (flag) atomicOr(status, (uint32_t)DEV_INDEX_OUT_OF_BOUNDS);
+    if (flags) flag_out_of_bounds(flag);
     return (uint32_t)V;
   }
 };
@@ -634,15 +635,15 @@ Layout layout(int64_t N, int64_t V, int64_t D, bool accumulate) {
   return l;
 }
 
-Tokens tokens_of(const EmbedParams& p, uint32_t* status) {
-  return Tokens{p.tokens, p.N, p.V, p.pad, p.is64, p.has_pad, status};
+Tokens tokens_of(const EmbedParams& p, FlagWord flag) {
+  return Tokens{p.tokens, p.N, p.V, p.pad, p.is64, p.has_pad, flag};
 }
 
 }  // namespace
 
-hipError_t launch_embed(const EmbedParams& p, uint32_t* status, hipStream_t s) {
+hipError_t launch_embed(const EmbedParams& p, FlagWord flag, hipStream_t s) {
   if (p.N <= 0 || p.D <= 0) return hipSuccess;
-  const Tokens t = tokens_of(p, status);
+  const Tokens t = tokens_of(p, flag);
   // lanes for a row's groups of four; four rows at once where there are enough for every CU
   const bool many = (double)p.N * (double)p.D >= (double)(1 << 20);
   auto go = [&](auto lanes) {
@@ -660,9 +661,9 @@ int64_t embed_grad_scratch_bytes(int64_t N, int64_t V, int64_t D, bool accumulat
   return layout(N, V, D, accumulate).bytes;
 }
 
-hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* status, hipStream_t s) {
+hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, FlagWord flag, hipStream_t s) {
   if (p.V <= 0 || p.D <= 0 || (p.N <= 0 && p.accumulate)) return hipSuccess;
-  const Tokens t = tokens_of(p, status);
+  const Tokens t = tokens_of(p, flag);
   const Layout l = layout(p.N, p.V, p.D, p.accumulate != 0);
   char* base = static_cast<char*>(scratch);
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(base + l.keys[0]), reinterpret_cast<uint32_t*>(base + l.keys[1])};

@@ -29,6 +29,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "flag.h"
 #include "kernels.h"
 
 namespace shk {
@@ -82,7 +83,7 @@ struct ScanArgs {
   float* out[2];        // forward: h; backward: dz, du
   float* last;          // [B, D]: the state behind the last step; null: not wanted
   const void* lengths;  // [B]; null: all T
-  uint32_t* status;
+  FlagWord flag;
   double2* step;        // [chunks][B D]: the chunks' steps
   float* state;         // [B D]: a copy of the first states
   int64_t B, T, D, chunk, chunks;  // chunk: positions of one; chunks > 1: split
@@ -91,12 +92,12 @@ struct ScanArgs {
   int len64;
 };
 
-__device__ __forceinline__ int64_t scan_length(const ScanArgs& a, int64_t b, bool flag) {
+__device__ __forceinline__ int64_t scan_length(const ScanArgs& a, int64_t b, bool flags) {
   if (a.lengths == nullptr) return a.T;
   const int64_t n = a.len64 ? static_cast<const int64_t*>(a.lengths)[b]
                             : (int64_t) static_cast<const int32_t*>(a.lengths)[b];
   if (n < 0 || n > a.T) {
-    if (flag) atomicOr(a.status, (uint32_t)DEV_INDEX_OUT_OF_BOUNDS);
+    if (flags) flag_out_of_bounds(a.flag);
     return n < 0 ? 0 : a.T;
   }
   return n;
@@ -345,7 +346,7 @@ int64_t gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D, bool back) {
   return B <= 0 || T <= 0 || D <= 0 ? 0 : scan_bytes(B, T, D, back);
 }
 
-hipError_t launch_gated_scan(const GatedScanParams& p, float* scratch, uint32_t* status, hipStream_t s) {
+hipError_t launch_gated_scan(const GatedScanParams& p, float* scratch, FlagWord flag, hipStream_t s) {
   if (p.B <= 0 || p.D <= 0) return hipSuccess;
   ScanArgs a{};
   a.z = p.z;
@@ -355,14 +356,14 @@ hipError_t launch_gated_scan(const GatedScanParams& p, float* scratch, uint32_t*
   a.last = p.last;
   a.lengths = p.lengths;
   a.len64 = p.len64;
-  a.status = status;
+  a.flag = flag;
   a.B = p.B;
   a.T = p.T;
   a.D = p.D;
   return launch_scan<false>(a, scratch, s);
 }
 
-hipError_t launch_gated_scan_grad(const GatedScanGradParams& p, float* scratch, uint32_t* status, hipStream_t s) {
+hipError_t launch_gated_scan_grad(const GatedScanGradParams& p, float* scratch, FlagWord flag, hipStream_t s) {
   if (p.B <= 0 || p.D <= 0) return hipSuccess;
   ScanArgs a{};
   a.z = p.z;
@@ -376,7 +377,7 @@ hipError_t launch_gated_scan_grad(const GatedScanGradParams& p, float* scratch, 
   a.last = p.dh0;
   a.lengths = p.lengths;
   a.len64 = p.len64;
-  a.status = status;
+  a.flag = flag;
   a.B = p.B;
   a.T = p.T;
   a.D = p.D;

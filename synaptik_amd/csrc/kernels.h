@@ -278,6 +278,13 @@ struct MxLinearParams {
 hipError_t launch_mx_linear(const MxLinearParams& p, void* scratch, hipStream_t s);
 int64_t mx_linear_scratch_bytes(int64_t M, int64_t N, int64_t K);
 
+// Where a step flags an index out of bounds (flag.h): a run's status word, or a word of host memory in runs
+// whose steps flag nothing else.
+struct FlagWord {
+  uint32_t* word;
+  int host;
+};
+
 // Rows of a table [V, D] by token (embed.hip): y [N, D] (row stride ldy) = scale * w[token], zero at the
 // padding token. The gradient reads dy in w's place, with row stride ldy, and writes the table's
 // gradient [V, D] to y, or adds to it.
@@ -289,8 +296,8 @@ struct EmbedParams {
   int is64, has_pad, accumulate;
   float scale;
 };
-hipError_t launch_embed(const EmbedParams& p, uint32_t* status, hipStream_t s);
-hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, uint32_t* status, hipStream_t s);
+hipError_t launch_embed(const EmbedParams& p, FlagWord flag, hipStream_t s);
+hipError_t launch_embed_grad(const EmbedParams& p, void* scratch, FlagWord flag, hipStream_t s);
 int64_t embed_grad_scratch_bytes(int64_t N, int64_t V, int64_t D, bool accumulate);
 
 // Layer norm over the last axis (layer_norm.hip): y [R, C] from x [R, C]; gamma, beta [C] may be null.
@@ -330,7 +337,7 @@ struct GatedScanParams {
   int64_t B, T, D;
   int len64;
 };
-hipError_t launch_gated_scan(const GatedScanParams& p, float* scratch, uint32_t* status, hipStream_t s);
+hipError_t launch_gated_scan(const GatedScanParams& p, float* scratch, FlagWord flag, hipStream_t s);
 // Gradients of z, u and h0 from those of h and of the last state (dlast; null: zero); dh0 (null: not
 // wanted) may be dlast.
 struct GatedScanGradParams {
@@ -347,7 +354,7 @@ struct GatedScanGradParams {
   int64_t B, T, D;
   int len64;
 };
-hipError_t launch_gated_scan_grad(const GatedScanGradParams& p, float* scratch, uint32_t* status, hipStream_t s);
+hipError_t launch_gated_scan_grad(const GatedScanGradParams& p, float* scratch, FlagWord flag, hipStream_t s);
 int64_t gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D, bool back);
 
 // Divergence from a teacher's K largest logits of each row (distill.hip), and its gradient (null: not
@@ -363,7 +370,7 @@ struct DistillParams {
   int is64;
   float T, g;
 };
-hipError_t launch_distill(const DistillParams& p, void* scratch, uint32_t* status, hipStream_t s);
+hipError_t launch_distill(const DistillParams& p, void* scratch, FlagWord flag, hipStream_t s);
 int64_t distill_scratch_bytes(int64_t R);
 
 // Y[C,R] = X[R,C]^T
