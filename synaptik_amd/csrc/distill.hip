@@ -36,7 +36,7 @@ struct DistillArgs {
   float* grad;           // null: the loss alone
   float* row_loss;       // [R]
   const uint32_t* count; // [parts]: rows that have an entry; null: counted here
-  FlagWord flag;
+  uint32_t* status;
   int64_t R, C;
   int K, is64, parts, slots, shift;
   float per_T;           // log2(e) / T
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
       const int64_t i = entry_index(a, r * a.K + j);
       const float t = a.t[r * a.K + j];
       const bool inside = i >= 0 && i < a.C;
-      if (!inside && i != -1) flag_out_of_bounds(a.flag);
+      if (!inside && i != -1) atomicOr(a.status, (uint32_t)DEV_INDEX_OUT_OF_BOUNDS);
       const bool there = inside && t != -INFINITY;
       index[j] = there ? (int)i : -1;
       any |= there;
@@ -297,9 +297,9 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) di
   }
 }
 
-// The loss: binary64 sum of the row losses, over the number of rows that have one.
+// The loss: binary64 sum of the row losses, over the number of rows that have one. Hands on the flag.
 __global__ void __launch_bounds__(1024) distill_finish(const float* __restrict__ row_loss, int64_t R, double T2,
-                                                       float* loss) {
+                                                       float* loss, FlagWord flag) {
   __shared__ double lds[2][16];
   double s = 0.0, n = 0.0;
 #pragma unroll 4
@@ -310,7 +310,10 @@ __global__ void __launch_bounds__(1024) distill_finish(const float* __restrict__
   }
   double v[2] = {s, n};
   group_sums<1024, 2>(v, &lds[0][0]);
-  if (threadIdx.x == 0) loss[0] = (float)(v[0] * T2 / v[1]);
+  if (threadIdx.x == 0) {
+    loss[0] = (float)(v[0] * T2 / v[1]);
+    hand_on(flag);
+  }
 }
 
 constexpr int COUNT_PARTS = 64;
@@ -341,7 +344,7 @@ hipError_t launch_distill(const DistillParams& p, void* scratch, FlagWord flag, 
   a.t = p.teacher;
   a.grad = p.grad;
   a.row_loss = static_cast<float*>(scratch);
-  a.flag = flag;
+  a.status = flag.status;
   a.R = p.R;
   a.C = p.C;
   a.K = (int)p.K;
@@ -370,7 +373,7 @@ hipError_t launch_distill(const DistillParams& p, void* scratch, FlagWord flag, 
   else if (p.C <= 1024 * 4 * 16) launch_groups<1024, 9, 16>(a, s);
   else launch_rows<1024, 0>(a, s);
   hipLaunchKernelGGL(distill_finish, dim3(1), dim3(1024), 0, s, (const float*)a.row_loss, p.R,
-                     (double)p.T * (double)p.T, p.loss);
+                     (double)p.T * (double)p.T, p.loss, flag);
   return hipGetLastError();
 }
 

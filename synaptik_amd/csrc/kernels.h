@@ -279,10 +279,10 @@ hipError_t launch_mx_linear(const MxLinearParams& p, void* scratch, hipStream_t 
 int64_t mx_linear_scratch_bytes(int64_t M, int64_t N, int64_t K);
 
 // Where a step flags an index out of bounds (flag.h): a run's status word, or a word of host memory in runs
-// whose steps flag nothing else.
+// whose steps flag nothing else (null in others).
 struct FlagWord {
-  uint32_t* word;
-  int host;
+  uint32_t* status;
+  uint32_t* host;
 };
 
 // Rows of a table [V, D] by token (embed.hip): y [N, D] (row stride ldy) = scale * w[token], zero at the

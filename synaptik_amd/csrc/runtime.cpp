@@ -1507,7 +1507,7 @@ hipError_t enqueue_steps(const Program& pr, Lease& ls, const Bound& b, hipStream
   if (n > 0 && pr.steps[n - 1].rec.opcode == OP_STEP_COMMIT)
     commit = b.get<int64_t>(pr.steps[n - 1].rec.slot[0]);
   const size_t launched = commit != nullptr ? n - 1 : n;
-  const shk::FlagWord flag{pr.host_flags ? ls.host_status : ls.status, pr.host_flags ? 1 : 0};
+  const shk::FlagWord flag{ls.status, pr.host_flags ? ls.host_status : nullptr};
   // folded steps go into the run's last launch (not in profiled runs: their per-step events
   // bracket every step's own launch)
   auto skipped = [&](size_t j) { return !profile && pr.folded(j); };

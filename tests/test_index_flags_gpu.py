@@ -154,3 +154,25 @@ def test_programs_whose_steps_launch_nothing(ctx, N, D):
         prog.run(ins, outs)
         prog.run_static(ins, outs)
     prog.close()
+
+
+@pytest.mark.parametrize("bad", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("concurrent", [False, True])
+def test_two_steps_of_one_program(ctx, bad, concurrent):
+    """Either step's flag is reported, also where the two run beside each other; it is gone in the next run."""
+    R, C = 50, 3000
+    pb = ProgramBuilder()
+    ins, outs = [], []
+    for _ in range(2):
+        ins += [pb.input(R * C), pb.input(R, "i32"), pb.input(R)]
+        outs += [pb.output(1), pb.output(R * C)]
+        pb.distill(*ins[-3:], outs[-2], R, C, 1, grad=outs[-1])
+    prog = HipProgram(ctx, pb.image())
+    prog.set_concurrent(concurrent)
+    good, wrong = (ctx.upload(np.full(R, v, np.int32)) for v in (C - 1, C))
+    z, t = ctx.upload(np.zeros(R * C, np.float32)), ctx.upload(np.zeros(R, np.float32))
+    bo = [ctx.buffer(s.nbytes) for s in outs]
+    for _ in range(10):
+        expect(not any(bad), lambda: prog.run([z, wrong if bad[0] else good, t, z, wrong if bad[1] else good, t], bo))
+        prog.run([z, good, t, z, good, t], bo)
+    prog.close()
