@@ -66,7 +66,7 @@ __device__ __forceinline__ void gates(float z, double& f, float& k) {
   k = (float)(e * y);
 }
 
-// What bounds it: memory, if the 36 to 55 vector operations a position and channel (30 of them the gate) run beside the
+// What bounds it: memory, if the 37 to 54 vector operations a position and channel (30 of them the gate) run beside the
 // loads. So a wave's next positions are on their way while it works on these, addresses are the wave's
 // (a scalar base, a lane's offset), and nothing spills. [16, 4096, 1024] backward, 1.6 GB, takes 308 us in
 // one pass, 5.2 TB/s (lanes' own 64-bit addresses and spills: 2030 us); [1, 65536, 512] forward, 403 MB,
