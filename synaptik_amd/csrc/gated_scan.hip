@@ -19,7 +19,7 @@
 // is handed from run to run: binary32 is what happens within the TS positions of one run, each run's result
 // from s = 0, and the outputs. With z from 6 to 12 and u constant, begun with the state u, h was off by up to
 // 8e-5 of u after 2048 positions and 1.3e-3 after 65536 with binary32 throughout, and is off by 2e-7. That
-// costs 0 to 4 % of the time. (A call of up to 8 positions has no runs to join and is binary64 throughout;
+// costs 0 to 5 % of the time. (A call of up to 8 positions has no runs to join and is binary64 throughout;
 // from call to call states are the binary32 values in memory.)
 //
 // A sequence shorter than T holds its state behind its end (z = inf there: f = 1, 1 - f = 0): its last

@@ -396,8 +396,10 @@ class ProgramBuilder:
         the sequences into `last` [B, D], which may be h0: with T = 1 that moves a server's requests
         on by a token. (Sequences stored position by position, [T, B, D], are one of width B D.)
 
-        A run that fails has moved states in place on all the same: a caller that repeats failed runs
-        gives `last` a buffer of its own and exchanges the two after success.
+        Over any number of a call's positions a state is off by at most 52 2^-24 (to first order) of the
+        sizes of the terms that it sums. A run that fails has moved states in place on all the same: a
+        caller that repeats failed runs gives `last` a buffer of its own and exchanges the two after
+        success.
 
         lengths [B] (i32 or i64) are the positions that each sequence has: those behind are not
         read, H is zero there, and `last` is the state at the end, h0 for a length of zero. A length
